@@ -142,6 +142,31 @@ int sdh_gemm_nt_bf16(int64_t M, int64_t N, int64_t K, const float* A, int64_t ld
 int sdh_linear_swiglu(const float* x, const uint16_t* w1, const uint16_t* w3, float* y, int64_t rows, int64_t in,
                       int64_t hidden);
 
+/* ---- low-rank adapters (no counterpart in the reference) ------------------ */
+/* C[t, :] += scale[a] (X[t, :] A_a^T) B_a^T (without accumulate: = that) for the
+ * rows t of each run of rows, a its adapter: beside a projection of the same X
+ * that all rows share (sdh_gemm_nt_*, before it with accumulate, or after it with
+ * the projection accumulating). X [M, K] and C [M, N] fp32, leading dimensions in
+ * elements; A [adapters, rank, K] and B [adapters, N, rank] bf16, dense; scale
+ * [adapters] or NULL for ones; rank at most 1024. segments [count, 4] int32 on
+ * the device, 16-byte aligned: a run's first row, its rows, its adapter, and how
+ * many of the adapter's ranks count (rows of A_a and columns of B_a from there on
+ * are not read as numbers). A run with no such adapter (-1) or rank 0 adds
+ * nothing: its rows are left, or zero without accumulate. Runs must not share
+ * rows; entries past the matrix are cut to it; rows of no run are left as they
+ * were. Everything is held in fp32, X unrounded. C must not overlap an input. */
+int sdh_lora_nt_bf16(int64_t M, int64_t N, int64_t K, const float* X, int64_t ldx, const uint16_t* A,
+                     const uint16_t* B, int64_t rank, int64_t adapters, const float* scale, const int32_t* segments,
+                     int64_t count, float* C, int64_t ldc, int accumulate);
+/* As sdh_lora_nt_bf16, X bf16 (the operand of sdh_gemm_nt_bf16_packed). */
+int sdh_lora_nt_bf16_packed(int64_t M, int64_t N, int64_t K, const uint16_t* X, int64_t ldx, const uint16_t* A,
+                            const uint16_t* B, int64_t rank, int64_t adapters, const float* scale,
+                            const int32_t* segments, int64_t count, float* C, int64_t ldc, int accumulate);
+/* As sdh_lora_nt_bf16, A and B fp32. */
+int sdh_lora_nt_f32(int64_t M, int64_t N, int64_t K, const float* X, int64_t ldx, const float* A, const float* B,
+                    int64_t rank, int64_t adapters, const float* scale, const int32_t* segments, int64_t count,
+                    float* C, int64_t ldc, int accumulate);
+
 /* ---- norms -------------------------------------------------------------- */
 /* backend_cuda.h:48 group_norm(); tensor.h:166. x, y [N, C, HW]; gamma, beta
  * [C]; C % groups == 0. y may equal x. Large segments may run on the
@@ -270,6 +295,29 @@ int sdh_qknorm_rope_attention(float* q, const float* k, const float* v, void* ou
  * step's 2e-2). Head dimensions above 128 run as sdh_attention's. */
 int sdh_attention_fp16(const float* q, const float* k, const float* v, void* out, int out_bf16, int64_t N,
                        int64_t Sq, int64_t Skv, int heads, int kv_heads, int64_t d, int causal);
+
+/* No counterpart in the reference: attention over sequences packed into one
+ * tensor, every sequence's queries to its own keys. q and out [Tq, heads*d], k
+ * and v [Tk, kv_heads*d], heads as sdh_attention's, out float32 or (out_bf16)
+ * its bf16 bits. spans [seqs, 4] int32 on the device, 16-byte aligned: a
+ * sequence's first query row, its lq query rows, its first key row, its lk key
+ * rows. Rows may lie anywhere (packed, padded, keys in slots of a cache; several
+ * sequences may read the same keys), but no query row may belong to two
+ * sequences; entries past the tensors are cut to them. out rows of no sequence
+ * are left as they were.
+ *   Query i stands at position p = i + lk - lq (the last query at the last key)
+ * and sees key j when j < prefix[s], or when (not causal or j <= p) and (window
+ * 0 or |p - j| < window). prefix [seqs] int32 on the device, or NULL for none.
+ *   Scores: scale * q.k; with cap > 0 then cap * tanh(score / cap); with bias
+ * [heads, 2 radius + 1] then + bias[h, clamp(j - p, -radius, radius) + radius]
+ * (-inf hides a key). A query that sees no key gives zeros. Keys that a query
+ * does not see do not change its result, whatever their values are.
+ *   out must not overlap an input. The arrays are read when the work runs, so a
+ * captured graph takes the spans that they hold at each replay. */
+int sdh_attention_packed(const float* q, const float* k, const float* v, void* out, int out_bf16, int64_t Tq,
+                         int64_t Tk, int heads, int kv_heads, int64_t d, const int32_t* spans, int64_t seqs,
+                         float scale, int causal, int64_t window, const int32_t* prefix, float cap,
+                         const float* bias, int64_t radius);
 
 /* ---- activations ----------------------------------------------------------- */
 /* backend_cuda.h:61 swiglu(); tensor.h:191. y = gate / (1 + exp(-gate)) * up. */

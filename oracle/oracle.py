@@ -394,6 +394,96 @@ class Oracle:
         o = np.matmul(p, vh)
         return o.transpose(0, 2, 1, 3).reshape(N, len(rows), inner).astype(np.float32)
 
+    # -- attention over packed sequences (no reference counterpart) --
+    def attention_packed(self, q, k, v, out, spans, heads, kv_heads, scale, causal=False, window=0, prefix=None,
+                         cap=0.0, bias=None, radius=0):
+        """float64 definition of sdh_attention_packed. Returns the result (rows of no
+        sequence as in `out`) and a bound for its fp32 evaluation, per value.
+
+        The bound: a score is off by at most (d + 48) 2^-24 sum|q k| scale (its d
+        fp32 sums; the operands held to 2^-22, three roundings of the scaled score)
+        + 8 2^-24 (cap + |x|) (tanh to 5 2^-24 of itself, the bias' sum), the exponent
+        by 2^-24 |x| of that again; softmax turns a score error e into at most 2 e per
+        weight, and the weighted sum adds (keys + 64) 2^-24 sum p|v| (weights and
+        values held to 2^-21)."""
+        plant = getattr(self, "_plant_py", 0)
+        q, k, v = (np.asarray(a, np.float32) for a in (q, k, v))
+        d = q.shape[1] // heads
+        want, tol = np.array(out, np.float64), np.zeros(q.shape)
+        u = 2.0 ** -24
+        for s, (q0, lq, k0, lk) in enumerate(np.asarray(spans)):
+            q0, k0 = min(max(int(q0), 0), len(q)), min(max(int(k0), 0), len(k))
+            lq, lk = min(max(int(lq), 0), len(q) - q0), min(max(int(lk), 0), len(k) - k0)
+            pre = min(max(int(prefix[s]), 0), lk) if prefix is not None else 0
+            j = np.arange(lk)
+            for i in range(lq):
+                p = i + lk - lq
+                if plant == 20:  # planted: the first query at the first key
+                    p = i
+                see = np.ones(lk, bool)
+                if causal:
+                    see &= j <= p
+                if window:
+                    see &= np.abs(p - j) < (window + 1 if plant == 21 else window)  # planted 21: the window one wider
+                if plant != 22:  # planted 22: no prefix
+                    see |= j < pre
+                js = j[see]
+                for h in range(heads):
+                    row, c = q0 + i, slice(h * d, h * d + d)
+                    want[row, c], tol[row, c] = 0.0, 0.0
+                    if not len(js):
+                        continue
+                    g = h // (heads // kv_heads)
+                    kk = k[k0 + js, g * d:g * d + d].astype(np.float64)
+                    vv = v[k0 + js, g * d:g * d + d].astype(np.float64)
+                    qq = q[row, c].astype(np.float64)
+                    x = kk @ qq * scale
+                    e = (d + 48) * u * (np.abs(kk) @ np.abs(qq)) * abs(scale)
+                    if bias is not None and plant == 23:  # planted: the bias inside the cap
+                        x = x + bias[h, np.clip(js - p, -radius, radius) + radius]
+                    if cap:
+                        x = cap * np.tanh(x / cap)
+                    if bias is not None and plant != 23:
+                        x = x + bias[h, np.clip(js - p, -radius, radius) + radius].astype(np.float64)
+                    if np.all(x == -np.inf):
+                        continue
+                    e = e + 9 * u * (cap + np.where(np.isfinite(x), np.abs(x), 0))
+                    low = np.finfo(np.float32).min  # sums with the lowest value are taken in fp32: they stay there
+                    x = np.where((x < low / 2) & (x > -np.inf), low, x)
+                    w = np.exp(x - x.max())
+                    w = w / w.sum()
+                    near = np.max(e[w > 1e-30])
+                    if x.max() == low:
+                        near = 0.0
+                    want[row, c] = w @ vv
+                    tol[row, c] = (2 * near + (len(js) + 64) * u) * (w @ np.abs(vv))
+        return want, tol
+
+    # -- low-rank adapters (no reference counterpart) --
+    def lora(self, x, A, B, scale, segments, c0, accumulate=True):
+        """float64 definition of sdh_lora_nt_* and the bound of its fp32 evaluation: each
+        of the K + rank products of a value is summed once (K + rank + 8 roundings of
+        sum |s x a b|), C once more."""
+        plant = getattr(self, "_plant_py", 0)
+        x, want = np.asarray(x, np.float64), np.array(c0, np.float64)
+        S = np.zeros_like(want)
+        u = 2.0 ** -24
+        for first, rows, a, r in np.asarray(segments):
+            first = min(max(int(first), 0), len(x))
+            rows, r = min(max(int(rows), 0), len(x) - first), min(max(int(r), 0), A.shape[1])
+            at = slice(first, first + rows)
+            if not accumulate:
+                want[at] = 0.0
+            if a < 0 or a >= len(A) or not r:
+                continue
+            if plant == 30:  # planted: every rank counts
+                r = A.shape[1]
+            f = 1.0 if scale is None or plant == 31 else float(scale[a])  # planted 31: no scale
+            Aa, Ba = A[a, :r].astype(np.float64), B[a, :, :r].astype(np.float64)
+            S[at] = (x.shape[1] + r + 8) * u * abs(f) * (np.abs(x[at]) @ np.abs(Aa).T @ np.abs(Ba).T) + 2 * u * np.abs(want[at])
+            want[at] += f * (x[at] @ Aa.T @ Ba.T)
+        return want, S
+
     # -- the Z-Image transformer (zimage.cpp:71-228) --
     def zimage_forward(self, weights, x, t, cap, heads, bf16_names=(), act_bf16=False, patch=2, eps=1e-5,
                        theta=256.0, t_scale=1000.0, axes=(32, 48, 48)):

@@ -53,6 +53,14 @@ STUB(int sdh_attention_fp16(const float*, const float*, const float*, void*, int
                              int64_t, int))
 STUB(int sdh_qknorm_rope_attention(float*, const float*, const float*, void*, int, int64_t, int64_t, int, int64_t,
                                     const float*, const float*, float, const float*, const float*, int))
+STUB(int sdh_attention_packed(const float*, const float*, const float*, void*, int, int64_t, int64_t, int, int, int64_t,
+                               const int32_t*, int64_t, float, int, int64_t, const int32_t*, float, const float*, int64_t))
+STUB(int sdh_lora_nt_bf16(int64_t, int64_t, int64_t, const float*, int64_t, const uint16_t*, const uint16_t*, int64_t, int64_t,
+                           const float*, const int32_t*, int64_t, float*, int64_t, int))
+STUB(int sdh_lora_nt_bf16_packed(int64_t, int64_t, int64_t, const uint16_t*, int64_t, const uint16_t*, const uint16_t*, int64_t,
+                                  int64_t, const float*, const int32_t*, int64_t, float*, int64_t, int))
+STUB(int sdh_lora_nt_f32(int64_t, int64_t, int64_t, const float*, int64_t, const float*, const float*, int64_t, int64_t,
+                          const float*, const int32_t*, int64_t, float*, int64_t, int))
 STUB(int sdh_swiglu(const float*, const float*, float*, int64_t))
 STUB(int sdh_geglu(const float*, float*, int64_t, int64_t))
 STUB(int sdh_silu(float*, int64_t))

@@ -96,6 +96,11 @@ SIGNATURES = {
     "sdh_attention_fp16": [_vp, _vp, _vp, _vp, C.c_int, _i64, _i64, _i64, C.c_int, C.c_int, _i64, C.c_int],
     "sdh_qknorm_rope_attention": [_vp, _vp, _vp, _vp, C.c_int, _i64, _i64, C.c_int, _i64, _vp, _vp, _fl, _vp, _vp,
                                   C.c_int],
+    "sdh_attention_packed": [_vp, _vp, _vp, _vp, _int, _i64, _i64, _int, _int, _i64, _vp, _i64, _fl, _int, _i64, _vp, _fl,
+                             _vp, _i64],
+    "sdh_lora_nt_bf16": [_i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _int],
+    "sdh_lora_nt_bf16_packed": [_i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _int],
+    "sdh_lora_nt_f32": [_i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _int],
     "sdh_upsample_nearest2x": [_vp, _vp, _i64, _i64, _i64],
     "sdh_concat_channels": [_vp, _vp, _vp, _i64, _i64, _i64, _i64],
     "sdh_nchw_to_nlc": [_vp, _vp, _i64, _i64, _i64],
@@ -146,8 +151,8 @@ def _p(x) -> Optional[int]:
 
 
 class DArray:
-    """An array in the backend's device arena: float32 (activations) or
-    uint16 (bf16 bit patterns, for weights)."""
+    """An array in the backend's device arena: float32 (activations), uint16
+    (bf16 bit patterns, for weights) or int32 (which rows are whose)."""
 
     def __init__(self, backend: "Backend", shape: Sequence[int], ptr: Optional[int] = None, owned: bool = True,
                  dtype=np.float32):
@@ -155,8 +160,8 @@ class DArray:
         self.shape = tuple(int(s) for s in shape)
         self.size = int(np.prod(self.shape)) if self.shape else 1
         self.dtype = np.dtype(dtype)
-        if self.dtype not in (np.dtype(np.float32), np.dtype(np.uint16)):
-            raise TypeError("DArray holds float32 or uint16 (bf16) data")
+        if self.dtype not in (np.dtype(np.float32), np.dtype(np.uint16), np.dtype(np.int32)):
+            raise TypeError("DArray holds float32, uint16 (bf16) or int32 data")
         self.nbytes = self.size * self.dtype.itemsize
         self.owned = owned
         if ptr is None:
@@ -239,6 +244,13 @@ class Backend:
         """Device-to-device copy on the library stream (sdh_copy)."""
         self.check(self.lib.sdh_copy(_p(dst), _p(src), nbytes))
 
+    def register_external(self, ptr: int, nbytes: int):
+        """Lets ops take device memory that the library did not allocate (sdh_register_external)."""
+        self.check(self.lib.sdh_register_external(ptr, nbytes))
+
+    def unregister_external(self, ptr: int):
+        self.check(self.lib.sdh_unregister_external(ptr))
+
     def memory_stats(self):
         r, u = C.c_size_t(), C.c_size_t()
         self.check(self.lib.sdh_memory_stats(C.byref(r), C.byref(u)))
@@ -248,8 +260,8 @@ class Backend:
         return DArray(self, shape)
 
     def array(self, a: np.ndarray) -> DArray:
-        """float32 arrays stay float32; uint16 arrays are bf16 bit patterns."""
-        dt = np.uint16 if np.asarray(a).dtype == np.uint16 else np.float32
+        """float32 and int32 arrays keep their type; uint16 arrays are bf16 bit patterns."""
+        dt = np.asarray(a).dtype if np.asarray(a).dtype in (np.uint16, np.int32) else np.float32
         a = np.ascontiguousarray(a, dtype=dt)
         return DArray(self, a.shape, dtype=dt).upload(a)
 
@@ -342,6 +354,13 @@ class Backend:
         self.call("sdh_attention_fp16", _p(q), _p(k), _p(v), _p(out), int(bool(out_bf16)), N, Sq, Skv, heads,
                   kv_heads, d, int(bool(causal)))
 
+    def attention_packed(self, q, k, v, out, Tq, Tk, heads, kv_heads, d, spans, seqs, scale, causal=False, window=0,
+                         prefix=None, cap=0.0, bias=None, radius=0, out_bf16=False):
+        """Attention over packed sequences: spans [seqs, 4] int32 holds each one's first query row, query rows,
+        first key row and key rows; masks, cap and bias as sdh_attention_packed."""
+        self.call("sdh_attention_packed", _p(q), _p(k), _p(v), _p(out), int(bool(out_bf16)), Tq, Tk, heads, kv_heads, d,
+                  _p(spans), seqs, scale, int(bool(causal)), window, _p(prefix), cap, _p(bias), radius)
+
     def swiglu(self, g, u, y, n):
         self.call("sdh_swiglu", _p(g), _p(u), _p(y), n)
 
@@ -409,6 +428,23 @@ class Backend:
 
     def gemm_nt_f32(self, M, N, K, A, lda, B, ldb, C, ldc, bias=None, accumulate=False):
         self.call("sdh_gemm_nt_f32", M, N, K, _p(A), lda, _p(B), ldb, _p(C), ldc, _p(bias), int(bool(accumulate)))
+
+    # low-rank adapters: C (+)= scale_a (X A_a^T) B_a^T per run of rows; segments [count, 4] int32 holds each run's
+    # first row, rows, adapter (-1: none) and rank
+    def lora_nt_bf16(self, M, N, K, X, ldx, A, B, rank, adapters, scale, segments, count, C, ldc, accumulate=True):
+        self.call("sdh_lora_nt_bf16", M, N, K, _p(X), ldx, _p(A), _p(B), rank, adapters, _p(scale), _p(segments), count,
+                  _p(C), ldc, int(bool(accumulate)))
+
+    def lora_nt_bf16_packed(self, M, N, K, X16, ldx, A, B, rank, adapters, scale, segments, count, C, ldc,
+                            accumulate=True):
+        """As lora_nt_bf16, X16 holding bf16 bits."""
+        self.call("sdh_lora_nt_bf16_packed", M, N, K, _p(X16), ldx, _p(A), _p(B), rank, adapters, _p(scale),
+                  _p(segments), count, _p(C), ldc, int(bool(accumulate)))
+
+    def lora_nt_f32(self, M, N, K, X, ldx, A, B, rank, adapters, scale, segments, count, C, ldc, accumulate=True):
+        """As lora_nt_bf16, A and B fp32."""
+        self.call("sdh_lora_nt_f32", M, N, K, _p(X), ldx, _p(A), _p(B), rank, adapters, _p(scale), _p(segments), count,
+                  _p(C), ldc, int(bool(accumulate)))
 
     def conv2d(self, x, N, Cin, H, W, w, Cout, kh, kw, bias, stride, pad, out, Ho, Wo):
         self.call("sdh_conv2d", _p(x), N, Cin, H, W, _p(w), Cout, kh, kw, _p(bias), stride, pad, _p(out), Ho, Wo)
