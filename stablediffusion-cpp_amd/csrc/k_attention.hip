@@ -64,13 +64,12 @@
 #include <cstdlib>
 #include <type_traits>
 
-#include "sdh_internal.hpp"
+#include "fp16_pair.hpp"
 
 namespace sdh {
 namespace {
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned short u16;
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
@@ -110,21 +109,6 @@ __device__ __forceinline__ void split(float x, _Float16& hi, _Float16& lo) {
     hi = (_Float16)x;
     lo = (_Float16)(x - (float)hi);
 }
-// Two softmax weights in [0, 2^16) into hi + lo: hi is p towards zero in fp16
-// (v_cvt_pkrtz), lo = p - hi rounded to fp16 (|lo| < 2^-10 p, so the pair is
-// within 2^-21 p; below 2^-14, where fp16 is subnormal, within 2^-25
-// absolutely). v_fma_mixlo/mixhi take hi's half as it lies in the packed pair and
-// round the exact difference into a half: three instructions a pair, where
-// masking, subtracting and packing took six.
-__device__ __forceinline__ void split_weights(float p0, float p1, h2& hi, h2& lo) {
-    hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(p0, p1));
-    const unsigned h = __builtin_bit_cast(unsigned, hi);
-    unsigned l;
-    asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(l) : "v"(h), "v"(p0));
-    asm("v_fma_mixhi_f16 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(l) : "v"(h), "v"(p1));
-    lo = __builtin_bit_cast(h2, l);
-}
-
 // Exponent e of a block whose largest magnitude is amax: amax 2^-e lies in
 // [2^13, 2^14). Zero, subnormal, inf and NaN maxima give 0 (no scaling).
 __device__ __forceinline__ int block_exp(float amax) {
@@ -596,7 +580,7 @@ __global__ __launch_bounds__(KEYS ? 64 * kKeyWaves : kThreads, 1) void k_attn_fw
                 const float p0 = s[ks >> 1][(ks & 1) * 8 + e], p1 = s[ks >> 1][(ks & 1) * 8 + e + 1];
                 if constexpr (SPLIT) {
                     h2 hi, lo;
-                    split_weights(p0, p1, hi, lo);
+                    split_pair(p0, p1, hi, lo);
                     ph[ks][e] = hi[0], ph[ks][e + 1] = hi[1];
                     pl[ks][e] = lo[0], pl[ks][e + 1] = lo[1];
                 } else {

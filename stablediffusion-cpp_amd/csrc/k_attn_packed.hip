@@ -14,6 +14,7 @@
 #include <string>
 #include <type_traits>
 
+#include "fp16_pair.hpp"
 #include "spans.hpp"
 
 namespace sdh {
@@ -135,6 +136,553 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_attn_packed_rows(Packed P) {
     }
 }
 
+// ---------------------------------------------------------------------------
+// Head dimensions up to 128 (padded to DP = 64 or 128), on the MFMA units.
+//
+// A workgroup takes kTileRows rows of one sequence and key/value head, a row being a
+// (query, head of the group) pair, heads fastest: the heads that share a key/value head
+// share its tiles. It walks the 64-key tiles that any of its rows sees. The eight waves
+// bring a tile in together, eight keys each, from fp32 in memory to fp16 pairs in LDS,
+// and each wave then takes 32 rows against it.
+//
+// Operands are fp16 pairs hi + lo in block floating point, products hi hi + hi lo +
+// lo hi with fp32 sums (2^-21 of each product). A block is a row of q, or the eight keys
+// that a wave brought in: with k or v scaled by 2^-e to at most 2^14, a score is
+// s 2^(e_q + e_k), and a weight is formed as p 2^(14 + e_v - E), E the largest e_v that the
+// lane's row has seen, so that the sums of all blocks share the scale 2^(14 - E).
+// Rows in LDS are ordered so that the eight scores of a lane's half of a 16-key step are
+// eight neighbouring keys: one block, one exponent. Tiles at the border of what the rows
+// see have an exponent for each key: an unseen key, whatever its size, then has no say
+// in the others'. Values that are not finite go into the tiles as zeros, since 0 * inf would
+// reach the rows that do not see them, and are added at the end; a key that is not finite
+// makes the scores of the rows that see it NaN, and only those.
+//
+// S^T = K Q^T and O^T = V^T P^T by v_mfma_f32_32x32x16_f16: lane l holds row l % 32 of
+// the wave in both, its statistics are its own, and its weights are the second product's
+// operand as they lie.
+// ---------------------------------------------------------------------------
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+using dev::f4;
+
+constexpr int kKT = 64, kWaves = 8, kThreads = 64 * kWaves, kTileRows = 32 * kWaves;
+// The reference m of the weights is raised when a tile's largest score passes it by more
+// than this (in units of log2): weights stay below 2^(14 + kLazy), inside fp16.
+constexpr float kLazy = 1.5f;
+constexpr int kUnsetE = -1000;  // no values seen yet
+constexpr int kFarE = -40;      // weights' exponents relative to E are not taken below this (2^-40 of the largest sum)
+
+__device__ __forceinline__ int swz_v(int r) { return (r >> 1) & 7; }
+template <int DP>
+__device__ __forceinline__ int swz_k(int r) {
+    return DP == 128 ? (r & 15) : ((r >> 1) & 7);
+}
+__device__ __forceinline__ int row_of_key(int j) { return (j & ~12) | ((j & 4) << 1) | ((j & 8) >> 1); }
+
+template <int CTRL>
+__device__ __forceinline__ int dpp_i(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, false);
+}
+// Largest non-negative int over aligned groups of W lanes (8, 16 or 64).
+template <int W>
+__device__ __forceinline__ int group_imax(int v) {
+    v = max(v, dpp_i<0xB1>(v));
+    v = max(v, dpp_i<0x4E>(v));
+    v = max(v, dpp_i<0x141>(v));
+    if constexpr (W >= 16) v = max(v, dpp_i<0x140>(v));
+    if constexpr (W == 64) {
+        const int a = __builtin_amdgcn_readlane(v, 0), b = __builtin_amdgcn_readlane(v, 16), c = __builtin_amdgcn_readlane(v, 32),
+                  d = __builtin_amdgcn_readlane(v, 48);
+        v = max(max(a, b), max(c, d));
+    }
+    return v;
+}
+__device__ __forceinline__ int abs_bits(float x) { return (int)(__float_as_uint(x) & 0x7FFFFFFFu); }
+constexpr int kInfBits = 0x7F800000;
+// The exponent that brings a block's largest magnitude into [2^13, 2^14); zero and
+// subnormal blocks the least there is.
+__device__ __forceinline__ int block_exp(int bits) { return min(max((bits >> 23) - 140, -126), 126); }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(127 + e) << 23); }  // e in [-126, 127]
+
+struct Tile {  // which rows a workgroup has
+    int seq, row0, rows;  // rows: of the whole sequence
+    int q0, lq, k0, lk, pre;
+};
+// The workgroup's place in the sequences' row tiles; false past the last.
+__device__ __forceinline__ bool find_tile(const Packed& P, int group, int tile_rows, int item, Tile& t) {
+    const int lane = threadIdx.x & 63;
+    for (int s0 = 0, before = 0; s0 < P.seqs; s0 += 64) {
+        int4 e = make_int4(0, 0, 0, 0);
+        if (s0 + lane < P.seqs) {
+            e = P.spans[s0 + lane];
+            dev::cut_span(e.x, e.y, P.Tq);
+        }
+        const int n = (e.y * group + tile_rows - 1) / tile_rows;
+        const int upto = before + dev::wave_scan(n);
+        const unsigned long long m = __ballot(item < upto);
+        if (m) {
+            const int at = (int)__ffsll(m) - 1;
+            t.seq = s0 + at;
+            t.q0 = __builtin_amdgcn_readlane(e.x, at);
+            t.lq = __builtin_amdgcn_readlane(e.y, at);
+            t.k0 = __builtin_amdgcn_readlane(e.z, at);
+            t.lk = __builtin_amdgcn_readlane(e.w, at);
+            dev::cut_span(t.k0, t.lk, P.Tk);
+            t.row0 = (item - __builtin_amdgcn_readlane(upto - n, at)) * tile_rows;
+            t.rows = t.lq * group;
+            t.pre = P.prefix ? min(max(P.prefix[t.seq], 0), t.lk) : 0;
+            return true;
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
+}
+
+template <int DP, bool OUT16, bool EXTRA, bool VEC>
+__global__ __launch_bounds__(kThreads, 1) void k_attn_packed_tiles(Packed P, int items) {
+    constexpr int DS = DP / 16, DT = DP / 32, KU = DP / 64, PART = kKT * DP;
+    // [K hi][K lo][V^T hi][V^T lo] of two tiles
+    __shared__ __attribute__((aligned(1024))) u16 buf[2][4 * PART];
+    __shared__ __attribute__((aligned(16))) int exps[2][2][8];      // of k, v, eight keys each
+    __shared__ __attribute__((aligned(16))) int key_exps[2][2][kKT];  // at a border: of each key
+    __shared__ __attribute__((aligned(16))) int bads[2][8];         // values that are not finite
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int fr = lane & 31, fh = lane >> 5;
+    const int group = P.heads / P.kv_heads;
+    // Workgroups are dealt to the 8 XCDs in turn; renumbered so that an XCD has
+    // neighbouring row tiles of a sequence and head, whose keys its L2 then holds.
+    const int per = gridDim.x >> 3, rem = gridDim.x & 7, xcd = blockIdx.x & 7;
+    const int lb = xcd * per + min(xcd, rem) + (blockIdx.x >> 3);
+    const int kh = lb / items;
+    Tile T;
+    if (!find_tile(P, group, kTileRows, lb - kh * items, T)) return;
+    const int d = P.d, lk = T.lk, pre = T.pre;
+    const int64_t inner = (int64_t)P.heads * d, kv_inner = (int64_t)P.kv_heads * d;
+    const int r = T.row0 + w * 32 + fr;
+    const int rc = min(r, T.rows - 1), qi = rc / group, h = kh * group + (rc - qi * group);
+    const int shift = lk - T.lq;
+    const int p = qi + shift;
+    const Seen see = seen_from(P, p, lk, pre);
+    const Seen wg_first = seen_from(P, T.row0 / group + shift, lk, pre),
+               wg_last = seen_from(P, (min(T.row0 + kTileRows, T.rows) - 1) / group + shift, lk, pre);
+    const int wg_lo = wg_first.lo, wg_hi = wg_last.hi;
+    const bool active = T.row0 + w * 32 < T.rows;
+    const int first_lo = __builtin_amdgcn_readlane(see.lo, 0), last_hi = __builtin_amdgcn_readlane(see.hi, 31);
+    const int npre = (pre + kKT - 1) / kKT, next = max(npre, wg_lo / kKT);
+    const int nt = npre + (wg_hi > wg_lo ? max(0, (wg_hi + kKT - 1) / kKT - next) : 0);
+    auto key_of = [&](int n) { return (n < npre ? n : next + n - npre) * kKT; };
+
+    // Q: the B operand of S^T, row qi of head h, dims ds*16 + fh*8 .. +7
+    const float* qp = P.q + (T.q0 + qi) * inner + (int64_t)h * d;
+    h8 qh[DS], ql[DS];
+    int eq;
+    {
+        float x[DS][8];
+        int top = 0;
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds) {
+            const int c0 = ds * 16 + fh * 8;
+            if constexpr (VEC) {
+                const float* a = qp + min(c0, d - 8);
+                const f4 u = *(const f4*)a, v = *(const f4*)(a + 4);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[ds][e] = c0 < d ? (e < 4 ? u[e & 3] : v[e & 3]) : 0.f;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[ds][e] = c0 + e < d ? qp[c0 + e] : 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = max(top, abs_bits(x[ds][e]));
+        }
+        top = max(top, __shfl_xor(top, 32, 64));
+        eq = block_exp(top);
+        const float sc = copysignf(pow2(-eq), P.scale);  // a negative scale turns q's sign
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                h2 hi, lo;
+                split_pair(x[ds][e] * sc, x[ds][e + 1] * sc, hi, lo);
+                qh[ds][e] = hi[0], qh[ds][e + 1] = hi[1];
+                ql[ds][e] = lo[0], ql[ds][e + 1] = lo[1];
+            }
+    }
+    const float scale = fabsf(P.scale);
+
+    // A tile on its way: this wave's eight keys. k: 16-byte chunks of their rows; v: the
+    // lane's columns of all eight.
+    constexpr int KCH = DP / 8;  // chunks of a row
+    const int kch = lane & (KCH - 1), krow = lane / KCH;
+    constexpr int KROWS = 64 / KCH;
+    float kx[KU][8], vx[8][KU];
+    const float* kbase = P.k + T.k0 * kv_inner + (int64_t)kh * d;
+    const float* vbase = P.v + T.k0 * kv_inner + (int64_t)kh * d;
+    // a tile that some of the workgroup's rows see in part
+    auto border = [&](int k0) { return !(k0 + kKT <= pre || (k0 >= wg_last.lo && k0 + kKT <= wg_first.hi)); };
+    auto wanted = [&](int j) { return j < lk && (j < pre || (j >= wg_lo && j < wg_hi)); };
+    auto fetch = [&](int n) __attribute__((always_inline)) {
+        const int j0 = key_of(n) + w * 8;
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+            const float* a = kbase + (int64_t)min(j0 + u * KROWS + krow, lk - 1) * kv_inner;
+            if constexpr (VEC) {
+                a += min(kch * 8, d - 8);
+                const f4 x = *(const f4*)a, y = *(const f4*)(a + 4);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) kx[u][e] = e < 4 ? x[e & 3] : y[e & 3];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) kx[u][e] = a[min(kch * 8 + e, d - 1)];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float* a = vbase + (int64_t)min(j0 + i, lk - 1) * kv_inner;
+            if constexpr (VEC && KU == 2) {
+                const f2 x = *(const f2*)(a + min(lane * 2, d - 2));
+                vx[i][0] = x.x, vx[i][1] = x.y;
+            } else {
+#pragma unroll
+                for (int u = 0; u < KU; ++u) vx[i][u] = a[min(lane * KU + u, d - 1)];
+            }
+        }
+    };
+    // Into LDS: scaled, split, in the order of the fragments' reads.
+    auto store = [&](int n, int b) __attribute__((always_inline)) {
+        const int k0 = key_of(n), j0 = k0 + w * 8;
+        int ktop = 0, vtop = 0;
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+            const bool ok = wanted(j0 + u * KROWS + krow);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (!ok || kch * 8 + e >= d) kx[u][e] = 0.f;
+                ktop = max(ktop, abs_bits(kx[u][e]));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool ok = wanted(j0 + i);
+#pragma unroll
+            for (int u = 0; u < KU; ++u) {
+                if (!ok || lane * KU + u >= d) vx[i][u] = 0.f;
+                vtop = max(vtop, abs_bits(vx[i][u]));
+            }
+        }
+        ktop = group_imax<64>(ktop);
+        vtop = group_imax<64>(vtop);
+        const bool bad = vtop >= kInfBits;
+        if (bad) {
+            vtop = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int u = 0; u < KU; ++u) {
+                    if (abs_bits(vx[i][u]) >= kInfBits) vx[i][u] = 0.f;
+                    vtop = max(vtop, abs_bits(vx[i][u]));
+                }
+            vtop = group_imax<64>(vtop);
+        }
+        const int ek = block_exp(ktop), ev = block_exp(vtop);
+        if (lane == 0) {
+            exps[b][0][w] = ek;
+            exps[b][1][w] = ev;
+            bads[b][w] = bad;
+        }
+        float ks[KU], vs[8];
+#pragma unroll
+        for (int u = 0; u < KU; ++u) ks[u] = pow2(-ek);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) vs[i] = pow2(-ev);
+        if (border(k0)) {
+#pragma unroll
+            for (int u = 0; u < KU; ++u) {
+                int top = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = max(top, abs_bits(kx[u][e]));
+                const int e = block_exp(group_imax<KCH>(top));
+                ks[u] = pow2(-e);
+                if (kch == 0) key_exps[b][0][w * 8 + u * KROWS + krow] = e;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                int top = 0;
+#pragma unroll
+                for (int u = 0; u < KU; ++u) top = max(top, abs_bits(vx[i][u]));
+                const int e = block_exp(group_imax<64>(top));
+                vs[i] = pow2(-e);
+                if (lane == 0) key_exps[b][1][w * 8 + i] = e;
+            }
+        }
+        u16 *kd = buf[b], *vd = buf[b] + 2 * PART;
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+            const int row = row_of_key(w * 8 + u * KROWS + krow);
+            h8 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                h2 a, c;
+                split_pair(kx[u][e] * ks[u], kx[u][e + 1] * ks[u], a, c);
+                hi[e] = a[0], hi[e + 1] = a[1];
+                lo[e] = c[0], lo[e + 1] = c[1];
+            }
+            const int at = row * DP + ((kch ^ swz_k<DP>(row)) << 3);
+            *(h8*)(kd + at) = hi;
+            *(h8*)(kd + PART + at) = lo;
+        }
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+            const int row = lane * KU + u;
+            h8 hi, lo;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                h2 a, c;
+                split_pair(vx[i][u] * vs[i], vx[i + 1][u] * vs[i + 1], a, c);
+                hi[i] = a[0], hi[i + 1] = a[1];
+                lo[i] = c[0], lo[i + 1] = c[1];
+            }
+            const int at = row * kKT + ((w ^ swz_v(row)) << 3);
+            *(h8*)(vd + at) = hi;
+            *(h8*)(vd + PART + at) = lo;
+        }
+    };
+
+    f32x16 o[DT], s[2];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
+    float m = -INFINITY, sum = 0.f;  // the reference (log2 units without EXTRA), this lane's keys' sum of weights
+    int E = kUnsetE;
+
+    auto scores = [&](const u16* kd) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[j][i] = 0.f;
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds) {
+            h8 kf[2][2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int row = j * 32 + fr, at = row * DP + (((ds * 2 + fh) ^ swz_k<DP>(row)) << 3);
+                kf[j][0] = *(const h8*)(kd + at);
+                kf[j][1] = *(const h8*)(kd + PART + at);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[j][0], qh[ds], s[j], 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[j][0], ql[ds], s[j], 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[j][1], qh[ds], s[j], 0, 0, 0);
+        }
+    };
+    // Score register i of half j is key k0 + j*32 + (i/8)*16 + fh*8 + i%8.
+    auto key_at = [&](int j, int i) { return j * 32 + (i >> 3) * 16 + fh * 8 + (i & 7); };
+    auto visible = [&](int j) { return (j < pre) | ((j >= see.lo) & (j < see.hi)); };
+
+    // s -> weights in place, the statistics and the scale of o brought up to date
+    auto softmax = [&](int k0, int b) __attribute__((always_inline)) {
+        const bool edge = border(k0);
+        int ek[4], ev[4], emax = kUnsetE;
+        if (edge) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                ek[u] = ev[u] = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int j = u * 16 + fh * 8 + i;
+                    const bool ok = visible(k0 + j);
+                    s[u >> 1][(u & 1) * 8 + i] = ldexpf(s[u >> 1][(u & 1) * 8 + i], key_exps[b][0][j]);
+                    if (ok) emax = max(emax, key_exps[b][1][j]);
+                }
+            }
+            emax = max(emax, __shfl_xor(emax, 32, 64));
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                ek[u] = exps[b][0][u * 2 + fh];
+                ev[u] = exps[b][1][u * 2 + fh];
+                emax = max(emax, max(exps[b][1][u * 2], exps[b][1][u * 2 + 1]));
+            }
+        }
+        float ct[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)  // kept normal: -inf stays -inf, zero zero
+            ct[u] = fminf(fmaxf(ldexpf(EXTRA ? scale : scale * kLog2e, eq + ek[u]), 1.17549435e-38f), 3.40282347e38f);
+        if constexpr (EXTRA) {
+            const float* bp = P.bias + (int64_t)h * (2 * P.radius + 1) + P.radius;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float x = s[j][i] * ct[j * 2 + (i >> 3)];
+                    if (P.cap > 0.f) x = P.cap * tanh_near(x / P.cap);
+                    if (P.bias) x += bp[min(max(k0 + key_at(j, i) - p, -P.radius), P.radius)];
+                    s[j][i] = x;
+                }
+        }
+        if (edge) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (!visible(k0 + key_at(j, i))) s[j][i] = -INFINITY;
+        }
+        float mt = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            float mx = s[u >> 1][(u & 1) * 8];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[u >> 1][(u & 1) * 8 + i]);
+            mt = fmaxf(mt, EXTRA ? mx : mx * ct[u]);
+        }
+        mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+        const float mnew = mt > m + (EXTRA ? kLazy / kLog2e : kLazy) ? mt : m;
+        float alpha = 1.0f;
+        if (mnew != m) alpha = __builtin_amdgcn_exp2f(EXTRA ? (m - mnew) * kLog2e : m - mnew);
+        m = mnew;
+        const float ref = m == -INFINITY ? 0.f : m;
+        float ao = alpha;
+        if (emax > E) {
+            const int up = min(emax + 1, 126);  // a little ahead: the next tiles' are alike
+            ao = E == kUnsetE ? 0.f : ldexpf(alpha, max(E - up, -300));
+            E = up;
+        }
+        float total = 0.f;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int by = 14 + (edge ? 0 : max(ev[u] - E, kFarE));
+            float part = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float x = s[u >> 1][(u & 1) * 8 + i];
+                if constexpr (EXTRA) x = __builtin_amdgcn_exp2f(fmaf(x - ref, kLog2e, (float)by));
+                else x = __builtin_amdgcn_exp2f(fmaf(x, ct[u], (float)by - ref));
+                s[u >> 1][(u & 1) * 8 + i] = x;
+                part += x;
+            }
+            total += ldexpf(part, -by);
+        }
+        sum = fmaf(sum, alpha, total);
+        if (edge) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)  // an unseen key's weight is zero, its exponent may be above E
+                    s[u >> 1][(u & 1) * 8 + i] = ldexpf(s[u >> 1][(u & 1) * 8 + i],
+                                                        min(max(key_exps[b][1][u * 16 + fh * 8 + i] - E, kFarE), 0));
+        }
+        if (__ballot(ao != 1.0f)) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[dt][i] *= ao;
+        }
+    };
+    auto values = [&](const u16* vd) __attribute__((always_inline)) {
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            h8 ph, pl;
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                h2 hi, lo;
+                split_pair(s[ks >> 1][(ks & 1) * 8 + e], s[ks >> 1][(ks & 1) * 8 + e + 1], hi, lo);
+                ph[e] = hi[0], ph[e + 1] = hi[1];
+                pl[e] = lo[0], pl[e + 1] = lo[1];
+            }
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const int row = dt * 32 + fr, at = row * kKT + (((ks * 2 + fh) ^ swz_v(row)) << 3);
+                const h8 vh = *(const h8*)(vd + at), vl = *(const h8*)(vd + PART + at);
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph, o[dt], 0, 0, 0);
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl, o[dt], 0, 0, 0);
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph, o[dt], 0, 0, 0);
+            }
+        }
+    };
+
+    int bad_first = nt, bad_last = -1;  // the tiles that hold values that are not finite
+    if (nt > 0) {
+        fetch(0);
+        store(0, 0);
+    }
+    for (int n = 0; n < nt; ++n) {
+        const int b = n & 1, k0 = key_of(n);
+        if (n + 1 < nt) fetch(n + 1);
+        // tile n is in LDS, and nobody reads tile n - 1 any more
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (active && (k0 < pre || (k0 < last_hi && k0 + kKT > first_lo))) {
+            scores(buf[b]);
+            softmax(k0, b);
+            values(buf[b] + 2 * PART);
+        }
+        int any = 0;
+#pragma unroll
+        for (int g = 0; g < 8; ++g) any |= bads[b][g];
+        if (__builtin_amdgcn_readfirstlane(any)) {
+            bad_first = min(bad_first, n);
+            bad_last = n;
+        }
+        if (n + 1 < nt) store(n + 1, b ^ 1);
+    }
+
+    if (r >= T.rows) return;
+    sum += __shfl_xor(sum, 32, 64);
+    const float inv = sum == 0.f ? 0.f : ldexpf(1.0f / sum, E - 14);
+    for (int n = bad_first; n <= bad_last; ++n)
+        for (int j = key_of(n), end = min(j + kKT, lk); j < end; ++j) {
+            if (!visible(j)) continue;
+            const float* vp = vbase + j * kv_inner;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {  // columns past d are not stored
+                    const float x = vp[min(dt * 32 + (i >> 2) * 8 + fh * 4 + (i & 3), d - 1)];
+                    if (abs_bits(x) >= kInfBits) o[dt][i] += x;
+                }
+        }
+    const int64_t at = (T.q0 + qi) * inner + (int64_t)h * d;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int c = dt * 32 + g * 8 + fh * 4;
+            const f4 v = {o[dt][g * 4] * inv, o[dt][g * 4 + 1] * inv, o[dt][g * 4 + 2] * inv, o[dt][g * 4 + 3] * inv};
+            if constexpr (VEC) {
+                if (c >= d) continue;
+                if constexpr (OUT16) *(uint2*)((u16*)P.out + at + c) = dev::bf16x4(v);
+                else *(f4*)((float*)P.out + at + c) = v;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c + e < d) {
+                        if constexpr (OUT16) ((u16*)P.out)[at + c + e] = dev::bf16_rne(v[e]);
+                        else ((float*)P.out)[at + c + e] = v[e];
+                    }
+            }
+        }
+}
+
+template <int DP>
+void run_tiles(const Packed& P, bool out16, int64_t items) {
+    const bool vec = P.d % 8 == 0 && aligned16(P.q) && aligned16(P.k) && aligned16(P.v) && (out16 ? ((uintptr_t)P.out & 7) == 0 : aligned16(P.out));
+    const bool extra = P.cap > 0.f || P.bias;
+    using T_ = std::true_type;
+    using F_ = std::false_type;
+    auto go = [&](auto o16, auto ex, auto ve) {
+        k_attn_packed_tiles<DP, decltype(o16)::value, decltype(ex)::value, decltype(ve)::value>
+            <<<(unsigned)(items * P.kv_heads), kThreads, 0, stream()>>>(P, (int)items);
+    };
+    auto with = [&](auto o16) {
+        if (extra) vec ? go(o16, T_(), T_()) : go(o16, T_(), F_());
+        else vec ? go(o16, F_(), T_()) : go(o16, F_(), F_());
+    };
+    if (out16) with(T_());
+    else with(F_());
+}
+
 void run_attention_packed(const float* q, const float* k, const float* v, void* out, bool out16, int64_t Tq, int64_t Tk, int heads,
                           int kv_heads, int64_t d, const int32_t* spans, int64_t seqs, float scale, bool causal, int64_t window,
                           const int32_t* prefix, float cap, const float* bias, int64_t radius) {
@@ -168,6 +716,13 @@ void run_attention_packed(const float* q, const float* k, const float* v, void* 
     Packed P{q,    k,   v,   out, (const int4*)spans, prefix, bias, (int)Tq, (int)Tk, (int)seqs, heads, kv_heads, (int)d, causal ? 1 : 0,
              window < kMost ? (int)window : 0,  // a wider one hides nothing
              bias ? (int)radius : 0, scale, cap};
+    const int64_t rows = Tq * (heads / kv_heads), items = rows / kTileRows + std::min(seqs, Tq);
+    if (d <= 128 && rows < kMost && items * kv_heads * kThreads <= kMaxGridItems) {
+        if (d <= 64) run_tiles<64>(P, out16, items);
+        else run_tiles<128>(P, out16, items);
+        launched(op);
+        return;
+    }
     const int64_t gx = (Tq + kRowWaves - 1) / kRowWaves;
     need(gx * 64 * kRowWaves <= kMaxGridItems, op, "too many queries for one launch");
     const dim3 grid((unsigned)gx, (unsigned)heads);
