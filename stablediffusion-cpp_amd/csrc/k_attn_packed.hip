@@ -205,40 +205,6 @@ constexpr int kInfBits = 0x7F800000;
 __device__ __forceinline__ int block_exp(int bits) { return min(max((bits >> 23) - 140, -126), 126); }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(127 + e) << 23); }  // e in [-126, 127]
 
-struct Tile {  // which rows a workgroup has
-    int seq, row0, rows;  // rows: of the whole sequence
-    int q0, lq, k0, lk, pre;
-};
-// The workgroup's place in the sequences' row tiles; false past the last.
-__device__ __forceinline__ bool find_tile(const Packed& P, int group, int tile_rows, int item, Tile& t) {
-    const int lane = threadIdx.x & 63;
-    for (int s0 = 0, before = 0; s0 < P.seqs; s0 += 64) {
-        int4 e = make_int4(0, 0, 0, 0);
-        if (s0 + lane < P.seqs) {
-            e = P.spans[s0 + lane];
-            dev::cut_span(e.x, e.y, P.Tq);
-        }
-        const int n = (e.y * group + tile_rows - 1) / tile_rows;
-        const int upto = before + dev::wave_scan(n);
-        const unsigned long long m = __ballot(item < upto);
-        if (m) {
-            const int at = (int)__ffsll(m) - 1;
-            t.seq = s0 + at;
-            t.q0 = __builtin_amdgcn_readlane(e.x, at);
-            t.lq = __builtin_amdgcn_readlane(e.y, at);
-            t.k0 = __builtin_amdgcn_readlane(e.z, at);
-            t.lk = __builtin_amdgcn_readlane(e.w, at);
-            dev::cut_span(t.k0, t.lk, P.Tk);
-            t.row0 = (item - __builtin_amdgcn_readlane(upto - n, at)) * tile_rows;
-            t.rows = t.lq * group;
-            t.pre = P.prefix ? min(max(P.prefix[t.seq], 0), t.lk) : 0;
-            return true;
-        }
-        before = __builtin_amdgcn_readlane(upto, 63);
-    }
-    return false;
-}
-
 template <int DP, bool OUT16, bool EXTRA, bool VEC>
 __global__ __launch_bounds__(kThreads, 1) void k_attn_packed_tiles(Packed P, int items) {
     constexpr int DS = DP / 16, DT = DP / 32, KU = DP / 64, PART = kKT * DP;
@@ -255,26 +221,27 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_packed_tiles(Packed P, int
     const int per = gridDim.x >> 3, rem = gridDim.x & 7, xcd = blockIdx.x & 7;
     const int lb = xcd * per + min(xcd, rem) + (blockIdx.x >> 3);
     const int kh = lb / items;
-    Tile T;
-    if (!find_tile(P, group, kTileRows, lb - kh * items, T)) return;
-    const int d = P.d, lk = T.lk, pre = T.pre;
+    dev::SpanTile T;
+    if (!dev::find_tile(P.spans, P.seqs, P.Tq, group, kTileRows, lb - kh * items, T)) return;
+    dev::cut_span(T.z, T.w, P.Tk);
+    const int d = P.d, rows = T.rows * group, lk = T.w, pre = P.prefix ? min(max(P.prefix[T.index], 0), lk) : 0;
     const int64_t inner = (int64_t)P.heads * d, kv_inner = (int64_t)P.kv_heads * d;
     const int r = T.row0 + w * 32 + fr;
-    const int rc = min(r, T.rows - 1), qi = rc / group, h = kh * group + (rc - qi * group);
-    const int shift = lk - T.lq;
+    const int rc = min(r, rows - 1), qi = rc / group, h = kh * group + (rc - qi * group);
+    const int shift = lk - T.rows;
     const int p = qi + shift;
     const Seen see = seen_from(P, p, lk, pre);
     const Seen wg_first = seen_from(P, T.row0 / group + shift, lk, pre),
-               wg_last = seen_from(P, (min(T.row0 + kTileRows, T.rows) - 1) / group + shift, lk, pre);
+               wg_last = seen_from(P, (min(T.row0 + kTileRows, rows) - 1) / group + shift, lk, pre);
     const int wg_lo = wg_first.lo, wg_hi = wg_last.hi;
-    const bool active = T.row0 + w * 32 < T.rows;
+    const bool active = T.row0 + w * 32 < rows;
     const int first_lo = __builtin_amdgcn_readlane(see.lo, 0), last_hi = __builtin_amdgcn_readlane(see.hi, 31);
     const int npre = (pre + kKT - 1) / kKT, next = max(npre, wg_lo / kKT);
     const int nt = npre + (wg_hi > wg_lo ? max(0, (wg_hi + kKT - 1) / kKT - next) : 0);
     auto key_of = [&](int n) { return (n < npre ? n : next + n - npre) * kKT; };
 
     // Q: the B operand of S^T, row qi of head h, dims ds*16 + fh*8 .. +7
-    const float* qp = P.q + (T.q0 + qi) * inner + (int64_t)h * d;
+    const float* qp = P.q + (T.first + qi) * inner + (int64_t)h * d;
     h8 qh[DS], ql[DS];
     int eq;
     {
@@ -316,8 +283,8 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_packed_tiles(Packed P, int
     const int kch = lane & (KCH - 1), krow = lane / KCH;
     constexpr int KROWS = 64 / KCH;
     float kx[KU][8], vx[8][KU];
-    const float* kbase = P.k + T.k0 * kv_inner + (int64_t)kh * d;
-    const float* vbase = P.v + T.k0 * kv_inner + (int64_t)kh * d;
+    const float* kbase = P.k + T.z * kv_inner + (int64_t)kh * d;
+    const float* vbase = P.v + T.z * kv_inner + (int64_t)kh * d;
     // a tile that some of the workgroup's rows see in part
     auto border = [&](int k0) { return !(k0 + kKT <= pre || (k0 >= wg_last.lo && k0 + kKT <= wg_first.hi)); };
     auto wanted = [&](int j) { return j < lk && (j < pre || (j >= wg_lo && j < wg_hi)); };
@@ -628,7 +595,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_packed_tiles(Packed P, int
         if (n + 1 < nt) store(n + 1, b ^ 1);
     }
 
-    if (r >= T.rows) return;
+    if (r >= rows) return;
     sum += __shfl_xor(sum, 32, 64);
     const float inv = sum == 0.f ? 0.f : ldexpf(1.0f / sum, E - 14);
     for (int n = bad_first; n <= bad_last; ++n)
@@ -643,7 +610,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_packed_tiles(Packed P, int
                     if (abs_bits(x) >= kInfBits) o[dt][i] += x;
                 }
         }
-    const int64_t at = (T.q0 + qi) * inner + (int64_t)h * d;
+    const int64_t at = (T.first + qi) * inner + (int64_t)h * d;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll

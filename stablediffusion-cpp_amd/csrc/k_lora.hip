@@ -3,8 +3,15 @@
 // run's adapter (no reference function; the projection itself is
 // backend_cuda.h:38-43, gemm_nt_bf16 / gemm_nt_f32).
 //
-// fp32 throughout: X keeps its 24 bits (unlike the A of gemm_nt_bf16, which is
-// rounded to bf16), the weights theirs, H = X A^T and the sums are fp32.
+// Two launches: down, H = s_a X A_a^T into scratch, and up, C (+)= H B_a^T, both on
+// v_mfma_f32_32x32x16_bf16. fp32 accuracy: a float is the exact sum of three bf16
+// values (24 bits in steps of 8, cut towards zero, so nothing overflows and the range is
+// fp32's), a bf16 value its own; the products of the parts are exact in the fp32
+// accumulators. X keeps its 24 bits, unlike the A of gemm_nt_bf16. With fp32 weights the
+// product of the two smallest parts (below 2^-28) is left out.
+//
+// Both are bound by memory: X is read once (a workgroup has all ranks of its
+// rows), C read and written once, while A and B come from the L2s.
 #include <algorithm>
 #include <string>
 #include <type_traits>
@@ -15,63 +22,325 @@ namespace sdh {
 namespace {
 
 typedef unsigned short u16;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));  // 8 bf16
+using dev::f4;
 
-__device__ __forceinline__ float value(float v) { return v; }
-__device__ __forceinline__ float value(u16 b) { return __uint_as_float((unsigned)b << 16); }
+constexpr int kLoraWaves = 4, kLoraThreads = 64 * kLoraWaves;
 
-// A run of rows: its adapter and rank, the rank 0 where it has none.
-struct Run {
-    int first, rows, adapter, rank;
+// Eight values of a row on their way, and as MFMA operands.
+template <class T>
+struct Eight;
+template <>
+struct Eight<float> {
+    static constexpr int kParts = 3;
+    f4 a, b;
+    // The values p[at .. at + 7], zeros from `end` on. VEC: 16-byte aligned, and in memory all eight where the first is in
+    // front of `end` (those behind it are then cut off by the caller).
+    template <bool VEC>
+    __device__ __forceinline__ void load(const float* p, int at, int end) {
+        if constexpr (VEC) {
+            const f4* q = (const f4*)(p + (at < end ? at : 0));
+            a = q[0], b = q[1];
+            if (at >= end) a = b = f4{0.f, 0.f, 0.f, 0.f};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                a[e] = at + e < end ? p[at + e] : 0.f;
+                b[e] = at + 4 + e < end ? p[at + 4 + e] : 0.f;
+            }
+        }
+    }
+    // Zeros behind the first `n`.
+    __device__ __forceinline__ void cut(int n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (e >= n) a[e] = 0.f;
+            if (e + 4 >= n) b[e] = 0.f;
+        }
+    }
+    __device__ __forceinline__ void parts(bf16x8* out) const {
+        u32x4 hi, mid, lo;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x = i < 2 ? a[2 * i] : b[2 * i - 4], y = i < 2 ? a[2 * i + 1] : b[2 * i - 3];
+            const unsigned xh = __float_as_uint(x) & 0xFFFF0000u, yh = __float_as_uint(y) & 0xFFFF0000u;
+            const float xr = x - __uint_as_float(xh), yr = y - __uint_as_float(yh);
+            const unsigned xm = __float_as_uint(xr) & 0xFFFF0000u, ym = __float_as_uint(yr) & 0xFFFF0000u;
+            const float xl = xr - __uint_as_float(xm), yl = yr - __uint_as_float(ym);
+            hi[i] = xh >> 16 | yh;
+            mid[i] = xm >> 16 | ym;
+            lo[i] = __float_as_uint(xl) >> 16 | (__float_as_uint(yl) & 0xFFFF0000u);
+        }
+        out[0] = __builtin_bit_cast(bf16x8, hi);
+        out[1] = __builtin_bit_cast(bf16x8, mid);
+        out[2] = __builtin_bit_cast(bf16x8, lo);
+    }
 };
-__device__ __forceinline__ Run run_at(const int4* __restrict__ list, int s, int M, int adapters, int rank) {
-    const int4 e = list[s];
-    Run r{e.x, e.y, e.z, e.w};
-    dev::cut_span(r.first, r.rows, M);
-    r.rank = r.adapter < 0 || r.adapter >= adapters ? 0 : min(max(r.rank, 0), rank);
-    return r;
+template <>
+struct Eight<u16> {
+    static constexpr int kParts = 1;
+    u32x4 a;
+    template <bool VEC>
+    __device__ __forceinline__ void load(const u16* p, int at, int end) {
+        if constexpr (VEC) {
+            a = *(const u32x4*)(p + (at < end ? at : 0));
+            if (at >= end) a = u32x4{0u, 0u, 0u, 0u};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const unsigned x = at + e < end ? p[at + e] : 0u, y = at + e + 1 < end ? p[at + e + 1] : 0u;
+                a[e / 2] = x | y << 16;
+            }
+        }
+    }
+    __device__ __forceinline__ void cut(int n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] &= 2 * i >= n ? 0u : 2 * i + 1 >= n ? 0xFFFFu : ~0u;
+    }
+    __device__ __forceinline__ void parts(bf16x8* out) const { out[0] = __builtin_bit_cast(bf16x8, a); }
+};
+template <int PA, int PB>
+__device__ __forceinline__ f32x16 multiply(const bf16x8* a, const bf16x8* b, f32x16 c) {
+    // the smallest products first
+#pragma unroll
+    for (int s = PA + PB - 2 - (PA == 3 && PB == 3); s >= 0; --s)
+#pragma unroll
+        for (int i = 0; i < PA; ++i)
+            if (s - i >= 0 && s - i < PB) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[s - i], c, 0, 0, 0);
+    return c;
 }
 
-constexpr int kRowWaves = 4;
+struct Lora {
+    const void *x, *a, *b;
+    const float* scale;
+    const int4* runs;
+    float *h, *c;
+    int64_t ldx, ldc;
+    int M, N, K, rank, adapters, count, splits, hrank, accumulate;  // hrank: H's row, rank up to the next 32
+};
 
-// H[t, :] = s_a X[t] A_a^T, a wave per row.
-template <class TX, class TW>
-__global__ __launch_bounds__(64 * kRowWaves) void k_lora_down_rows(const TX* __restrict__ X, int64_t ldx, const TW* __restrict__ A,
-                                                                   const float* __restrict__ scale, const int4* __restrict__ runs, int n,
-                                                                   float* __restrict__ H, int M, int K, int rank, int adapters) {
-    const int lane = threadIdx.x & 63;
-    const int t = blockIdx.x * kRowWaves + (threadIdx.x >> 6);
-    if (t >= M) return;
-    const int s = dev::span_of_row(runs, n, t, M);
-    if (s < 0) return;
-    const Run r = run_at(runs, s, M, adapters, rank);
-    if (!r.rank) return;
-    const float f = scale ? scale[r.adapter] : 1.0f;
-    const TX* x = X + (int64_t)t * ldx;
-    for (int j = 0; j < r.rank; ++j) {
-        const TW* a = A + ((int64_t)r.adapter * rank + j) * K;
-        float v = 0.f;
-        for (int k = lane; k < K; k += 64) v = fmaf(value(x[k]), value(a[k]), v);
-        v = dev::wave_sum(v);
-        if (lane == 0) H[(int64_t)t * rank + j] = v * f;
+// The adapter of a run, -1 without one, and how many of its ranks count.
+__device__ __forceinline__ int adapter_of(const Lora& P, const dev::SpanTile& t, int& rank) {
+    const bool has = t.z >= 0 && t.z < P.adapters;
+    rank = has ? min(max(t.w, 0), P.rank) : 0;
+    return rank ? t.z : -1;
+}
+
+// ---------------------------------------------------------------------------
+// H[part][t, :] = s_a X[t] A_a^T over a share of K. A workgroup takes 32 RF rows of a run
+// and 32 RT ranks (blockIdx.z the block of ranks); K goes in blocks of 32 to its four
+// waves and to blockIdx.y's workgroups in turn. A lane reads 16 neighbouring values of
+// a row, the first eight for one MFMA step and the others for the next: whole lines,
+// and the sum does not mind the order.
+// ---------------------------------------------------------------------------
+template <class TX, class TW, int RT, int RF, bool VEC>
+__global__ __launch_bounds__(kLoraThreads) void k_lora_down(Lora P) {
+    __shared__ float part[kLoraWaves][RF * 32][33];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, fr = lane & 31, fh = lane >> 5;
+    dev::SpanTile t;
+    if (!dev::find_tile(P.runs, P.count, P.M, 1, RF * 32, blockIdx.x, t)) return;
+    int rank;
+    const int adapter = adapter_of(P, t, rank), j0 = blockIdx.z * RT * 32;
+    if (j0 >= rank) return;  // up reads none of them
+    const TX* x[RF];
+    const TW* a[RT];
+#pragma unroll
+    for (int i = 0; i < RF; ++i) x[i] = (const TX*)P.x + (t.first + min(t.row0 + i * 32 + fr, t.rows - 1)) * P.ldx;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) a[i] = (const TW*)P.a + ((int64_t)adapter * P.rank + min(j0 + i * 32 + fr, rank - 1)) * P.K;
+    f32x16 acc[RF][RT];
+#pragma unroll
+    for (int i = 0; i < RF; ++i)
+#pragma unroll
+        for (int j = 0; j < RT; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    Eight<TX> xn[2][RF];
+    Eight<TW> an[2][RT];
+    auto load = [&](int k) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int i = 0; i < RF; ++i) xn[u][i].template load<VEC>(x[i], k + fh * 16 + u * 8, P.K);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) an[u][i].template load<VEC>(a[i], k + fh * 16 + u * 8, P.K);
+        }
+    };
+    const int step = 32 * kLoraWaves * P.splits;
+    int k = (blockIdx.y * kLoraWaves + w) * 32;
+    if (k < P.K) load(k);
+    for (; k < P.K; k += step) {
+        Eight<TX> xc[2][RF];
+        Eight<TW> ac[2][RT];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int i = 0; i < RF; ++i) xc[u][i] = xn[u][i];
+#pragma unroll
+            for (int i = 0; i < RT; ++i) ac[u][i] = an[u][i];
+        }
+        if (k + step < P.K) load(k + step);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            bf16x8 xp[RF][Eight<TX>::kParts];
+#pragma unroll
+            for (int i = 0; i < RF; ++i) xc[u][i].parts(xp[i]);
+#pragma unroll
+            for (int j = 0; j < RT; ++j) {
+                bf16x8 ap[Eight<TW>::kParts];
+                ac[u][j].parts(ap);
+#pragma unroll
+                for (int i = 0; i < RF; ++i) acc[i][j] = multiply<Eight<TX>::kParts, Eight<TW>::kParts>(xp[i], ap, acc[i][j]);
+            }
+        }
+    }
+    const float f = P.scale ? P.scale[adapter] : 1.0f;
+    float* h = P.h + ((int64_t)blockIdx.y * P.M + t.first + t.row0) * P.hrank;
+    const int left = t.rows - t.row0;
+#pragma unroll
+    for (int j = 0; j < RT; ++j) {
+#pragma unroll
+        for (int i = 0; i < RF; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) part[w][i * 32 + (e >> 2) * 8 + fh * 4 + (e & 3)][fr] = acc[i][j][e];
+        __syncthreads();
+        for (int i = threadIdx.x; i < RF * 1024; i += kLoraThreads) {
+            const int row = i >> 5, c = i & 31, at = j0 + j * 32 + c;
+            const float v = (part[0][row][c] + part[1][row][c]) + (part[2][row][c] + part[3][row][c]);
+            if (row < left && at < P.hrank) h[(int64_t)row * P.hrank + at] = at < rank ? v * f : 0.f;
+        }
+        __syncthreads();
     }
 }
 
-// C[t, :] (+)= H[t] B_a^T, a thread per column.
-template <class TW>
-__global__ __launch_bounds__(256) void k_lora_up_rows(const float* __restrict__ H, const TW* __restrict__ B, const int4* __restrict__ runs,
-                                                      int n, float* __restrict__ C, int64_t ldc, int M, int N, int rank, int adapters,
-                                                      int accumulate) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    for (int t = blockIdx.y; t < M; t += gridDim.y) {
-        const int s = dev::span_of_row(runs, n, t, M);
-        if (s < 0) continue;
-        const Run r = run_at(runs, s, M, adapters, rank);
-        if (c >= N || (accumulate && !r.rank)) continue;
-        float v = 0.f;
-        const TW* b = B + ((int64_t)max(r.adapter, 0) * N + c) * rank;
-        for (int j = 0; j < r.rank; ++j) v = fmaf(H[(int64_t)t * rank + j], value(b[j]), v);
-        float* p = C + (int64_t)t * ldc + c;
-        *p = accumulate ? *p + v : v;
+// ---------------------------------------------------------------------------
+// C[t, :] (+)= H[t] B_a^T over the ranks j0 .. j0 + 16 KS. A wave keeps the parts of 32 rows
+// of H in registers and goes through `columns` columns, 32 at a time. The four waves of
+// a workgroup have neighbouring rows and the same columns (their B comes from the L1),
+// or, with FEW, the same rows and neighbouring columns.
+// ---------------------------------------------------------------------------
+template <class TW, int KS, bool FEW, bool VEC>
+__global__ __launch_bounds__(kLoraThreads) void k_lora_up(Lora P, int j0, int columns) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, fr = lane & 31, fh = lane >> 5;
+    dev::SpanTile t;
+    if (!dev::find_tile(P.runs, P.count, P.M, 1, FEW ? 32 : 32 * kLoraWaves, blockIdx.x, t)) return;
+    int rank;
+    const int adapter = adapter_of(P, t, rank);
+    const int row0 = t.row0 + (FEW ? 0 : w * 32), left = t.rows - row0;
+    int n = (FEW ? blockIdx.y * kLoraWaves + w : blockIdx.y) * columns;
+    const int n1 = min(n + columns, P.N);
+    if (left <= 0 || n >= n1 || (P.accumulate && j0 >= rank)) return;
+    const int64_t first = t.first + row0;
+    float* c = P.c + first * P.ldc;
+    if (adapter < 0) {  // only without accumulate; B may not be there at all
+        for (; n < n1; n += 32)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int r = (e >> 2) * 8 + fh * 4 + (e & 3);
+                if (n + fr < P.N && r < left) c[r * P.ldc + n + fr] = 0.f;
+            }
+        return;
+    }
+    bf16x8 hp[KS][3];
+    const float* h = P.h + (first + min(fr, left - 1)) * P.hrank;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        const int at = j0 + ks * 16 + fh * 8;
+        Eight<float> v;
+        v.a = v.b = f4{0.f, 0.f, 0.f, 0.f};
+        if (at < rank)
+            for (int s = 0; s < P.splits; ++s) {
+                const f4* q = (const f4*)(h + (int64_t)s * P.M * P.hrank + at);
+                v.a += q[0];
+                v.b += q[1];
+            }
+        v.parts(hp[ks]);
+    }
+    const TW* b = (const TW*)P.b + (int64_t)adapter * P.N * P.rank;
+    for (; n < n1; n += 32) {
+        const int col = n + fr;
+        const bool in = col < P.N;
+        Eight<TW> bn[KS];
+        const TW* row = b + (int64_t)min(col, P.N - 1) * P.rank;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) bn[ks].template load<VEC>(row, j0 + ks * 16 + fh * 8, rank);
+        if (VEC && rank % 8) {  // what lies behind the ranks that count may be anything
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) bn[ks].cut(rank - (j0 + ks * 16 + fh * 8));
+        }
+        f32x16 acc, y;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int r = (e >> 2) * 8 + fh * 4 + (e & 3);
+            acc[e] = P.accumulate && in && r < left ? c[r * P.ldc + col] : 0.f;
+            y[e] = 0.f;
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            bf16x8 bp[Eight<TW>::kParts];
+            bn[ks].parts(bp);
+            y = multiply<3, Eight<TW>::kParts>(hp[ks], bp, y);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int r = (e >> 2) * 8 + fh * 4 + (e & 3);
+            if (in && r < left) c[r * P.ldc + col] = acc[e] + y[e];
+        }
+    }
+}
+
+template <class TX, class TW>
+void launch_lora(Lora P, int64_t M, bool vec) {
+    using std::integral_constant;
+    using T_ = std::true_type;
+    using F_ = std::false_type;
+    const int cus = num_cus();
+    // Few rows a run: 32-row tiles.
+    const bool few = M <= 32 * (int64_t)P.count;
+    const int rt = P.rank <= 32 ? 1 : P.rank <= 64 ? 2 : 4, rf = few || rt > 2 || !vec ? 1 : 2;
+    const int64_t down = M / (32 * rf) + std::min<int64_t>(P.count, M);
+    if (P.rank > 0) {
+        // parts of K until the chip has two workgroups a CU, while each wave keeps two blocks
+        const int64_t most = std::max<int64_t>(1, P.K / (64 * kLoraWaves));
+        P.splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, 2 * cus / std::max<int64_t>(1, M / (32 * rf) + 1), 8}));
+    }
+    P.hrank = (P.rank + 31) / 32 * 32;
+    P.h = (float*)scratch(std::max<size_t>((size_t)P.splits * M * P.hrank * 4, 4));
+    if (P.rank > 0) {
+        const dim3 grid((unsigned)down, (unsigned)P.splits, (unsigned)((P.rank + rt * 32 - 1) / (rt * 32)));
+        auto go = [&](auto r, auto f, auto v) {
+            k_lora_down<TX, TW, decltype(r)::value, decltype(f)::value, decltype(v)::value><<<grid, kLoraThreads, 0, stream()>>>(P);
+        };
+        using One = integral_constant<int, 1>;
+        using Two = integral_constant<int, 2>;
+        using Four = integral_constant<int, 4>;
+        if (rt == 1) vec ? (rf == 2 ? go(One(), Two(), T_()) : go(One(), One(), T_())) : go(One(), One(), F_());
+        else if (rt == 2) vec ? (rf == 2 ? go(Two(), Two(), T_()) : go(Two(), One(), T_())) : go(Two(), One(), F_());
+        else vec ? go(Four(), One(), T_()) : go(Four(), One(), F_());
+    }
+    const int64_t tiles = M / (few ? 32 : 128) + std::min<int64_t>(P.count, M);
+    // columns a wave: enough waves to fill the chip, at most 512
+    const int64_t waves = std::max<int64_t>(1, M / 32 + (few ? P.count : 0));
+    int64_t columns = 512;
+    while (columns > 32 && waves * ((P.N + columns - 1) / columns) < 16 * (int64_t)cus) columns /= 2;
+    const bool bvec = P.rank % 8 == 0 && aligned16(P.b);
+    for (int j0 = 0; j0 == 0 || j0 < P.rank; j0 += 128) {
+        const int ks = std::min(P.rank - j0, 128);
+        const dim3 grid((unsigned)tiles, (unsigned)((P.N + columns * (few ? kLoraWaves : 1) - 1) / (columns * (few ? kLoraWaves : 1))));
+        auto go = [&](auto k, auto f, auto v) {
+            k_lora_up<TW, decltype(k)::value, decltype(f)::value, decltype(v)::value><<<grid, kLoraThreads, 0, stream()>>>(P, j0, (int)columns);
+        };
+        auto with = [&](auto f, auto v) {
+            if (ks <= 16) go(integral_constant<int, 1>(), f, v);
+            else if (ks <= 32) go(integral_constant<int, 2>(), f, v);
+            else if (ks <= 64) go(integral_constant<int, 4>(), f, v);
+            else go(integral_constant<int, 8>(), f, v);
+        };
+        if (few) bvec ? with(T_(), T_()) : with(T_(), F_());
+        else bvec ? with(F_(), T_()) : with(F_(), F_());
+        P.accumulate = 1;
     }
 }
 
@@ -105,14 +374,11 @@ void run_lora(const char* op, int64_t M, int64_t N, int64_t K, const TX* X, int6
     } else if (accumulate) {
         return;
     }
-    const int r = any ? (int)rank : 0, na = any ? (int)adapters : 0;
-    float* H = (float*)scratch(std::max<size_t>((size_t)(M * r) * 4, 4));
-    need((M + kRowWaves - 1) / kRowWaves * 64 * kRowWaves <= kMaxGridItems && N <= kMaxGridItems - 256, op, "matrix too large for one launch");
-    if (any)
-        k_lora_down_rows<TX, TW><<<blocks_for(M, kRowWaves), 64 * kRowWaves, 0, stream()>>>(X, ldx, A, scale, (const int4*)segments, (int)count, H,
-                                                                                         (int)M, (int)K, r, na);
-    k_lora_up_rows<TW><<<dim3(blocks_for(N, 256), (unsigned)std::min<int64_t>(M, 65535)), 256, 0, stream()>>>(H, B, (const int4*)segments, (int)count, C, ldc, (int)M,
-                                                                                   (int)N, r, na, accumulate ? 1 : 0);
+    need((N + 31) / 32 <= 65535 && (M / 32 + std::min(count, M) + 1) * kLoraThreads <= kMaxGridItems, op, "matrix too large for one launch");
+    Lora P{X, A, B, scale, (const int4*)segments, nullptr, C, ldx, ldc, (int)M, (int)N, (int)K, any ? (int)rank : 0, any ? (int)adapters : 0,
+           (int)count, 1, 0, accumulate ? 1 : 0};
+    const bool vec = K % 8 == 0 && ldx % (16 / sizeof(TX)) == 0 && aligned16(X) && aligned16(A);
+    launch_lora<TX, TW>(P, M, vec);
     launched(op);
 }
 

@@ -42,5 +42,41 @@ __device__ __forceinline__ int span_of_row(const int4* __restrict__ list, int n,
     return -1;
 }
 
+// A workgroup's place among the row tiles of all entries.
+struct SpanTile {
+    int index;        // the entry
+    int first, rows;  // its rows, cut to the tensor
+    int z, w;         // its other two words
+    int row0;         // the tile's first row within it, in rows times `mult`
+};
+// Entries have ceil(rows * mult / tile_rows) tiles each, numbered through; false past
+// the last one. Every lane of a wave gets the answer. rows * mult < 2^30 for all.
+__device__ __forceinline__ bool find_tile(const int4* __restrict__ list, int n, int total, int mult, int tile_rows, int item,
+                                          SpanTile& t) {
+    const int lane = threadIdx.x & 63;
+    for (int s0 = 0, before = 0; s0 < n; s0 += 64) {
+        int4 e = make_int4(0, 0, 0, 0);
+        if (s0 + lane < n) {
+            e = list[s0 + lane];
+            cut_span(e.x, e.y, total);
+        }
+        const int tiles = (e.y * mult + tile_rows - 1) / tile_rows;
+        const int upto = before + wave_scan(tiles);
+        const unsigned long long m = __ballot(item < upto);
+        if (m) {
+            const int at = (int)__ffsll(m) - 1;
+            t.index = s0 + at;
+            t.first = __builtin_amdgcn_readlane(e.x, at);
+            t.rows = __builtin_amdgcn_readlane(e.y, at);
+            t.z = __builtin_amdgcn_readlane(e.z, at);
+            t.w = __builtin_amdgcn_readlane(e.w, at);
+            t.row0 = (item - __builtin_amdgcn_readlane(upto - tiles, at)) * tile_rows;
+            return true;
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
+}
+
 }  // namespace dev
 }  // namespace sdh
