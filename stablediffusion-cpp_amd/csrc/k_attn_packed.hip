@@ -21,6 +21,8 @@ namespace sdh {
 namespace {
 
 typedef unsigned short u16;
+typedef float f2 __attribute__((ext_vector_type(2)));
+using dev::f4;
 constexpr float kLog2e = 1.44269504088896341f;
 
 struct Packed {
@@ -163,8 +165,14 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_attn_packed_rows(Packed P) {
 // ---------------------------------------------------------------------------
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f2 __attribute__((ext_vector_type(2)));
-using dev::f4;
+
+// Where the keys of a row are cut into parts (S.n of them, by blockIdx.y): each part's
+// sum of weighted values, and its reference and sum of weights, for k_attn_packed_join.
+struct Parts {
+    int n, stride;  // floats of a cell: d up to the next 4
+    float* o;       // [Tq, heads, n, stride]
+    f2* ml;         // [Tq, heads, n]
+};
 
 constexpr int kKT = 64, kWaves = 8, kThreads = 64 * kWaves, kTileRows = 32 * kWaves;
 // The reference m of the weights is raised when a tile's largest score passes it by more
@@ -206,7 +214,7 @@ __device__ __forceinline__ int block_exp(int bits) { return min(max((bits >> 23)
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(127 + e) << 23); }  // e in [-126, 127]
 
 template <int DP, bool OUT16, bool EXTRA, bool VEC>
-__global__ __launch_bounds__(kThreads, 1) void k_attn_packed_tiles(Packed P, int items) {
+__global__ __launch_bounds__(kThreads, 1) void k_attn_packed_tiles(Packed P, int items, Parts S) {
     constexpr int DS = DP / 16, DT = DP / 32, KU = DP / 64, PART = kKT * DP;
     // [K hi][K lo][V^T hi][V^T lo] of two tiles
     __shared__ __attribute__((aligned(1024))) u16 buf[2][4 * PART];
@@ -237,7 +245,8 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_packed_tiles(Packed P, int
     const bool active = T.row0 + w * 32 < rows;
     const int first_lo = __builtin_amdgcn_readlane(see.lo, 0), last_hi = __builtin_amdgcn_readlane(see.hi, 31);
     const int npre = (pre + kKT - 1) / kKT, next = max(npre, wg_lo / kKT);
-    const int nt = npre + (wg_hi > wg_lo ? max(0, (wg_hi + kKT - 1) / kKT - next) : 0);
+    const int all = npre + (wg_hi > wg_lo ? max(0, (wg_hi + kKT - 1) / kKT - next) : 0);
+    const int n0 = (int)((int64_t)all * blockIdx.y / S.n), nt = (int)((int64_t)all * (blockIdx.y + 1) / S.n);
     auto key_of = [&](int n) { return (n < npre ? n : next + n - npre) * kKT; };
 
     // Q: the B operand of S^T, row qi of head h, dims ds*16 + fh*8 .. +7
@@ -571,11 +580,11 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_packed_tiles(Packed P, int
     };
 
     int bad_first = nt, bad_last = -1;  // the tiles that hold values that are not finite
-    if (nt > 0) {
-        fetch(0);
-        store(0, 0);
+    if (n0 < nt) {
+        fetch(n0);
+        store(n0, n0 & 1);
     }
-    for (int n = 0; n < nt; ++n) {
+    for (int n = n0; n < nt; ++n) {
         const int b = n & 1, k0 = key_of(n);
         if (n + 1 < nt) fetch(n + 1);
         // tile n is in LDS, and nobody reads tile n - 1 any more
@@ -597,7 +606,9 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_packed_tiles(Packed P, int
 
     if (r >= rows) return;
     sum += __shfl_xor(sum, 32, 64);
-    const float inv = sum == 0.f ? 0.f : ldexpf(1.0f / sum, E - 14);
+    const int64_t cell = ((int64_t)(T.first + qi) * P.heads + h) * S.n + blockIdx.y;
+    // a part of the keys: the sums as they are, on the scale of the reference
+    const float inv = sum == 0.f ? 0.f : ldexpf(S.n > 1 ? 1.0f : 1.0f / sum, E - 14);
     for (int n = bad_first; n <= bad_last; ++n)
         for (int j = key_of(n), end = min(j + kKT, lk); j < end; ++j) {
             if (!visible(j)) continue;
@@ -610,6 +621,18 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_packed_tiles(Packed P, int
                     if (abs_bits(x) >= kInfBits) o[dt][i] += x;
                 }
         }
+    if (S.n > 1) {
+        if (fh == 0) S.ml[cell] = f2{m, sum};
+        float* to = S.o + cell * S.stride;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int c = dt * 32 + g * 8 + fh * 4;
+                if (c < d) *(f4*)(to + c) = f4{o[dt][g * 4] * inv, o[dt][g * 4 + 1] * inv, o[dt][g * 4 + 2] * inv, o[dt][g * 4 + 3] * inv};
+            }
+        return;
+    }
     const int64_t at = (T.first + qi) * inner + (int64_t)h * d;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -632,15 +655,255 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_packed_tiles(Packed P, int
         }
 }
 
+// ---------------------------------------------------------------------------
+// Few rows a sequence (single tokens): fp32 on the vector ALUs, R rows of one
+// key/value head a workgroup, each key and value read once for all of them.
+//
+// DP / 4 lanes have a key, four of its values each (whole rows of 64 or 128 values a load,
+// 2 or 4 keys), a wave kLoads loads of keys and as many of values at once. Every group of
+// lanes keeps a softmax of its own keys; they are put together at the end.
+// ---------------------------------------------------------------------------
+constexpr int kLoads = 8, kFewWaves = 4;
+
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {  // over aligned groups of 16 or 32
+    v = dev::group_sum<16>(v);
+    if constexpr (LANES == 32) {
+        const unsigned b = __float_as_uint(v);
+        const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);  // the two 16-lane rows side by side
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    return v;
+}
+
+template <int DP, int R, bool EXTRA>
+__global__ __launch_bounds__(64 * kFewWaves) void k_attn_packed_few(Packed P, int out16, Parts S) {
+    constexpr int LANES = DP / 4, KEYS = 64 / LANES, CHUNK = kLoads * KEYS, GROUPS = kFewWaves * KEYS;
+    __shared__ float so[GROUPS][R][DP];
+    __shared__ float sm[GROUPS][R], sl[GROUPS][R];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int sub = lane / LANES, c4 = lane % LANES * 4, d = P.d;
+    const int group = P.heads / P.kv_heads, kh = blockIdx.x % P.kv_heads;
+    dev::SpanTile T;
+    if (!dev::find_tile(P.spans, P.seqs, P.Tq, group, R, blockIdx.x / P.kv_heads, T)) return;
+    dev::cut_span(T.z, T.w, P.Tk);
+    const int lk = T.w, rows = T.rows * group, left = min(rows - T.row0, R), shift = lk - T.rows;
+    const int pre = P.prefix ? min(max(P.prefix[T.index], 0), lk) : 0;
+    const int64_t inner = (int64_t)P.heads * d, kv_inner = (int64_t)P.kv_heads * d;
+    f4 q[R], o[R];
+    float m[R], sum[R];
+    int place[R], lo[R], hi[R], head[R];
+    const float f = EXTRA ? P.scale : P.scale * kLog2e;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int rr = T.row0 + min(r, left - 1), qi = rr / group;
+        head[r] = kh * group + rr - qi * group;
+        place[r] = qi + shift;
+        const Seen see = seen_from(P, place[r], lk, pre);
+        lo[r] = see.lo, hi[r] = see.hi;
+        const float* a = P.q + (T.first + qi) * inner + (int64_t)head[r] * d;
+        q[r] = c4 < d ? *(const f4*)(a + c4) * f : f4{0.f, 0.f, 0.f, 0.f};
+        o[r] = f4{0.f, 0.f, 0.f, 0.f};
+        m[r] = -INFINITY, sum[r] = 0.f;
+    }
+    const int npre = (pre + CHUNK - 1) / CHUNK, next = max(npre, lo[0] / CHUNK);
+    const int all = npre + (hi[R - 1] > lo[0] ? max(0, (hi[R - 1] + CHUNK - 1) / CHUNK - next) : 0);
+    const int n0 = (int)((int64_t)all * blockIdx.y / S.n), n1 = (int)((int64_t)all * (blockIdx.y + 1) / S.n);
+    const int64_t base = T.z * kv_inner + (int64_t)kh * d + (c4 < d ? c4 : 0);
+    for (int n = n0 + w; n < n1; n += kFewWaves) {
+        const int k0 = (n < npre ? n : next + n - npre) * CHUNK;
+        f4 kx[kLoads], vx[kLoads];
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) kx[u] = *(const f4*)(P.k + base + min(k0 + u * KEYS + sub, lk - 1) * kv_inner);
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) vx[u] = *(const f4*)(P.v + base + min(k0 + u * KEYS + sub, lk - 1) * kv_inner);
+        const bool full = k0 + CHUNK <= pre || (k0 >= lo[R - 1] && k0 + CHUNK <= hi[0]);
+        auto visible = [&](int u, int r) {
+            const int j = k0 + u * KEYS + sub;
+            return (j < pre) | ((j >= lo[r]) & (j < hi[r]));
+        };
+        float s[kLoads][R];
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                s[u][r] = lanes_sum<LANES>(fmaf(q[r].x, kx[u].x, q[r].y * kx[u].y) + fmaf(q[r].z, kx[u].z, q[r].w * kx[u].w));
+        if constexpr (EXTRA) {
+#pragma unroll
+            for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    if (P.cap > 0.f) s[u][r] = P.cap * tanh_near(s[u][r] / P.cap);
+                    if (P.bias)
+                        s[u][r] += P.bias[(int64_t)head[r] * (2 * P.radius + 1) + P.radius +
+                                          min(max(k0 + u * KEYS + sub - place[r], -P.radius), P.radius)];
+                }
+        }
+        if (!full) {
+#pragma unroll
+            for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    if (!visible(u, r)) s[u][r] = -INFINITY;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float mx = s[0][r];
+#pragma unroll
+            for (int u = 1; u < kLoads; ++u) mx = fmaxf(mx, s[u][r]);
+            const float mnew = fmaxf(m[r], mx), ref = mnew == -INFINITY ? 0.f : mnew;
+            const float alpha = __builtin_amdgcn_exp2f(EXTRA ? (m[r] - ref) * kLog2e : m[r] - ref);
+            m[r] = mnew;
+            sum[r] *= alpha;
+            o[r] *= alpha;
+#pragma unroll
+            for (int u = 0; u < kLoads; ++u) {
+                s[u][r] = __builtin_amdgcn_exp2f(EXTRA ? (s[u][r] - ref) * kLog2e : s[u][r] - ref);
+                sum[r] += s[u][r];
+            }
+        }
+        if (full) {
+#pragma unroll
+            for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+                for (int r = 0; r < R; ++r) o[r] += s[u][r] * vx[u];
+        } else {
+#pragma unroll
+            for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    if (visible(u, r)) o[r] += s[u][r] * vx[u];  // 0 * inf is not zero
+        }
+    }
+    const int g0 = w * KEYS + sub;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        *(f4*)&so[g0][r][c4] = o[r];
+        if (c4 == 0) sm[g0][r] = m[r], sl[g0][r] = sum[r];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < left * LANES; i += 64 * kFewWaves) {
+        const int r = i / LANES, c = i % LANES * 4;
+        float top = sm[0][r];
+#pragma unroll
+        for (int g = 1; g < GROUPS; ++g) top = fmaxf(top, sm[g][r]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        f4 v = {0.f, 0.f, 0.f, 0.f};
+        float l = 0.f;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            const float x = __builtin_amdgcn_exp2f(EXTRA ? (sm[g][r] - ref) * kLog2e : sm[g][r] - ref);
+            l = fmaf(x, sl[g][r], l);
+            v += x * *(const f4*)&so[g][r][c];
+        }
+        if (c >= d) continue;
+        const int rr = T.row0 + r, qi = rr / group, h = kh * group + rr - qi * group;
+        const int64_t row = (int64_t)(T.first + qi) * P.heads + h;
+        if (S.n > 1) {
+            const int64_t cell = row * S.n + blockIdx.y;
+            if (c == 0) S.ml[cell] = f2{top, l};
+            *(f4*)(S.o + cell * S.stride + c) = v;
+        } else {
+            v *= l == 0.f ? 0.f : 1.0f / l;
+            if (out16) *(uint2*)((u16*)P.out + row * d + c) = dev::bf16x4(v);
+            else *(f4*)((float*)P.out + row * d + c) = v;
+        }
+    }
+}
+
+// out from the parts: a workgroup of eight 32-lane groups per (query row, head), each taking
+// every eighth part. `unit`: log2(e) where the references are not in log2 units.
+__global__ __launch_bounds__(256) void k_attn_packed_join(Packed P, int out16, Parts S, float unit) {
+    __shared__ float so[8][128];
+    __shared__ float sm[8], sl[8];
+    const int t = blockIdx.x, h = blockIdx.y, c = (threadIdx.x & 31) * 4, g = threadIdx.x >> 5;
+    if (dev::span_of_row(P.spans, P.seqs, t, P.Tq) < 0) return;
+    const int64_t row = (int64_t)t * P.heads + h, cell = row * S.n;
+    float top = -INFINITY, l = 0.f;
+    f4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s = g; s < S.n; s += 8) {
+        const f2 ml = S.ml[cell + s];
+        const float mnew = fmaxf(top, ml.x), ref = mnew == -INFINITY ? 0.f : mnew;
+        const float keep = __builtin_amdgcn_exp2f((top - ref) * unit), add = __builtin_amdgcn_exp2f((ml.x - ref) * unit);
+        l = l * keep + ml.y * add;
+        if (c < P.d) v = v * keep + *(const f4*)(S.o + (cell + s) * S.stride + c) * add;
+        top = mnew;
+    }
+    *(f4*)&so[g][c] = v;
+    if (c == 0) sm[g] = top, sl[g] = l;
+    __syncthreads();
+    if (g || c >= P.d) return;
+    top = sm[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, sm[i]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    v = f4{0.f, 0.f, 0.f, 0.f};
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float x = __builtin_amdgcn_exp2f((sm[i] - ref) * unit);
+        l = fmaf(x, sl[i], l);
+        v += x * *(const f4*)&so[i][c];
+    }
+    v *= l == 0.f ? 0.f : 1.0f / l;
+    const int64_t at = row * P.d + c;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (c + e < P.d) {
+            if (out16) ((u16*)P.out)[at + e] = dev::bf16_rne(v[e]);
+            else ((float*)P.out)[at + e] = v[e];
+        }
+}
+
+// The parts' memory, in scratch; the keys uncut where it cannot be had.
+Parts make_parts(const Packed& P, int64_t n) {
+    Parts S{(int)n, (P.d + 3) / 4 * 4, nullptr, nullptr};
+    const size_t cells = (size_t)P.Tq * P.heads * n, ob = (cells * S.stride * 4 + 255) / 256 * 256;
+    char* base = n > 1 ? (char*)try_scratch(ob + cells * sizeof(f2)) : nullptr;
+    if (!base) S.n = 1;
+    S.o = (float*)base;
+    S.ml = base ? (f2*)(base + ob) : nullptr;
+    return S;
+}
+
+void join_parts(const Packed& P, bool out16, const Parts& S, bool log2_units) {
+    if (S.n > 1)
+        k_attn_packed_join<<<dim3((unsigned)P.Tq, (unsigned)P.heads), 256, 0, stream()>>>(P, out16, S, log2_units ? 1.0f : kLog2e);
+}
+
+template <int DP>
+void run_few(const Packed& P, bool out16, int64_t items, int rows) {
+    const bool extra = P.cap > 0.f || P.bias;
+    // Parts of the keys until there are eight workgroups a CU, each wave with two chunks of an average sequence.
+    const int64_t wgs = items * P.kv_heads, keys = P.Tk / std::max(1, P.seqs);
+    const Parts S = make_parts(P, std::max<int64_t>(1, std::min<int64_t>({8 * num_cus() / wgs, keys / (kFewWaves * 64), 256})));
+    auto go = [&](auto r, auto ex) {
+        k_attn_packed_few<DP, decltype(r)::value, decltype(ex)::value>
+            <<<dim3((unsigned)wgs, (unsigned)S.n), 64 * kFewWaves, 0, stream()>>>(P, out16, S);
+    };
+    auto with = [&](auto ex) {
+        using std::integral_constant;
+        if (rows <= 1) go(integral_constant<int, 1>(), ex);
+        else if (rows <= 4) go(integral_constant<int, 4>(), ex);
+        else go(integral_constant<int, 8>(), ex);
+    };
+    if (extra) with(std::true_type());
+    else with(std::false_type());
+    join_parts(P, out16, S, !extra);
+}
+
 template <int DP>
 void run_tiles(const Packed& P, bool out16, int64_t items) {
     const bool vec = P.d % 8 == 0 && aligned16(P.q) && aligned16(P.k) && aligned16(P.v) && (out16 ? ((uintptr_t)P.out & 7) == 0 : aligned16(P.out));
     const bool extra = P.cap > 0.f || P.bias;
     using T_ = std::true_type;
     using F_ = std::false_type;
+    // Parts of the keys while the workgroups do not fill the chip, of eight tiles of an average sequence at least.
+    const int64_t wgs = items * P.kv_heads, keys = P.Tk / std::max(1, P.seqs);
+    const Parts S = make_parts(P, std::max<int64_t>(1, std::min<int64_t>(num_cus() / wgs, keys / (8 * kKT))));
     auto go = [&](auto o16, auto ex, auto ve) {
         k_attn_packed_tiles<DP, decltype(o16)::value, decltype(ex)::value, decltype(ve)::value>
-            <<<(unsigned)(items * P.kv_heads), kThreads, 0, stream()>>>(P, (int)items);
+            <<<dim3((unsigned)wgs, (unsigned)S.n), kThreads, 0, stream()>>>(P, (int)items, S);
     };
     auto with = [&](auto o16) {
         if (extra) vec ? go(o16, T_(), T_()) : go(o16, T_(), F_());
@@ -648,6 +911,7 @@ void run_tiles(const Packed& P, bool out16, int64_t items) {
     };
     if (out16) with(T_());
     else with(F_());
+    join_parts(P, out16, S, !extra);
 }
 
 void run_attention_packed(const float* q, const float* k, const float* v, void* out, bool out16, int64_t Tq, int64_t Tk, int heads,
@@ -683,7 +947,19 @@ void run_attention_packed(const float* q, const float* k, const float* v, void* 
     Packed P{q,    k,   v,   out, (const int4*)spans, prefix, bias, (int)Tq, (int)Tk, (int)seqs, heads, kv_heads, (int)d, causal ? 1 : 0,
              window < kMost ? (int)window : 0,  // a wider one hides nothing
              bias ? (int)radius : 0, scale, cap};
-    const int64_t rows = Tq * (heads / kv_heads), items = rows / kTileRows + std::min(seqs, Tq);
+    // A sequence's rows at one key/value head are few: see k_attn_packed_few.
+    const int64_t group = heads / kv_heads, live = std::min(seqs, Tq), mean = (Tq + live - 1) / live * group;
+    if (d <= 128 && d % 4 == 0 && mean <= 8 && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out)) {
+        const int r = mean <= 1 ? 1 : mean <= 4 ? 4 : 8;
+        const int64_t n = Tq * group / r + live;
+        if (Tq * group < kMost && n * kv_heads * 64 * kFewWaves <= kMaxGridItems) {
+            if (d <= 64) run_few<64>(P, out16, n, r);
+            else run_few<128>(P, out16, n, r);
+            launched(op);
+            return;
+        }
+    }
+    const int64_t rows = Tq * group, items = rows / kTileRows + live;
     if (d <= 128 && rows < kMost && items * kv_heads * kThreads <= kMaxGridItems) {
         if (d <= 64) run_tiles<64>(P, out16, items);
         else run_tiles<128>(P, out16, items);
