@@ -139,29 +139,33 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_attn_packed_rows(Packed P) {
 }
 
 // ---------------------------------------------------------------------------
-// Head dimensions up to 128 (padded to DP = 64 or 128), on the MFMA units.
+// Head dimensions up to 128 (padded to DP = 64 or 128), on the MFMA units, in two launches.
 //
-// A workgroup takes kTileRows rows of one sequence and key/value head, a row being a
-// (query, head of the group) pair, heads fastest: the heads that share a key/value head
-// share its tiles. It walks the 64-key tiles that any of its rows sees. The eight waves
-// bring a tile in together, eight keys each, from fp32 in memory to fp16 pairs in LDS,
-// and each wave then takes 32 rows against it.
+// k_attn_packed_split cuts k and v of a key/value head into tiles of 64 rows (of the
+// tensor: a tile may hold rows of several sequences) in library scratch, as fp16 pairs in
+// the order of the fragments' reads; a tile that no sequence reads is left out.
+// k_attn_packed_tiles takes kTileRows rows of one sequence and key/value head a workgroup,
+// a row being a (query, head of the group) pair, heads fastest: the heads that share a
+// key/value head share its tiles. It copies the tiles that any of its rows sees to LDS, and
+// each of its four waves takes 32 rows against them. Two workgroups fit a CU: while the
+// waves of one are at their MFMAs those of the other take exponentials.
 //
 // Operands are fp16 pairs hi + lo in block floating point, products hi hi + hi lo +
-// lo hi with fp32 sums (2^-21 of each product). A block is a row of q, or the eight keys
-// that a wave brought in: with k or v scaled by 2^-e to at most 2^14, a score is
-// s 2^(e_q + e_k), and a weight is formed as p 2^(14 + e_v - E), E the largest e_v that the
-// lane's row has seen, so that the sums of all blocks share the scale 2^(14 - E).
-// Rows in LDS are ordered so that the eight scores of a lane's half of a 16-key step are
-// eight neighbouring keys: one block, one exponent. Tiles at the border of what the rows
-// see have an exponent for each key: an unseen key, whatever its size, then has no say
-// in the others'. Values that are not finite go into the tiles as zeros, since 0 * inf would
-// reach the rows that do not see them, and are added at the end; a key that is not finite
-// makes the scores of the rows that see it NaN, and only those.
+// lo hi with fp32 sums (2^-21 of each product). A block is a row of q, or a tile of k or
+// v: scaled by 2^-e to at most 2^14, a score is s 2^(e_q + e_k), and a weight is formed as
+// p 2^(14 + e_v - E), E the largest e_v that the lane's row has met, so that the sums of
+// all tiles share the scale 2^(14 - E). The pair holds 22 bits down to 2^-16 of its
+// block's largest value.
+//   A key that a row does not see must not cost it bits: a tile whose keys are more than
+// 2^kSpread apart has an exponent for each key, and a row leaves E to the keys that it
+// sees. Values that are not finite go into the tiles as zeros, since 0 * inf would reach
+// the rows that do not see them, and are added at the end; a key that is not finite makes
+// the scores of the rows that see it NaN, and only those.
 //
 // S^T = K Q^T and O^T = V^T P^T by v_mfma_f32_32x32x16_f16: lane l holds row l % 32 of
-// the wave in both, its statistics are its own, and its weights are the second product's
-// operand as they lie.
+// the wave in both, its statistics are its own. K's rows are ordered so that the eight
+// scores of a lane's half of a 16-key step are eight neighbouring keys: its weights
+// are the second product's operand as they lie, V^T in the keys' own order.
 // ---------------------------------------------------------------------------
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -174,11 +178,12 @@ struct Parts {
     f2* ml;         // [Tq, heads, n]
 };
 
-constexpr int kKT = 64, kWaves = 8, kThreads = 64 * kWaves, kTileRows = 32 * kWaves;
+constexpr int kKT = 64, kWaves = 4, kThreads = 64 * kWaves, kTileRows = 32 * kWaves;
 // The reference m of the weights is raised when a tile's largest score passes it by more
 // than this (in units of log2): weights stay below 2^(14 + kLazy), inside fp16.
 constexpr float kLazy = 1.5f;
 constexpr int kUnsetE = -1000;  // no values seen yet
+constexpr int kSpread = 8;
 constexpr int kFarE = -40;      // weights' exponents relative to E are not taken below this (2^-40 of the largest sum)
 
 __device__ __forceinline__ int swz_v(int r) { return (r >> 1) & 7; }
@@ -206,6 +211,21 @@ __device__ __forceinline__ int group_imax(int v) {
     }
     return v;
 }
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+// The larger of each half over the wave's lanes.
+__device__ __forceinline__ unsigned wave_max_halves(unsigned v) {
+    auto larger = [](unsigned a, unsigned b) {
+        return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(us2, a), __builtin_bit_cast(us2, b)));
+    };
+    v = larger(v, dpp_i<0xB1>(v));
+    v = larger(v, dpp_i<0x4E>(v));
+    v = larger(v, dpp_i<0x141>(v));
+    v = larger(v, dpp_i<0x140>(v));
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = larger(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return larger(b[0], b[1]);
+}
 __device__ __forceinline__ int abs_bits(float x) { return (int)(__float_as_uint(x) & 0x7FFFFFFFu); }
 constexpr int kInfBits = 0x7F800000;
 // The exponent that brings a block's largest magnitude into [2^13, 2^14); zero and
@@ -213,14 +233,159 @@ constexpr int kInfBits = 0x7F800000;
 __device__ __forceinline__ int block_exp(int bits) { return min(max((bits >> 23) - 140, -126), 126); }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(127 + e) << 23); }  // e in [-126, 127]
 
-template <int DP, bool OUT16, bool EXTRA, bool VEC>
-__global__ __launch_bounds__(kThreads, 1) void k_attn_packed_tiles(Packed P, int items, Parts S) {
-    constexpr int DS = DP / 16, DT = DP / 32, KU = DP / 64, PART = kKT * DP;
-    // [K hi][K lo][V^T hi][V^T lo] of two tiles
-    __shared__ __attribute__((aligned(1024))) u16 buf[2][4 * PART];
-    __shared__ __attribute__((aligned(16))) int exps[2][2][8];      // of k, v, eight keys each
-    __shared__ __attribute__((aligned(16))) int key_exps[2][2][kKT];  // at a border: of each key
-    __shared__ __attribute__((aligned(16))) int bads[2][8];         // values that are not finite
+// A tile's exponents of k and v, and what is special about it.
+enum { kKeyExps = 1, kValueExps = 2, kNotFinite = 4 };
+struct Tiles {
+    u16* data;   // [kv_heads, n, 4 * 64 DP]: K hi, K lo, V^T hi, V^T lo
+    int4* info;  // [kv_heads, n]: e_k, e_v, flags
+    int* exps;   // [kv_heads, n, 2, 64]: of the keys, where the flags say so
+    int n;
+};
+
+template <int DP, bool VEC>
+__global__ __launch_bounds__(64 * kWaves) void k_attn_packed_split(Packed P, Tiles X) {
+    constexpr int PART = kKT * DP, KCH = DP / 8, KROWS = 64 / KCH, KU = 16 / KROWS;  // 16-byte chunks of a K row, rows of a wave's load, loads
+    constexpr int VU = DP / 64;                                                     // columns of v a lane has
+    __shared__ int tops[2][kWaves], flags[kWaves];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tile = blockIdx.x, kh = blockIdx.y, j0 = tile * kKT + w * 16, d = P.d;
+    const int64_t kv_inner = (int64_t)P.kv_heads * d;
+    const int kch = lane & (KCH - 1), krow = lane / KCH;
+    // sixteen keys a wave; k: 16-byte chunks of their rows, v: the lane's columns of all of them
+    float kx[KU][8], vx[16][VU];
+#pragma unroll
+    for (int u = 0; u < KU; ++u) {
+        const float* a = P.k + min(j0 + u * KROWS + krow, P.Tk - 1) * kv_inner + (int64_t)kh * d;
+        if constexpr (VEC) {
+            a += min(kch * 8, d - 8);
+            const f4 x = *(const f4*)a, y = *(const f4*)(a + 4);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) kx[u][e] = e < 4 ? x[e & 3] : y[e & 3];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) kx[u][e] = a[min(kch * 8 + e, d - 1)];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float* a = P.v + min(j0 + i, P.Tk - 1) * kv_inner + (int64_t)kh * d;
+        if constexpr (VEC && VU == 2) {
+            const f2 x = *(const f2*)(a + min(lane * 2, d - 2));
+            vx[i][0] = x.x, vx[i][1] = x.y;
+        } else {
+#pragma unroll
+            for (int u = 0; u < VU; ++u) vx[i][u] = a[min(lane * VU + u, d - 1)];
+        }
+    }
+    bool read = false;
+    for (int s0 = 0; s0 < P.seqs && !read; s0 += 64) {
+        int4 e = make_int4(0, 0, 0, 0);
+        if (s0 + lane < P.seqs) {
+            e = P.spans[s0 + lane];
+            dev::cut_span(e.z, e.w, P.Tk);
+        }
+        read = __ballot(e.y > 0 && e.w > 0 && e.z < tile * kKT + kKT && e.z + e.w > tile * kKT) != 0;
+    }
+    if (!read) return;
+    // a key's largest magnitudes, rows past the tensor and columns past d zero, and what is not finite
+    int ktop[KU], vtop[16], kmost = 0, vmost = 0, flag = 0;
+#pragma unroll
+    for (int u = 0; u < KU; ++u) {
+        ktop[u] = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (j0 + u * KROWS + krow >= P.Tk || kch * 8 + e >= d) kx[u][e] = 0.f;
+            ktop[u] = max(ktop[u], abs_bits(kx[u][e]));
+        }
+        ktop[u] = group_imax<KCH>(ktop[u]);
+        if (ktop[u] < kInfBits) kmost = max(kmost, ktop[u]);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        vtop[i] = 0;
+#pragma unroll
+        for (int u = 0; u < VU; ++u) {
+            if (j0 + i >= P.Tk || lane * VU + u >= d) vx[i][u] = 0.f;
+            if (abs_bits(vx[i][u]) >= kInfBits) vx[i][u] = 0.f, flag = kNotFinite;
+            vtop[i] = max(vtop[i], abs_bits(vx[i][u]));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {  // the upper halves order as the values do
+        const unsigned both = wave_max_halves(((unsigned)vtop[i] >> 16) | ((unsigned)vtop[i + 1] & 0xFFFF0000u));
+        vtop[i] = (int)(both << 16);
+        vtop[i + 1] = (int)(both & 0xFFFF0000u);
+        vmost = max(vmost, max(vtop[i], vtop[i + 1]));
+    }
+    kmost = group_imax<64>(kmost);
+    if (lane == 0) tops[0][w] = kmost, tops[1][w] = vmost;
+    __syncthreads();
+    kmost = max(max(tops[0][0], tops[0][1]), max(tops[0][2], tops[0][3]));
+    vmost = max(max(tops[1][0], tops[1][1]), max(tops[1][2], tops[1][3]));
+#pragma unroll
+    for (int u = 0; u < KU; ++u)
+        if (ktop[u] && abs((kmost >> 23) - (ktop[u] >> 23)) > kSpread) flag |= kKeyExps;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        if (vtop[i] && (vmost >> 23) - (vtop[i] >> 23) > kSpread) flag |= kValueExps;
+    flag = (__ballot(flag & kKeyExps) ? kKeyExps : 0) | (__ballot(flag & kValueExps) ? kValueExps : 0) | (__ballot(flag & kNotFinite) ? kNotFinite : 0);
+    if (lane == 0) flags[w] = flag;
+    __syncthreads();
+    flag = flags[0] | flags[1] | flags[2] | flags[3];
+    const int ek = block_exp(kmost), ev = block_exp(vmost);
+    const int64_t at = (int64_t)kh * X.n + tile;
+    if (threadIdx.x == 0) X.info[at] = make_int4(ek, ev, flag, 0);
+    int* exps = X.exps + at * 2 * kKT;
+    u16 *kd = X.data + at * 4 * PART, *vd = kd + 2 * PART;
+#pragma unroll
+    for (int u = 0; u < KU; ++u) {
+        const int key = w * 16 + u * KROWS + krow, e = flag & kKeyExps ? block_exp(ktop[u]) : ek;
+        if ((flag & kKeyExps) && kch == 0) exps[key] = e;
+        const float sc = pow2(-e);
+        h8 hi, lo;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            h2 a, c;
+            split_pair(kx[u][i] * sc, kx[u][i + 1] * sc, a, c);
+            hi[i] = a[0], hi[i + 1] = a[1];
+            lo[i] = c[0], lo[i + 1] = c[1];
+        }
+        const int row = row_of_key(key), to = row * DP + ((kch ^ swz_k<DP>(row)) << 3);
+        *(h8*)(kd + to) = hi;
+        *(h8*)(kd + PART + to) = lo;
+    }
+    float vs[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int e = flag & kValueExps ? block_exp(vtop[i]) : ev;
+        if ((flag & kValueExps) && lane == 0) exps[kKT + w * 16 + i] = e;
+        vs[i] = pow2(-e);
+    }
+#pragma unroll
+    for (int u = 0; u < VU; ++u)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            h8 hi, lo;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                h2 a, c;
+                split_pair(vx[b * 8 + i][u] * vs[b * 8 + i], vx[b * 8 + i + 1][u] * vs[b * 8 + i + 1], a, c);
+                hi[i] = a[0], hi[i + 1] = a[1];
+                lo[i] = c[0], lo[i + 1] = c[1];
+            }
+            const int row = lane * VU + u, to = row * kKT + (((w * 2 + b) ^ swz_v(row)) << 3);
+            *(h8*)(vd + to) = hi;
+            *(h8*)(vd + PART + to) = lo;
+        }
+}
+
+// table: the values of bias that the group's heads have, kept in LDS; 0 where they are read from memory.
+template <int DP, bool EXTRA, bool VEC>
+__global__ __launch_bounds__(kThreads, 2) void k_attn_packed_tiles(Packed P, Tiles X, int out16, int items, int table, Parts S) {
+    constexpr int DS = DP / 16, DT = DP / 32, PART = kKT * DP;
+    __shared__ __attribute__((aligned(1024))) u16 kbuf[2 * PART];  // rows of K, hi and lo
+    __shared__ __attribute__((aligned(1024))) u16 vbuf[2 * PART];  // rows of V^T
+    extern __shared__ float biases[];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int fr = lane & 31, fh = lane >> 5;
     const int group = P.heads / P.kv_heads;
@@ -239,15 +404,34 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_packed_tiles(Packed P, int
     const int shift = lk - T.rows;
     const int p = qi + shift;
     const Seen see = seen_from(P, p, lk, pre);
-    const Seen wg_first = seen_from(P, T.row0 / group + shift, lk, pre),
-               wg_last = seen_from(P, (min(T.row0 + kTileRows, rows) - 1) / group + shift, lk, pre);
-    const int wg_lo = wg_first.lo, wg_hi = wg_last.hi;
+    const int wg_lo = seen_from(P, T.row0 / group + shift, lk, pre).lo,
+              wg_hi = seen_from(P, (min(T.row0 + kTileRows, rows) - 1) / group + shift, lk, pre).hi;
     const bool active = T.row0 + w * 32 < rows;
-    const int first_lo = __builtin_amdgcn_readlane(see.lo, 0), last_hi = __builtin_amdgcn_readlane(see.hi, 31);
-    const int npre = (pre + kKT - 1) / kKT, next = max(npre, wg_lo / kKT);
-    const int all = npre + (wg_hi > wg_lo ? max(0, (wg_hi + kKT - 1) / kKT - next) : 0);
+    const int first_lo = __builtin_amdgcn_readlane(see.lo, 0), last_lo = __builtin_amdgcn_readlane(see.lo, 31);
+    const int first_hi = __builtin_amdgcn_readlane(see.hi, 0), last_hi = __builtin_amdgcn_readlane(see.hi, 31);
+    // The tensor's tiles with a key of the prefix, then those with a key of the intervals; this part's share of them.
+    const int t0 = T.z / kKT, npre = pre ? (T.z + pre + kKT - 1) / kKT - t0 : 0;
+    const int next = max(t0 + npre, (T.z + wg_lo) / kKT);
+    const int all = npre + (wg_hi > wg_lo ? max(0, (T.z + wg_hi + kKT - 1) / kKT - next) : 0);
     const int n0 = (int)((int64_t)all * blockIdx.y / S.n), nt = (int)((int64_t)all * (blockIdx.y + 1) / S.n);
-    auto key_of = [&](int n) { return (n < npre ? n : next + n - npre) * kKT; };
+    auto tile_of = [&](int n) { return n < npre ? t0 + n : next + n - npre; };
+    const u16* data = X.data + (int64_t)kh * X.n * 4 * PART;
+    const int4* info = X.info + (int64_t)kh * X.n;
+    auto copy = [&](int tile, int part, u16* to) __attribute__((always_inline)) {
+        // Buffer loads, not global_load_lds: the compiler counts a FLAT-encoded copy into LDS as
+        // pending on the LDS counter too, and then waits for every LDS read in full.
+        const __amdgpu_buffer_rsrc_t rsrc =
+            __builtin_amdgcn_make_buffer_rsrc((void*)(data + (int64_t)tile * 4 * PART + part * 2 * PART), (short)0, 4 * PART, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < 4 * PART / (kThreads * 16); ++i) {
+            const int chunk = (i * kWaves + w) * 64;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(to + chunk * 8), 16, lane * 16, chunk * 16, 0,
+                                                     0);
+        }
+    };
+    if (n0 < nt) copy(tile_of(n0), 0, kbuf);
+    if (EXTRA && table)  // [group, 2 radius + 1]
+        for (int i = threadIdx.x; i < table; i += kThreads) biases[i] = P.bias[(int64_t)kh * table + i];
 
     // Q: the B operand of S^T, row qi of head h, dims ds*16 + fh*8 .. +7
     const float* qp = P.q + (T.first + qi) * inner + (int64_t)h * d;
@@ -284,145 +468,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_packed_tiles(Packed P, int
                 ql[ds][e] = lo[0], ql[ds][e + 1] = lo[1];
             }
     }
-    const float scale = fabsf(P.scale);
-
-    // A tile on its way: this wave's eight keys. k: 16-byte chunks of their rows; v: the
-    // lane's columns of all eight.
-    constexpr int KCH = DP / 8;  // chunks of a row
-    const int kch = lane & (KCH - 1), krow = lane / KCH;
-    constexpr int KROWS = 64 / KCH;
-    float kx[KU][8], vx[8][KU];
-    const float* kbase = P.k + T.z * kv_inner + (int64_t)kh * d;
-    const float* vbase = P.v + T.z * kv_inner + (int64_t)kh * d;
-    // a tile that some of the workgroup's rows see in part
-    auto border = [&](int k0) { return !(k0 + kKT <= pre || (k0 >= wg_last.lo && k0 + kKT <= wg_first.hi)); };
-    auto wanted = [&](int j) { return j < lk && (j < pre || (j >= wg_lo && j < wg_hi)); };
-    auto fetch = [&](int n) __attribute__((always_inline)) {
-        const int j0 = key_of(n) + w * 8;
-#pragma unroll
-        for (int u = 0; u < KU; ++u) {
-            const float* a = kbase + (int64_t)min(j0 + u * KROWS + krow, lk - 1) * kv_inner;
-            if constexpr (VEC) {
-                a += min(kch * 8, d - 8);
-                const f4 x = *(const f4*)a, y = *(const f4*)(a + 4);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) kx[u][e] = e < 4 ? x[e & 3] : y[e & 3];
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) kx[u][e] = a[min(kch * 8 + e, d - 1)];
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float* a = vbase + (int64_t)min(j0 + i, lk - 1) * kv_inner;
-            if constexpr (VEC && KU == 2) {
-                const f2 x = *(const f2*)(a + min(lane * 2, d - 2));
-                vx[i][0] = x.x, vx[i][1] = x.y;
-            } else {
-#pragma unroll
-                for (int u = 0; u < KU; ++u) vx[i][u] = a[min(lane * KU + u, d - 1)];
-            }
-        }
-    };
-    // Into LDS: scaled, split, in the order of the fragments' reads.
-    auto store = [&](int n, int b) __attribute__((always_inline)) {
-        const int k0 = key_of(n), j0 = k0 + w * 8;
-        int ktop = 0, vtop = 0;
-#pragma unroll
-        for (int u = 0; u < KU; ++u) {
-            const bool ok = wanted(j0 + u * KROWS + krow);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if (!ok || kch * 8 + e >= d) kx[u][e] = 0.f;
-                ktop = max(ktop, abs_bits(kx[u][e]));
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const bool ok = wanted(j0 + i);
-#pragma unroll
-            for (int u = 0; u < KU; ++u) {
-                if (!ok || lane * KU + u >= d) vx[i][u] = 0.f;
-                vtop = max(vtop, abs_bits(vx[i][u]));
-            }
-        }
-        ktop = group_imax<64>(ktop);
-        vtop = group_imax<64>(vtop);
-        const bool bad = vtop >= kInfBits;
-        if (bad) {
-            vtop = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int u = 0; u < KU; ++u) {
-                    if (abs_bits(vx[i][u]) >= kInfBits) vx[i][u] = 0.f;
-                    vtop = max(vtop, abs_bits(vx[i][u]));
-                }
-            vtop = group_imax<64>(vtop);
-        }
-        const int ek = block_exp(ktop), ev = block_exp(vtop);
-        if (lane == 0) {
-            exps[b][0][w] = ek;
-            exps[b][1][w] = ev;
-            bads[b][w] = bad;
-        }
-        float ks[KU], vs[8];
-#pragma unroll
-        for (int u = 0; u < KU; ++u) ks[u] = pow2(-ek);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) vs[i] = pow2(-ev);
-        if (border(k0)) {
-#pragma unroll
-            for (int u = 0; u < KU; ++u) {
-                int top = 0;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top = max(top, abs_bits(kx[u][e]));
-                const int e = block_exp(group_imax<KCH>(top));
-                ks[u] = pow2(-e);
-                if (kch == 0) key_exps[b][0][w * 8 + u * KROWS + krow] = e;
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                int top = 0;
-#pragma unroll
-                for (int u = 0; u < KU; ++u) top = max(top, abs_bits(vx[i][u]));
-                const int e = block_exp(group_imax<64>(top));
-                vs[i] = pow2(-e);
-                if (lane == 0) key_exps[b][1][w * 8 + i] = e;
-            }
-        }
-        u16 *kd = buf[b], *vd = buf[b] + 2 * PART;
-#pragma unroll
-        for (int u = 0; u < KU; ++u) {
-            const int row = row_of_key(w * 8 + u * KROWS + krow);
-            h8 hi, lo;
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                h2 a, c;
-                split_pair(kx[u][e] * ks[u], kx[u][e + 1] * ks[u], a, c);
-                hi[e] = a[0], hi[e + 1] = a[1];
-                lo[e] = c[0], lo[e + 1] = c[1];
-            }
-            const int at = row * DP + ((kch ^ swz_k<DP>(row)) << 3);
-            *(h8*)(kd + at) = hi;
-            *(h8*)(kd + PART + at) = lo;
-        }
-#pragma unroll
-        for (int u = 0; u < KU; ++u) {
-            const int row = lane * KU + u;
-            h8 hi, lo;
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                h2 a, c;
-                split_pair(vx[i][u] * vs[i], vx[i + 1][u] * vs[i + 1], a, c);
-                hi[i] = a[0], hi[i + 1] = a[1];
-                lo[i] = c[0], lo[i + 1] = c[1];
-            }
-            const int at = row * kKT + ((w ^ swz_v(row)) << 3);
-            *(h8*)(vd + at) = hi;
-            *(h8*)(vd + PART + at) = lo;
-        }
-    };
+    const float scale = EXTRA ? fabsf(P.scale) : fabsf(P.scale) * kLog2e;
 
     f32x16 o[DT], s[2];
 #pragma unroll
@@ -432,88 +478,105 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_packed_tiles(Packed P, int
     float m = -INFINITY, sum = 0.f;  // the reference (log2 units without EXTRA), this lane's keys' sum of weights
     int E = kUnsetE;
 
-    auto scores = [&](const u16* kd) __attribute__((always_inline)) {
+    auto scores = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[j][i] = 0.f;
-#pragma unroll
-        for (int ds = 0; ds < DS; ++ds) {
-            h8 kf[2][2];
+        h8 kf[2][2][2];  // [step % 2][half][hi, lo]: a step's fragments are read ahead of the MFMAs before it
+        auto fetch = [&](int ds) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int row = j * 32 + fr, at = row * DP + (((ds * 2 + fh) ^ swz_k<DP>(row)) << 3);
-                kf[j][0] = *(const h8*)(kd + at);
-                kf[j][1] = *(const h8*)(kd + PART + at);
+                kf[ds & 1][j][0] = *(const h8*)(kbuf + at);
+                kf[ds & 1][j][1] = *(const h8*)(kbuf + PART + at);
             }
+        };
+        fetch(0);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[j][0], qh[ds], s[j], 0, 0, 0);
+        for (int ds = 0; ds < DS; ++ds) {
+            if (ds + 1 < DS) fetch(ds + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            const int b = ds & 1;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[j][0], ql[ds], s[j], 0, 0, 0);
+            for (int j = 0; j < 2; ++j) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[b][j][0], qh[ds], s[j], 0, 0, 0);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[j][1], qh[ds], s[j], 0, 0, 0);
+            for (int j = 0; j < 2; ++j) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[b][j][0], ql[ds], s[j], 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[b][j][1], qh[ds], s[j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // Score register i of half j is key k0 + j*32 + (i/8)*16 + fh*8 + i%8.
-    auto key_at = [&](int j, int i) { return j * 32 + (i >> 3) * 16 + fh * 8 + (i & 7); };
-    auto visible = [&](int j) { return (j < pre) | ((j >= see.lo) & (j < see.hi)); };
-
-    // s -> weights in place, the statistics and the scale of o brought up to date
-    auto softmax = [&](int k0, int b) __attribute__((always_inline)) {
-        const bool edge = border(k0);
-        int ek[4], ev[4], emax = kUnsetE;
-        if (edge) {
+    auto visible = [&](int j) { return ((unsigned)j < (unsigned)pre) | ((j >= see.lo) & (j < see.hi)); };
+    // Score register i of half j is the tile's key j*32 + (i/8)*16 + fh*8 + i%8.
+    // s -> weights in place, the statistics and the scale of o brought up to date. k0: the
+    // sequence's key at the tile's first row (below zero in front of the sequence).
+    auto softmax = [&](int k0, int tile) __attribute__((always_inline)) {
+        const int4 about = info[tile];
+        const int flag = about.z;
+        const int* exps = X.exps + ((int64_t)kh * X.n + tile) * 2 * kKT;
+        const bool edge = !((k0 >= 0 && k0 + kKT <= pre) || (k0 >= last_lo && k0 + kKT <= first_hi));  // of this wave
+        int emax = about.y;
+        if (edge && !((k0 < pre && k0 + kKT > 0) || (k0 < see.hi && k0 + kKT > see.lo))) emax = kUnsetE;
+        // kept normal: -inf stays -inf, zero zero
+        const float ct = fminf(fmaxf(ldexpf(scale, eq + (flag & kKeyExps ? 0 : about.x)), 1.17549435e-38f), 3.40282347e38f);
+        if (flag & kKeyExps) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                ek[u] = ev[u] = 0;
+            for (int u = 0; u < 4; ++u)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int j = u * 16 + fh * 8 + i;
-                    const bool ok = visible(k0 + j);
-                    s[u >> 1][(u & 1) * 8 + i] = ldexpf(s[u >> 1][(u & 1) * 8 + i], key_exps[b][0][j]);
-                    if (ok) emax = max(emax, key_exps[b][1][j]);
-                }
-            }
+                for (int i = 0; i < 8; ++i) s[u >> 1][(u & 1) * 8 + i] = ldexpf(s[u >> 1][(u & 1) * 8 + i], exps[u * 16 + fh * 8 + i]);
+        }
+        if (flag & kValueExps) {
+            emax = kUnsetE;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (visible(k0 + u * 16 + fh * 8 + i)) emax = max(emax, exps[kKT + u * 16 + fh * 8 + i]);
             emax = max(emax, __shfl_xor(emax, 32, 64));
-        } else {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                ek[u] = exps[b][0][u * 2 + fh];
-                ev[u] = exps[b][1][u * 2 + fh];
-                emax = max(emax, max(exps[b][1][u * 2], exps[b][1][u * 2 + 1]));
-            }
         }
-        float ct[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u)  // kept normal: -inf stays -inf, zero zero
-            ct[u] = fminf(fmaxf(ldexpf(EXTRA ? scale : scale * kLog2e, eq + ek[u]), 1.17549435e-38f), 3.40282347e38f);
         if constexpr (EXTRA) {
-            const float* bp = P.bias + (int64_t)h * (2 * P.radius + 1) + P.radius;
+            const int mid = (h - kh * group) * (2 * P.radius + 1) + P.radius;
+            const float* bp = P.bias + (int64_t)kh * group * (2 * P.radius + 1);
+            if (P.cap > 0.f) {
+                const float in = ct / P.cap;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float x = s[j][i] * ct[j * 2 + (i >> 3)];
-                    if (P.cap > 0.f) x = P.cap * tanh_near(x / P.cap);
-                    if (P.bias) x += bp[min(max(k0 + key_at(j, i) - p, -P.radius), P.radius)];
-                    s[j][i] = x;
-                }
+                    for (int i = 0; i < 16; ++i) s[j][i] = P.cap * tanh_near(s[j][i] * in);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[j][i] *= ct;
+            }
+            if (table) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        s[u >> 1][(u & 1) * 8 + i] += biases[mid + min(max(k0 + u * 16 + fh * 8 + i - p, -P.radius), P.radius)];
+            } else if (P.bias) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        s[u >> 1][(u & 1) * 8 + i] += bp[mid + min(max(k0 + u * 16 + fh * 8 + i - p, -P.radius), P.radius)];
+            }
         }
         if (edge) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int u = 0; u < 4; ++u)
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (!visible(k0 + key_at(j, i))) s[j][i] = -INFINITY;
+                for (int i = 0; i < 8; ++i)
+                    if (!visible(k0 + u * 16 + fh * 8 + i)) s[u >> 1][(u & 1) * 8 + i] = -INFINITY;
         }
-        float mt = -INFINITY;
+        float mt = s[0][0];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            float mx = s[u >> 1][(u & 1) * 8];
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[u >> 1][(u & 1) * 8 + i]);
-            mt = fmaxf(mt, EXTRA ? mx : mx * ct[u]);
-        }
+            for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[j][i]);
+        if constexpr (!EXTRA) mt *= ct;
         mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
         const float mnew = mt > m + (EXTRA ? kLazy / kLog2e : kLazy) ? mt : m;
         float alpha = 1.0f;
@@ -526,29 +589,25 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_packed_tiles(Packed P, int
             ao = E == kUnsetE ? 0.f : ldexpf(alpha, max(E - up, -300));
             E = up;
         }
+        const int by = 14 + (flag & kValueExps ? 0 : max(about.y - E, kFarE));
+        const float up = (float)by - (EXTRA ? 0.f : ref);
         float total = 0.f;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int by = 14 + (edge ? 0 : max(ev[u] - E, kFarE));
-            float part = 0.f;
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float x = s[u >> 1][(u & 1) * 8 + i];
-                if constexpr (EXTRA) x = __builtin_amdgcn_exp2f(fmaf(x - ref, kLog2e, (float)by));
-                else x = __builtin_amdgcn_exp2f(fmaf(x, ct[u], (float)by - ref));
-                s[u >> 1][(u & 1) * 8 + i] = x;
-                part += x;
+            for (int i = 0; i < 16; ++i) {
+                const float x = __builtin_amdgcn_exp2f(EXTRA ? fmaf(s[j][i] - ref, kLog2e, up) : fmaf(s[j][i], ct, up));
+                s[j][i] = x;
+                total += x;
             }
-            total += ldexpf(part, -by);
-        }
-        sum = fmaf(sum, alpha, total);
-        if (edge) {
+        sum = fmaf(sum, alpha, ldexpf(total, -by));
+        if (flag & kValueExps) {
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
                 for (int i = 0; i < 8; ++i)  // an unseen key's weight is zero, its exponent may be above E
-                    s[u >> 1][(u & 1) * 8 + i] = ldexpf(s[u >> 1][(u & 1) * 8 + i],
-                                                        min(max(key_exps[b][1][u * 16 + fh * 8 + i] - E, kFarE), 0));
+                    s[u >> 1][(u & 1) * 8 + i] =
+                        ldexpf(s[u >> 1][(u & 1) * 8 + i], min(max(exps[kKT + u * 16 + fh * 8 + i] - E, kFarE), 0));
         }
         if (__ballot(ao != 1.0f)) {
 #pragma unroll
@@ -556,8 +615,16 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_packed_tiles(Packed P, int
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[dt][i] *= ao;
         }
+        return flag & kNotFinite;
     };
-    auto values = [&](const u16* vd) __attribute__((always_inline)) {
+    auto values = [&]() __attribute__((always_inline)) {
+        h8 vf[2][2];  // [step % 2][hi, lo], steps (16 keys, 32 columns), columns fastest
+        auto fetch = [&](int i) __attribute__((always_inline)) {
+            const int row = i % DT * 32 + fr, at = row * kKT + (((i / DT * 2 + fh) ^ swz_v(row)) << 3);
+            vf[i & 1][0] = *(const h8*)(vbuf + at);
+            vf[i & 1][1] = *(const h8*)(vbuf + PART + at);
+        };
+        fetch(0);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
             h8 ph, pl;
@@ -570,49 +637,45 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_packed_tiles(Packed P, int
             }
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                const int row = dt * 32 + fr, at = row * kKT + (((ks * 2 + fh) ^ swz_v(row)) << 3);
-                const h8 vh = *(const h8*)(vd + at), vl = *(const h8*)(vd + PART + at);
-                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph, o[dt], 0, 0, 0);
-                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl, o[dt], 0, 0, 0);
-                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph, o[dt], 0, 0, 0);
+                const int i = ks * DT + dt, b = i & 1;
+                if (i + 1 < 4 * DT) fetch(i + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[b][0], ph, o[dt], 0, 0, 0);
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[b][0], pl, o[dt], 0, 0, 0);
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[b][1], ph, o[dt], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     };
+    // The copies have landed, the LDS reads are done, for every wave.
+    auto meet = [&]() __attribute__((always_inline)) { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
     int bad_first = nt, bad_last = -1;  // the tiles that hold values that are not finite
-    if (n0 < nt) {
-        fetch(n0);
-        store(n0, n0 & 1);
-    }
     for (int n = n0; n < nt; ++n) {
-        const int b = n & 1, k0 = key_of(n);
-        if (n + 1 < nt) fetch(n + 1);
-        // tile n is in LDS, and nobody reads tile n - 1 any more
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (active && (k0 < pre || (k0 < last_hi && k0 + kKT > first_lo))) {
-            scores(buf[b]);
-            softmax(k0, b);
-            values(buf[b] + 2 * PART);
+        const int tile = tile_of(n), k0 = tile * kKT - T.z;
+        const bool mine = active && ((k0 < pre && k0 + kKT > 0) || (k0 < last_hi && k0 + kKT > first_lo));
+        meet();  // K of this tile is there, V of the last one no longer read
+        copy(tile, 1, vbuf);
+        if (mine) scores();
+        meet();
+        if (n + 1 < nt) copy(tile_of(n + 1), 0, kbuf);
+        if (mine) {
+            if (softmax(k0, tile)) {
+                bad_first = min(bad_first, n);
+                bad_last = n;
+            }
+            values();
         }
-        int any = 0;
-#pragma unroll
-        for (int g = 0; g < 8; ++g) any |= bads[b][g];
-        if (__builtin_amdgcn_readfirstlane(any)) {
-            bad_first = min(bad_first, n);
-            bad_last = n;
-        }
-        if (n + 1 < nt) store(n + 1, b ^ 1);
     }
 
     if (r >= rows) return;
     sum += __shfl_xor(sum, 32, 64);
-    const int64_t cell = ((int64_t)(T.first + qi) * P.heads + h) * S.n + blockIdx.y;
     // a part of the keys: the sums as they are, on the scale of the reference
     const float inv = sum == 0.f ? 0.f : ldexpf(S.n > 1 ? 1.0f : 1.0f / sum, E - 14);
     for (int n = bad_first; n <= bad_last; ++n)
-        for (int j = key_of(n), end = min(j + kKT, lk); j < end; ++j) {
+        for (int j = max(tile_of(n) * kKT - T.z, 0), end = min(tile_of(n) * kKT - T.z + kKT, lk); j < end; ++j) {
             if (!visible(j)) continue;
-            const float* vp = vbase + j * kv_inner;
+            const float* vp = P.v + (T.z + j) * kv_inner + (int64_t)kh * d;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -621,34 +684,25 @@ __global__ __launch_bounds__(kThreads, 1) void k_attn_packed_tiles(Packed P, int
                     if (abs_bits(x) >= kInfBits) o[dt][i] += x;
                 }
         }
-    if (S.n > 1) {
-        if (fh == 0) S.ml[cell] = f2{m, sum};
-        float* to = S.o + cell * S.stride;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int c = dt * 32 + g * 8 + fh * 4;
-                if (c < d) *(f4*)(to + c) = f4{o[dt][g * 4] * inv, o[dt][g * 4 + 1] * inv, o[dt][g * 4 + 2] * inv, o[dt][g * 4 + 3] * inv};
-            }
-        return;
-    }
-    const int64_t at = (T.first + qi) * inner + (int64_t)h * d;
+    const int64_t row = (int64_t)(T.first + qi) * P.heads + h, cell = row * S.n + blockIdx.y, at = row * d;
+    if (S.n > 1 && fh == 0) S.ml[cell] = f2{m, sum};
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int c = dt * 32 + g * 8 + fh * 4;
+            if (c >= d) continue;
             const f4 v = {o[dt][g * 4] * inv, o[dt][g * 4 + 1] * inv, o[dt][g * 4 + 2] * inv, o[dt][g * 4 + 3] * inv};
-            if constexpr (VEC) {
-                if (c >= d) continue;
-                if constexpr (OUT16) *(uint2*)((u16*)P.out + at + c) = dev::bf16x4(v);
+            if (S.n > 1) {
+                *(f4*)(S.o + cell * S.stride + c) = v;
+            } else if constexpr (VEC) {
+                if (out16) *(uint2*)((u16*)P.out + at + c) = dev::bf16x4(v);
                 else *(f4*)((float*)P.out + at + c) = v;
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (c + e < d) {
-                        if constexpr (OUT16) ((u16*)P.out)[at + c + e] = dev::bf16_rne(v[e]);
+                        if (out16) ((u16*)P.out)[at + c + e] = dev::bf16_rne(v[e]);
                         else ((float*)P.out)[at + c + e] = v[e];
                     }
             }
@@ -855,14 +909,20 @@ __global__ __launch_bounds__(256) void k_attn_packed_join(Packed P, int out16, P
         }
 }
 
-// The parts' memory, in scratch; the keys uncut where it cannot be had.
-Parts make_parts(const Packed& P, int64_t n) {
+// The parts' memory; where it cannot be had the keys stay uncut. `behind`: bytes that the
+// caller needs in front of it, whose address is put into `front` (null with nothing to be had).
+Parts make_parts(const Packed& P, int64_t n, size_t behind, char*& front) {
     Parts S{(int)n, (P.d + 3) / 4 * 4, nullptr, nullptr};
     const size_t cells = (size_t)P.Tq * P.heads * n, ob = (cells * S.stride * 4 + 255) / 256 * 256;
-    char* base = n > 1 ? (char*)try_scratch(ob + cells * sizeof(f2)) : nullptr;
-    if (!base) S.n = 1;
-    S.o = (float*)base;
-    S.ml = base ? (f2*)(base + ob) : nullptr;
+    behind = (behind + 255) / 256 * 256;
+    front = n > 1 ? (char*)try_scratch(behind + ob + cells * sizeof(f2)) : nullptr;
+    if (front) {
+        S.o = (float*)(front + behind);
+        S.ml = (f2*)(front + behind + ob);
+    } else {
+        S.n = 1;
+        if (behind) front = (char*)try_scratch(behind);
+    }
     return S;
 }
 
@@ -876,7 +936,8 @@ void run_few(const Packed& P, bool out16, int64_t items, int rows) {
     const bool extra = P.cap > 0.f || P.bias;
     // Parts of the keys until there are eight workgroups a CU, each wave with two chunks of an average sequence.
     const int64_t wgs = items * P.kv_heads, keys = P.Tk / std::max(1, P.seqs);
-    const Parts S = make_parts(P, std::max<int64_t>(1, std::min<int64_t>({8 * num_cus() / wgs, keys / (kFewWaves * 64), 256})));
+    char* none;
+    const Parts S = make_parts(P, std::max<int64_t>(1, std::min<int64_t>({8 * num_cus() / wgs, keys / (kFewWaves * 64), 256})), 0, none);
     auto go = [&](auto r, auto ex) {
         k_attn_packed_few<DP, decltype(r)::value, decltype(ex)::value>
             <<<dim3((unsigned)wgs, (unsigned)S.n), 64 * kFewWaves, 0, stream()>>>(P, out16, S);
@@ -892,26 +953,36 @@ void run_few(const Packed& P, bool out16, int64_t items, int rows) {
     join_parts(P, out16, S, !extra);
 }
 
+// False where the tiles' scratch cannot be had.
 template <int DP>
-void run_tiles(const Packed& P, bool out16, int64_t items) {
-    const bool vec = P.d % 8 == 0 && aligned16(P.q) && aligned16(P.k) && aligned16(P.v) && (out16 ? ((uintptr_t)P.out & 7) == 0 : aligned16(P.out));
+bool run_tiles(const Packed& P, bool out16, int64_t items) {
+    const bool kvec = P.d % 8 == 0 && aligned16(P.k) && aligned16(P.v),
+               qvec = P.d % 8 == 0 && aligned16(P.q) && (out16 ? ((uintptr_t)P.out & 7) == 0 : aligned16(P.out));
+    // Parts of the keys while the workgroups do not fill the chip, of eight tiles of an average sequence at least.
+    const int64_t wgs = items * P.kv_heads, keys = P.Tk / std::max(1, P.seqs), ntiles = (P.Tk + kKT - 1) / kKT;
+    const size_t cells = (size_t)ntiles * P.kv_heads, tb = cells * 4 * kKT * DP * 2;
+    char* front;
+    const Parts S = make_parts(P, std::max<int64_t>(1, std::min<int64_t>(2 * num_cus() / wgs, keys / (8 * kKT))),
+                               tb + cells * (sizeof(int4) + 2 * kKT * sizeof(int)), front);
+    if (!front) return false;
+    const Tiles X{(u16*)front, (int4*)(front + tb), (int*)(front + tb + cells * sizeof(int4)), (int)ntiles};
+    const dim3 sg((unsigned)ntiles, (unsigned)P.kv_heads);
+    if (kvec) k_attn_packed_split<DP, true><<<sg, 64 * kWaves, 0, stream()>>>(P, X);
+    else k_attn_packed_split<DP, false><<<sg, 64 * kWaves, 0, stream()>>>(P, X);
+    // What two workgroups of a CU leave of its LDS takes the bias of a group's heads, if it fits.
+    const int64_t values = P.bias ? (int64_t)(P.heads / P.kv_heads) * (2 * P.radius + 1) : 0;
+    const int table = values * 4 <= 14 * 1024 ? (int)values : 0;
     const bool extra = P.cap > 0.f || P.bias;
     using T_ = std::true_type;
     using F_ = std::false_type;
-    // Parts of the keys while the workgroups do not fill the chip, of eight tiles of an average sequence at least.
-    const int64_t wgs = items * P.kv_heads, keys = P.Tk / std::max(1, P.seqs);
-    const Parts S = make_parts(P, std::max<int64_t>(1, std::min<int64_t>(num_cus() / wgs, keys / (8 * kKT))));
-    auto go = [&](auto o16, auto ex, auto ve) {
-        k_attn_packed_tiles<DP, decltype(o16)::value, decltype(ex)::value, decltype(ve)::value>
-            <<<dim3((unsigned)wgs, (unsigned)S.n), kThreads, 0, stream()>>>(P, (int)items, S);
+    auto go = [&](auto ex, auto ve) {
+        k_attn_packed_tiles<DP, decltype(ex)::value, decltype(ve)::value>
+            <<<dim3((unsigned)wgs, (unsigned)S.n), kThreads, (unsigned)table * 4, stream()>>>(P, X, out16, (int)items, table, S);
     };
-    auto with = [&](auto o16) {
-        if (extra) vec ? go(o16, T_(), T_()) : go(o16, T_(), F_());
-        else vec ? go(o16, F_(), T_()) : go(o16, F_(), F_());
-    };
-    if (out16) with(T_());
-    else with(F_());
+    if (extra) qvec ? go(T_(), T_()) : go(T_(), F_());
+    else qvec ? go(F_(), T_()) : go(F_(), F_());
     join_parts(P, out16, S, !extra);
+    return true;
 }
 
 void run_attention_packed(const float* q, const float* k, const float* v, void* out, bool out16, int64_t Tq, int64_t Tk, int heads,
@@ -960,11 +1031,11 @@ void run_attention_packed(const float* q, const float* k, const float* v, void* 
         }
     }
     const int64_t rows = Tq * group, items = rows / kTileRows + live;
-    if (d <= 128 && rows < kMost && items * kv_heads * kThreads <= kMaxGridItems) {
-        if (d <= 64) run_tiles<64>(P, out16, items);
-        else run_tiles<128>(P, out16, items);
-        launched(op);
-        return;
+    if (d <= 128 && rows < kMost && items * kv_heads * kThreads <= kMaxGridItems && (Tk + kKT) * 4 <= kMaxGridItems) {
+        if (d <= 64 ? run_tiles<64>(P, out16, items) : run_tiles<128>(P, out16, items)) {
+            launched(op);
+            return;
+        }
     }
     const int64_t gx = (Tq + kRowWaves - 1) / kRowWaves;
     need(gx * 64 * kRowWaves <= kMaxGridItems, op, "too many queries for one launch");
