@@ -51,14 +51,19 @@ __device__ __forceinline__ Seen seen_from(const Packed& P, int p, int lk, int pr
 }
 
 // tanh to about 3e-7 of itself. Near zero 1 - e would cancel: a polynomial (its next
-// term is below 2e-8 of the sum at 0.35).
-__device__ __forceinline__ float tanh_near(float x) {
-    const float a = fabsf(x), x2 = x * x;
-    const float e = __builtin_amdgcn_exp2f(-2.0f * kLog2e * a);
-    const float far = copysignf((1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), x);
+// term is below 2e-8 of the sum at kTanhNear).
+constexpr float kTanhNear = 0.35f;
+__device__ __forceinline__ float tanh_small(float x) {
+    const float x2 = x * x;
     const float p = fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, -1382.0f / 155925.0f, 62.0f / 2835.0f), -17.0f / 315.0f), 2.0f / 15.0f),
                          -1.0f / 3.0f);
-    return a < 0.35f ? fmaf(x * x2, p, x) : far;
+    return fmaf(x * x2, p, x);
+}
+__device__ __forceinline__ float tanh_near(float x) {
+    const float a = fabsf(x);
+    const float e = __builtin_amdgcn_exp2f(-2.0f * kLog2e * a);
+    const float far = copysignf((1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), x);
+    return a < kTanhNear ? tanh_small(x) : far;
 }
 
 // ---------------------------------------------------------------------------
@@ -144,11 +149,10 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_attn_packed_rows(Packed P) {
 // k_attn_packed_split cuts k and v of a key/value head into tiles of 64 rows (of the
 // tensor: a tile may hold rows of several sequences) in library scratch, as fp16 pairs in
 // the order of the fragments' reads; a tile that no sequence reads is left out.
-// k_attn_packed_tiles takes kTileRows rows of one sequence and key/value head a workgroup,
+// k_attn_packed_tiles takes 32 rows a wave of one sequence and key/value head a workgroup,
 // a row being a (query, head of the group) pair, heads fastest: the heads that share a
 // key/value head share its tiles. It copies the tiles that any of its rows sees to LDS, and
-// each of its four waves takes 32 rows against them. Two workgroups fit a CU: while the
-// waves of one are at their MFMAs those of the other take exponentials.
+// each of its waves takes 32 rows against them.
 //
 // Operands are fp16 pairs hi + lo in block floating point, products hi hi + hi lo +
 // lo hi with fp32 sums (2^-21 of each product). A block is a row of q, or a tile of k or
@@ -178,7 +182,7 @@ struct Parts {
     f2* ml;         // [Tq, heads, n]
 };
 
-constexpr int kKT = 64, kWaves = 4, kThreads = 64 * kWaves, kTileRows = 32 * kWaves;
+constexpr int kKT = 64, kSplitWaves = 4;
 // The reference m of the weights is raised when a tile's largest score passes it by more
 // than this (in units of log2): weights stay below 2^(14 + kLazy), inside fp16.
 constexpr float kLazy = 1.5f;
@@ -243,10 +247,10 @@ struct Tiles {
 };
 
 template <int DP, bool VEC>
-__global__ __launch_bounds__(64 * kWaves) void k_attn_packed_split(Packed P, Tiles X) {
+__global__ __launch_bounds__(64 * kSplitWaves) void k_attn_packed_split(Packed P, Tiles X) {
     constexpr int PART = kKT * DP, KCH = DP / 8, KROWS = 64 / KCH, KU = 16 / KROWS;  // 16-byte chunks of a K row, rows of a wave's load, loads
     constexpr int VU = DP / 64;                                                     // columns of v a lane has
-    __shared__ int tops[2][kWaves], flags[kWaves];
+    __shared__ int tops[2][kSplitWaves], flags[kSplitWaves];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tile = blockIdx.x, kh = blockIdx.y, j0 = tile * kKT + w * 16, d = P.d;
     const int64_t kv_inner = (int64_t)P.kv_heads * d;
@@ -379,12 +383,20 @@ __global__ __launch_bounds__(64 * kWaves) void k_attn_packed_split(Packed P, Til
         }
 }
 
+// Eight waves a workgroup, one workgroup a CU; for DP = 64, whose tiles are half the size and
+// whose sequences are mostly shorter, four and two.
+template <int DP>
+constexpr int kWaves = DP == 128 ? 8 : 4;
+
 // table: the values of bias that the group's heads have, kept in LDS; 0 where they are read from memory.
 template <int DP, bool EXTRA, bool VEC>
-__global__ __launch_bounds__(kThreads, 2) void k_attn_packed_tiles(Packed P, Tiles X, int out16, int items, int table, Parts S) {
+__global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_packed_tiles(Packed P, Tiles X, int out16, int items, int table,
+                                                                                          Parts S) {
+    constexpr int WAVES = kWaves<DP>, kThreads = 64 * WAVES, kTileRows = 32 * WAVES;
     constexpr int DS = DP / 16, DT = DP / 32, PART = kKT * DP;
-    __shared__ __attribute__((aligned(1024))) u16 kbuf[2 * PART];  // rows of K, hi and lo
-    __shared__ __attribute__((aligned(1024))) u16 vbuf[2 * PART];  // rows of V^T
+    // Rows of K, hi and lo, of two tiles, and of V^T. Objects of their own, so that the compiler
+    // knows which copy a read has to wait for.
+    __shared__ __attribute__((aligned(1024))) u16 kbuf0[2 * PART], kbuf1[2 * PART], vbuf0[2 * PART], vbuf1[2 * PART];
     extern __shared__ float biases[];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int fr = lane & 31, fh = lane >> 5;
@@ -408,6 +420,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn_packed_tiles(Packed P, Til
               wg_hi = seen_from(P, (min(T.row0 + kTileRows, rows) - 1) / group + shift, lk, pre).hi;
     const bool active = T.row0 + w * 32 < rows;
     const int first_lo = __builtin_amdgcn_readlane(see.lo, 0), last_lo = __builtin_amdgcn_readlane(see.lo, 31);
+    const int first_p = __builtin_amdgcn_readlane(p, 0), last_p = __builtin_amdgcn_readlane(p, 31);
     const int first_hi = __builtin_amdgcn_readlane(see.hi, 0), last_hi = __builtin_amdgcn_readlane(see.hi, 31);
     // The tensor's tiles with a key of the prefix, then those with a key of the intervals; this part's share of them.
     const int t0 = T.z / kKT, npre = pre ? (T.z + pre + kKT - 1) / kKT - t0 : 0;
@@ -424,12 +437,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn_packed_tiles(Packed P, Til
             __builtin_amdgcn_make_buffer_rsrc((void*)(data + (int64_t)tile * 4 * PART + part * 2 * PART), (short)0, 4 * PART, 0x00020000);
 #pragma unroll
         for (int i = 0; i < 4 * PART / (kThreads * 16); ++i) {
-            const int chunk = (i * kWaves + w) * 64;
+            const int chunk = (i * WAVES + w) * 64;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(to + chunk * 8), 16, lane * 16, chunk * 16, 0,
                                                      0);
         }
     };
-    if (n0 < nt) copy(tile_of(n0), 0, kbuf);
+    if (n0 < nt) copy(tile_of(n0), 0, kbuf0);
     if (EXTRA && table)  // [group, 2 radius + 1]
         for (int i = threadIdx.x; i < table; i += kThreads) biases[i] = P.bias[(int64_t)kh * table + i];
 
@@ -470,7 +483,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn_packed_tiles(Packed P, Til
     }
     const float scale = EXTRA ? fabsf(P.scale) : fabsf(P.scale) * kLog2e;
 
-    f32x16 o[DT], s[2];
+    f32x16 o[DT];     // O^T
+    float x[32];      // S^T of the newest tile: x[i] of the lane is the tile's key (i/8)*16 + fh*8 + i%8
+    h8 ph[4], pl[4];  // its weights
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -478,16 +493,19 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn_packed_tiles(Packed P, Til
     float m = -INFINITY, sum = 0.f;  // the reference (log2 units without EXTRA), this lane's keys' sum of weights
     int E = kUnsetE;
 
-    auto scores = [&]() __attribute__((always_inline)) {
+    auto scores = [&](const u16* kbuf) __attribute__((always_inline)) {
+        f32x16 s[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[j][i] = 0.f;
+        int row0 = fr;
+        asm volatile("" : "+v"(row0));  // the addresses are formed here, not kept in registers through the loop
         h8 kf[2][2][2];  // [step % 2][half][hi, lo]: a step's fragments are read ahead of the MFMAs before it
         auto fetch = [&](int ds) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int row = j * 32 + fr, at = row * DP + (((ds * 2 + fh) ^ swz_k<DP>(row)) << 3);
+                const int row = j * 32 + row0, at = row * DP + (((ds * 2 + fh) ^ swz_k<DP>(row)) << 3);
                 kf[ds & 1][j][0] = *(const h8*)(kbuf + at);
                 kf[ds & 1][j][1] = *(const h8*)(kbuf + PART + at);
             }
@@ -506,25 +524,28 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn_packed_tiles(Packed P, Til
             for (int j = 0; j < 2; ++j) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[b][j][1], qh[ds], s[j], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[i] = s[i >> 4][i & 15];
     };
-    auto visible = [&](int j) { return ((unsigned)j < (unsigned)pre) | ((j >= see.lo) & (j < see.hi)); };
-    // Score register i of half j is the tile's key j*32 + (i/8)*16 + fh*8 + i%8.
+    auto visible = [&](int j) { return ((unsigned)j < (unsigned)pre) | ((unsigned)(j - see.lo) < (unsigned)(see.hi - see.lo)); };
+    // Keeps the compiler from working on all 32 scores at once, for which there are no registers.
+    auto few = [](int i) __attribute__((always_inline)) {
+        if (i % 8 == 7) __builtin_amdgcn_sched_barrier(0);
+    };
     // s -> weights in place, the statistics and the scale of o brought up to date. k0: the
     // sequence's key at the tile's first row (below zero in front of the sequence).
-    auto softmax = [&](int k0, int tile) __attribute__((always_inline)) {
-        const int4 about = info[tile];
-        const int flag = about.z;
+    auto softmax = [&](int k0, int tile, int tile_ek, int tile_ev, int flag) __attribute__((always_inline)) {
         const int* exps = X.exps + ((int64_t)kh * X.n + tile) * 2 * kKT;
         const bool edge = !((k0 >= 0 && k0 + kKT <= pre) || (k0 >= last_lo && k0 + kKT <= first_hi));  // of this wave
-        int emax = about.y;
+        int emax = tile_ev;
         if (edge && !((k0 < pre && k0 + kKT > 0) || (k0 < see.hi && k0 + kKT > see.lo))) emax = kUnsetE;
         // kept normal: -inf stays -inf, zero zero
-        const float ct = fminf(fmaxf(ldexpf(scale, eq + (flag & kKeyExps ? 0 : about.x)), 1.17549435e-38f), 3.40282347e38f);
+        const float ct = fminf(fmaxf(ldexpf(scale, eq + (flag & kKeyExps ? 0 : tile_ek)), 1.17549435e-38f), 3.40282347e38f);
         if (flag & kKeyExps) {
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) s[u >> 1][(u & 1) * 8 + i] = ldexpf(s[u >> 1][(u & 1) * 8 + i], exps[u * 16 + fh * 8 + i]);
+                for (int i = 0; i < 8; ++i) x[u * 8 + i] = ldexpf(x[u * 8 + i], exps[u * 16 + fh * 8 + i]);
         }
         if (flag & kValueExps) {
             emax = kUnsetE;
@@ -537,45 +558,83 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn_packed_tiles(Packed P, Til
         }
         if constexpr (EXTRA) {
             const int mid = (h - kh * group) * (2 * P.radius + 1) + P.radius;
-            const float* bp = P.bias + (int64_t)kh * group * (2 * P.radius + 1);
+            const float in = P.cap > 0.f ? ct / P.cap : ct;
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                    x[i] *= in;
+                    top = fmaxf(top, fabsf(x[i]));
+                }
             if (P.cap > 0.f) {
-                const float in = ct / P.cap;
+                // Scores well inside the cap, as most are, take the polynomial alone (half the
+                // instructions, no exponential).
+                const bool small = !__ballot(!(top < kTanhNear));
+                if (small) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
+                    for (int i = 0; i < 32; ++i) {
+                            x[i] = P.cap * tanh_small(x[i]);
+                            few(i);
+                        }
+                } else {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) s[j][i] = P.cap * tanh_near(s[j][i] * in);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[j][i] *= ct;
+                    for (int i = 0; i < 32; ++i) {
+                            asm volatile("" : "+v"(x[i]));  // the polynomials are not to be formed in front of the branch
+                            x[i] = P.cap * tanh_near(x[i]);
+                            few(i);
+                        }
+                }
             }
-            if (table) {
+            if (P.bias) {
+                const int from = k0 - last_p, to = k0 + kKT - 1 - first_p;  // the wave's distances
+                const int at = k0 + fh * 8 - p;
+                const float* bp = P.bias + (int64_t)kh * group * (2 * P.radius + 1);
+                if (to <= -P.radius || from >= P.radius) {  // one value for all
+                    const float v = table ? biases[mid + (from >= P.radius ? P.radius : -P.radius)] : bp[mid + (from >= P.radius ? P.radius : -P.radius)];
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
+                    for (int i = 0; i < 32; ++i) x[i] += v;
+                } else if (table && from >= -P.radius && to <= P.radius) {  // none clamped
+                    const float* b = biases + mid + at;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        s[u >> 1][(u & 1) * 8 + i] += biases[mid + min(max(k0 + u * 16 + fh * 8 + i - p, -P.radius), P.radius)];
-            } else if (P.bias) {
+                    for (int u = 0; u < 4; ++u)
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
+                        for (int i = 0; i < 8; ++i) {
+                            x[u * 8 + i] += b[u * 16 + i];
+                            few(i);
+                        }
+                } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        s[u >> 1][(u & 1) * 8 + i] += bp[mid + min(max(k0 + u * 16 + fh * 8 + i - p, -P.radius), P.radius)];
+                    for (int u = 0; u < 4; ++u)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int c = mid + min(max(at + u * 16 + i, -P.radius), P.radius);
+                            x[u * 8 + i] += table ? biases[c] : bp[c];
+                            few(i);
+                        }
+                }
             }
         }
-        if (edge) {
+        if (edge && (k0 >= pre || !pre)) {
+            const int c = k0 + fh * 8 - see.lo;
+            const unsigned n = see.hi - see.lo;
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (!visible(k0 + u * 16 + fh * 8 + i)) s[u >> 1][(u & 1) * 8 + i] = -INFINITY;
+                for (int i = 0; i < 8; ++i) {
+                    if ((unsigned)(c + u * 16 + i) >= n) x[u * 8 + i] = -INFINITY;
+                    few(i);
+                }
+        } else if (edge) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (!visible(k0 + u * 16 + fh * 8 + i)) x[u * 8 + i] = -INFINITY;
+                    few(i);
+                }
         }
-        float mt = s[0][0];
+        float mt = x[0];
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[j][i]);
+        for (int i = 0; i < 32; ++i) mt = fmaxf(mt, x[i]);
         if constexpr (!EXTRA) mt *= ct;
         mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
         const float mnew = mt > m + (EXTRA ? kLazy / kLog2e : kLazy) ? mt : m;
@@ -589,16 +648,14 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn_packed_tiles(Packed P, Til
             ao = E == kUnsetE ? 0.f : ldexpf(alpha, max(E - up, -300));
             E = up;
         }
-        const int by = 14 + (flag & kValueExps ? 0 : max(about.y - E, kFarE));
+        const int by = 14 + (flag & kValueExps ? 0 : max(tile_ev - E, kFarE));
         const float up = (float)by - (EXTRA ? 0.f : ref);
         float total = 0.f;
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float x = __builtin_amdgcn_exp2f(EXTRA ? fmaf(s[j][i] - ref, kLog2e, up) : fmaf(s[j][i], ct, up));
-                s[j][i] = x;
-                total += x;
+        for (int i = 0; i < 32; ++i) {
+                const float e = __builtin_amdgcn_exp2f(EXTRA ? fmaf(x[i] - ref, kLog2e, up) : fmaf(x[i], ct, up));
+                x[i] = e;
+                total += e;
             }
         sum = fmaf(sum, alpha, ldexpf(total, -by));
         if (flag & kValueExps) {
@@ -606,8 +663,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn_packed_tiles(Packed P, Til
             for (int u = 0; u < 4; ++u)
 #pragma unroll
                 for (int i = 0; i < 8; ++i)  // an unseen key's weight is zero, its exponent may be above E
-                    s[u >> 1][(u & 1) * 8 + i] =
-                        ldexpf(s[u >> 1][(u & 1) * 8 + i], min(max(exps[kKT + u * 16 + fh * 8 + i] - E, kFarE), 0));
+                    x[u * 8 + i] =
+                        ldexpf(x[u * 8 + i], min(max(exps[kKT + u * 16 + fh * 8 + i] - E, kFarE), 0));
         }
         if (__ballot(ao != 1.0f)) {
 #pragma unroll
@@ -615,57 +672,81 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn_packed_tiles(Packed P, Til
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[dt][i] *= ao;
         }
-        return flag & kNotFinite;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                h2 hi, lo;
+                split_pair(x[u * 8 + i], x[u * 8 + i + 1], hi, lo);
+                ph[u][i] = hi[0], ph[u][i + 1] = hi[1];
+                pl[u][i] = lo[0], pl[u][i + 1] = lo[1];
+            }
     };
-    auto values = [&]() __attribute__((always_inline)) {
-        h8 vf[2][2];  // [step % 2][hi, lo], steps (16 keys, 32 columns), columns fastest
+    // 2 DT steps of two (16 keys, 32 columns), columns fastest; the two accumulators in turn.
+    auto values = [&](const u16* vbuf) __attribute__((always_inline)) {
+        int row0 = fr;
+        asm volatile("" : "+v"(row0));
+        h8 vf[2][2][2];  // [step % 2][of the two][hi, lo]
         auto fetch = [&](int i) __attribute__((always_inline)) {
-            const int row = i % DT * 32 + fr, at = row * kKT + (((i / DT * 2 + fh) ^ swz_v(row)) << 3);
-            vf[i & 1][0] = *(const h8*)(vbuf + at);
-            vf[i & 1][1] = *(const h8*)(vbuf + PART + at);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int ks = (i * 2 + u) / DT, row = (i * 2 + u) % DT * 32 + row0, at = row * kKT + (((ks * 2 + fh) ^ swz_v(row)) << 3);
+                vf[i & 1][u][0] = *(const h8*)(vbuf + at);
+                vf[i & 1][u][1] = *(const h8*)(vbuf + PART + at);
+            }
         };
         fetch(0);
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            h8 ph, pl;
+        for (int i = 0; i < 2 * DT; ++i) {
+            if (i + 1 < 2 * DT) fetch(i + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            const int b = i & 1, ks = i * 2 / DT, dt = i * 2 % DT;
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                h2 hi, lo;
-                split_pair(s[ks >> 1][(ks & 1) * 8 + e], s[ks >> 1][(ks & 1) * 8 + e + 1], hi, lo);
-                ph[e] = hi[0], ph[e + 1] = hi[1];
-                pl[e] = lo[0], pl[e + 1] = lo[1];
-            }
+            for (int u = 0; u < 2; ++u) o[dt + u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[b][u][0], ph[ks], o[dt + u], 0, 0, 0);
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                const int i = ks * DT + dt, b = i & 1;
-                if (i + 1 < 4 * DT) fetch(i + 1);
-                __builtin_amdgcn_sched_barrier(0);
-                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[b][0], ph, o[dt], 0, 0, 0);
-                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[b][0], pl, o[dt], 0, 0, 0);
-                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[b][1], ph, o[dt], 0, 0, 0);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+            for (int u = 0; u < 2; ++u) o[dt + u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[b][u][0], pl[ks], o[dt + u], 0, 0, 0);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) o[dt + u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[b][u][1], ph[ks], o[dt + u], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // The copies have landed, the LDS reads are done, for every wave.
-    auto meet = [&]() __attribute__((always_inline)) { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-
+    // Meeting n: K of tile n and V of tile n - 1 have landed, and nobody reads K of n - 1 or V of
+    // n - 2 any more, whose buffers then take K of n + 1 and V of n. The two waves of a SIMD (w and
+    // w + 4) meet at different places of their work, the first in front of the weighted values,
+    // the other in front of the softmax: one's MFMAs run while the other takes exponentials.
+    auto meet = [&](int n, u16* kn, u16* vn) __attribute__((always_inline)) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (n + 1 < nt) copy(tile_of(n + 1), 0, kn);
+        if (n < nt) copy(tile_of(n), 1, vn);
+    };
+    const bool late = w < WAVES / 2;
     int bad_first = nt, bad_last = -1;  // the tiles that hold values that are not finite
-    for (int n = n0; n < nt; ++n) {
+    // kc, vc: this tile's; vn: the next one's V (the next but one's K goes into kc)
+    auto step = [&](int n, u16* kc, u16* vc, u16* vn) __attribute__((always_inline)) {
         const int tile = tile_of(n), k0 = tile * kKT - T.z;
         const bool mine = active && ((k0 < pre && k0 + kKT > 0) || (k0 < last_hi && k0 + kKT > first_lo));
-        meet();  // K of this tile is there, V of the last one no longer read
-        copy(tile, 1, vbuf);
-        if (mine) scores();
-        meet();
-        if (n + 1 < nt) copy(tile_of(n + 1), 0, kbuf);
-        if (mine) {
-            if (softmax(k0, tile)) {
-                bad_first = min(bad_first, n);
-                bad_last = n;
-            }
-            values();
+        // asked for here, so that the answer is there after the products
+        const int4 about = info[tile];
+        const int tile_ek = __builtin_amdgcn_readfirstlane(about.x), tile_ev = __builtin_amdgcn_readfirstlane(about.y),
+                  flag = __builtin_amdgcn_readfirstlane(about.z);
+        if (flag & kNotFinite) {
+            bad_first = min(bad_first, n);
+            bad_last = n;
         }
+        if (!mine) {
+            meet(n + 1, kc, vn);
+            return;
+        }
+        scores(kc);
+        if (!late) meet(n + 1, kc, vn);
+        softmax(k0, tile, tile_ek, tile_ev, flag);
+        if (late) meet(n + 1, kc, vn);
+        values(vc);
+    };
+    if (n0 < nt) meet(n0, kbuf1, vbuf0);
+    for (int n = n0; n < nt; n += 2) {
+        step(n, kbuf0, vbuf0, vbuf1);
+        if (n + 1 < nt) step(n + 1, kbuf1, vbuf1, vbuf0);
     }
 
     if (r >= rows) return;
@@ -953,31 +1034,33 @@ void run_few(const Packed& P, bool out16, int64_t items, int rows) {
     join_parts(P, out16, S, !extra);
 }
 
-// False where the tiles' scratch cannot be had.
+// `rows` rows (queries times the heads of a group) of `live` sequences; false where the tiles'
+// scratch cannot be had.
 template <int DP>
-bool run_tiles(const Packed& P, bool out16, int64_t items) {
+bool run_tiles(const Packed& P, bool out16, int64_t rows, int64_t live) {
     const bool kvec = P.d % 8 == 0 && aligned16(P.k) && aligned16(P.v),
                qvec = P.d % 8 == 0 && aligned16(P.q) && (out16 ? ((uintptr_t)P.out & 7) == 0 : aligned16(P.out));
     // Parts of the keys while the workgroups do not fill the chip, of eight tiles of an average sequence at least.
-    const int64_t wgs = items * P.kv_heads, keys = P.Tk / std::max(1, P.seqs), ntiles = (P.Tk + kKT - 1) / kKT;
+    const int64_t items = rows / (32 * kWaves<DP>) + live, wgs = items * P.kv_heads, keys = P.Tk / std::max(1, P.seqs), ntiles = (P.Tk + kKT - 1) / kKT;
+    if (wgs * 64 * kWaves<DP> > kMaxGridItems) return false;
     const size_t cells = (size_t)ntiles * P.kv_heads, tb = cells * 4 * kKT * DP * 2;
     char* front;
-    const Parts S = make_parts(P, std::max<int64_t>(1, std::min<int64_t>(2 * num_cus() / wgs, keys / (8 * kKT))),
+    const Parts S = make_parts(P, std::max<int64_t>(1, std::min<int64_t>(num_cus() * (8 / kWaves<DP>) / wgs, keys / (8 * kKT))),
                                tb + cells * (sizeof(int4) + 2 * kKT * sizeof(int)), front);
     if (!front) return false;
     const Tiles X{(u16*)front, (int4*)(front + tb), (int*)(front + tb + cells * sizeof(int4)), (int)ntiles};
     const dim3 sg((unsigned)ntiles, (unsigned)P.kv_heads);
-    if (kvec) k_attn_packed_split<DP, true><<<sg, 64 * kWaves, 0, stream()>>>(P, X);
-    else k_attn_packed_split<DP, false><<<sg, 64 * kWaves, 0, stream()>>>(P, X);
-    // What two workgroups of a CU leave of its LDS takes the bias of a group's heads, if it fits.
+    if (kvec) k_attn_packed_split<DP, true><<<sg, 64 * kSplitWaves, 0, stream()>>>(P, X);
+    else k_attn_packed_split<DP, false><<<sg, 64 * kSplitWaves, 0, stream()>>>(P, X);
+    // What the tiles leave of a CU's LDS takes the bias of a group's heads, if it fits.
     const int64_t values = P.bias ? (int64_t)(P.heads / P.kv_heads) * (2 * P.radius + 1) : 0;
-    const int table = values * 4 <= 14 * 1024 ? (int)values : 0;
+    const int table = values * 4 <= 14 * 1024 * (kWaves<DP> / 4) ? (int)values : 0;
     const bool extra = P.cap > 0.f || P.bias;
     using T_ = std::true_type;
     using F_ = std::false_type;
     auto go = [&](auto ex, auto ve) {
         k_attn_packed_tiles<DP, decltype(ex)::value, decltype(ve)::value>
-            <<<dim3((unsigned)wgs, (unsigned)S.n), kThreads, (unsigned)table * 4, stream()>>>(P, X, out16, (int)items, table, S);
+            <<<dim3((unsigned)wgs, (unsigned)S.n), 64 * kWaves<DP>, (unsigned)table * 4, stream()>>>(P, X, out16, (int)items, table, S);
     };
     if (extra) qvec ? go(T_(), T_()) : go(T_(), F_());
     else qvec ? go(F_(), T_()) : go(F_(), F_());
@@ -1030,9 +1113,8 @@ void run_attention_packed(const float* q, const float* k, const float* v, void* 
             return;
         }
     }
-    const int64_t rows = Tq * group, items = rows / kTileRows + live;
-    if (d <= 128 && rows < kMost && items * kv_heads * kThreads <= kMaxGridItems && (Tk + kKT) * 4 <= kMaxGridItems) {
-        if (d <= 64 ? run_tiles<64>(P, out16, items) : run_tiles<128>(P, out16, items)) {
+    if (d <= 128 && Tq * group < kMost && (Tk + kKT) * 4 <= kMaxGridItems) {
+        if (d <= 64 ? run_tiles<64>(P, out16, Tq * group, live) : run_tiles<128>(P, out16, Tq * group, live)) {
             launched(op);
             return;
         }
