@@ -559,13 +559,12 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
         if constexpr (EXTRA) {
             const int mid = (h - kh * group) * (2 * P.radius + 1) + P.radius;
             const float in = P.cap > 0.f ? ct / P.cap : ct;
-            float top = 0.f;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                    x[i] *= in;
-                    top = fmaxf(top, fabsf(x[i]));
-                }
+            for (int i = 0; i < 32; ++i) x[i] *= in;
             if (P.cap > 0.f) {
+                float top = 0.f;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(x[i]));
                 // Scores well inside the cap, as most are, take the polynomial alone (half the
                 // instructions, no exponential).
                 const bool small = !__ballot(!(top < kTanhNear));
@@ -649,14 +648,19 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
             E = up;
         }
         const int by = 14 + (flag & kValueExps ? 0 : max(tile_ev - E, kFarE));
-        const float up = (float)by - (EXTRA ? 0.f : ref);
         float total = 0.f;
+        // A reference far out (biases of the type's lowest value) is taken off before the product,
+        // which would overflow.
+        if (EXTRA && __ballot(!(fabsf(ref) < 1e4f))) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-                const float e = __builtin_amdgcn_exp2f(EXTRA ? fmaf(x[i] - ref, kLog2e, up) : fmaf(x[i], ct, up));
-                x[i] = e;
-                total += e;
-            }
+            for (int i = 0; i < 32; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i] - ref, kLog2e, (float)by));
+        } else {
+            const float f = EXTRA ? kLog2e : ct, up = (float)by - (EXTRA ? ref * kLog2e : ref);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], f, up));
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) total += x[i];
         sum = fmaf(sum, alpha, ldexpf(total, -by));
         if (flag & kValueExps) {
 #pragma unroll
