@@ -157,33 +157,36 @@ __global__ __launch_bounds__(kLoraThreads) void k_lora_down(Lora P) {
         for (int j = 0; j < RT; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    Eight<TX> xn[2][RF];
-    Eight<TW> an[2][RT];
-    auto load = [&](int k) __attribute__((always_inline)) {
+    // bf16 rows are half the bytes a block: two blocks on their way
+    constexpr int DEPTH = sizeof(TX) == 2 ? 2 : 1, U = 2 * DEPTH;
+    Eight<TX> xn[U][RF];
+    Eight<TW> an[U][RT];
+    const int step = 32 * kLoraWaves * P.splits;
+    auto load = [&](int k0) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < U; ++u) {
+            const int k = k0 + u / 2 * step;
 #pragma unroll
-            for (int i = 0; i < RF; ++i) xn[u][i].template load<VEC>(x[i], k + fh * 16 + u * 8, P.K);
+            for (int i = 0; i < RF; ++i) xn[u][i].template load<VEC>(x[i], k + fh * 16 + u % 2 * 8, P.K);
 #pragma unroll
-            for (int i = 0; i < RT; ++i) an[u][i].template load<VEC>(a[i], k + fh * 16 + u * 8, P.K);
+            for (int i = 0; i < RT; ++i) an[u][i].template load<VEC>(a[i], k + fh * 16 + u % 2 * 8, P.K);
         }
     };
-    const int step = 32 * kLoraWaves * P.splits;
     int k = (blockIdx.y * kLoraWaves + w) * 32;
     if (k < P.K) load(k);
-    for (; k < P.K; k += step) {
-        Eight<TX> xc[2][RF];
-        Eight<TW> ac[2][RT];
+    for (; k < P.K; k += DEPTH * step) {
+        Eight<TX> xc[U][RF];
+        Eight<TW> ac[U][RT];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < U; ++u) {
 #pragma unroll
             for (int i = 0; i < RF; ++i) xc[u][i] = xn[u][i];
 #pragma unroll
             for (int i = 0; i < RT; ++i) ac[u][i] = an[u][i];
         }
-        if (k + step < P.K) load(k + step);
+        if (k + DEPTH * step < P.K) load(k + DEPTH * step);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < U; ++u) {
             bf16x8 xp[RF][Eight<TX>::kParts];
 #pragma unroll
             for (int i = 0; i < RF; ++i) xc[u][i].parts(xp[i]);
@@ -217,12 +220,14 @@ __global__ __launch_bounds__(kLoraThreads) void k_lora_down(Lora P) {
 
 // ---------------------------------------------------------------------------
 // C[t, :] (+)= H[t] B_a^T over the ranks j0 .. j0 + 16 KS. A wave keeps the parts of 32 rows
-// of H in registers and goes through `columns` columns, 32 at a time. The four waves of
-// a workgroup have neighbouring rows and the same columns (their B comes from the L1),
-// or, with FEW, the same rows and neighbouring columns.
+// of H in registers and goes through `columns` columns, 128 at a time: four products, the
+// j-th with the columns 4 i + j, so that a lane's four results of a row are neighbours and a
+// row of C moves in 512-byte pieces (CV; else by single values). The four waves of a
+// workgroup have neighbouring rows and the same columns (their B comes from the L1), or,
+// with FEW, the same rows and neighbouring columns.
 // ---------------------------------------------------------------------------
-template <class TW, int KS, bool FEW, bool VEC>
-__global__ __launch_bounds__(kLoraThreads) void k_lora_up(Lora P, int j0, int columns) {
+template <class TW, int KS, bool FEW, bool VEC, bool CV>
+__global__ __launch_bounds__(kLoraThreads, KS <= 4 ? 2 : 1) void k_lora_up(Lora P, int j0, int columns) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, fr = lane & 31, fh = lane >> 5;
     dev::SpanTile t;
     if (!dev::find_tile(P.runs, P.count, P.M, 1, FEW ? 32 : 32 * kLoraWaves, blockIdx.x, t)) return;
@@ -234,13 +239,22 @@ __global__ __launch_bounds__(kLoraThreads) void k_lora_up(Lora P, int j0, int co
     if (left <= 0 || n >= n1 || (P.accumulate && j0 >= rank)) return;
     const int64_t first = t.first + row0;
     float* c = P.c + first * P.ldc;
-    if (adapter < 0) {  // only without accumulate; B may not be there at all
-        for (; n < n1; n += 32)
+    auto row_of = [&](int e) { return (e >> 2) * 8 + fh * 4 + (e & 3); };
+    auto put = [&](int e, int col, const f4& v) __attribute__((always_inline)) {
+        float* to = c + row_of(e) * P.ldc + col;
+        if (row_of(e) >= left) return;
+        if constexpr (CV) {
+            if (col < P.N) dev::st_stream((f4*)to, v);
+        } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int r = (e >> 2) * 8 + fh * 4 + (e & 3);
-                if (n + fr < P.N && r < left) c[r * P.ldc + n + fr] = 0.f;
-            }
+            for (int j = 0; j < 4; ++j)
+                if (col + j < P.N) to[j] = v[j];
+        }
+    };
+    if (adapter < 0) {  // only without accumulate; B may not be there at all
+        for (; n < n1; n += 128)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) put(e, n + fr * 4, f4{0.f, 0.f, 0.f, 0.f});
         return;
     }
     bf16x8 hp[KS][3];
@@ -259,35 +273,160 @@ __global__ __launch_bounds__(kLoraThreads) void k_lora_up(Lora P, int j0, int co
         v.parts(hp[ks]);
     }
     const TW* b = (const TW*)P.b + (int64_t)adapter * P.N * P.rank;
-    for (; n < n1; n += 32) {
-        const int col = n + fr;
-        const bool in = col < P.N;
-        Eight<TW> bn[KS];
-        const TW* row = b + (int64_t)min(col, P.N - 1) * P.rank;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) bn[ks].template load<VEC>(row, j0 + ks * 16 + fh * 8, rank);
-        if (VEC && rank % 8) {  // what lies behind the ranks that count may be anything
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) bn[ks].cut(rank - (j0 + ks * 16 + fh * 8));
-        }
-        f32x16 acc, y;
+    for (; n < n1; n += 128) {
+        const int col = n + fr * 4;
+        f4 y[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const int r = (e >> 2) * 8 + fh * 4 + (e & 3);
-            acc[e] = P.accumulate && in && r < left ? c[r * P.ldc + col] : 0.f;
-            y[e] = 0.f;
+            y[e] = f4{0.f, 0.f, 0.f, 0.f};
+            if (!P.accumulate || row_of(e) >= left) continue;
+            const float* from = c + row_of(e) * P.ldc + col;
+            if constexpr (CV) {
+                if (col < P.N) y[e] = *(const f4*)from;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (col + j < P.N) y[e][j] = from[j];
+            }
+        }
+        f32x16 acc[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            Eight<TW> bn[KS];
+            const TW* row = b + (int64_t)min(col + j, P.N - 1) * P.rank;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) bn[ks].template load<VEC>(row, j0 + ks * 16 + fh * 8, rank);
+            if (VEC && rank % 8) {  // what lies behind the ranks that count may be anything
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) bn[ks].cut(rank - (j0 + ks * 16 + fh * 8));
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                bf16x8 bp[Eight<TW>::kParts];
+                bn[ks].parts(bp);
+                acc[j] = multiply<3, Eight<TW>::kParts>(hp[ks], bp, acc[j]);
+            }
         }
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            bf16x8 bp[Eight<TW>::kParts];
-            bn[ks].parts(bp);
-            y = multiply<3, Eight<TW>::kParts>(hp[ks], bp, y);
+        for (int e = 0; e < 16; ++e) put(e, col, y[e] + f4{acc[0][e], acc[1][e], acc[2][e], acc[3][e]});
+    }
+}
+
+// The same for runs of many rows: the waves of a workgroup have neighbouring rows and share
+// each 128 columns of B through LDS. Read from memory by its rows, a fragment (32 rows of B,
+// 16 bytes each a lane) costs the L1 an access a lane: 60 million of them took 112 of 185 us
+// at [12528,64] x [10240,64]^T. The copies to LDS are of whole rows, 16 bytes a lane, two
+// stages; LDS row j*32 + i holds column 4 i + j, its 16-byte piece c at c ^ swizzle(row), so
+// that 16 neighbouring rows are read from 16 different pieces of a 256-byte window.
+template <class TW, int KS, bool CV>
+__global__ __launch_bounds__(kLoraThreads, KS <= 4 ? 2 : 1) void k_lora_up_shared(Lora P, int j0, int columns) {
+    constexpr int PER = 16 / sizeof(TW), PIECES = KS * 16 / PER, ROW = PIECES * 16, STAGE = 128 * ROW;  // pieces a row, bytes
+    constexpr int TURN = PIECES >= 16 ? 1 : 16 / PIECES;  // rows in 256 bytes
+    __shared__ __attribute__((aligned(1024))) char stage0[STAGE], stage1[STAGE];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 31, fh = lane >> 5;
+    dev::SpanTile t;
+    if (!dev::find_tile(P.runs, P.count, P.M, 1, 32 * kLoraWaves, blockIdx.x, t)) return;
+    int rank;
+    const int adapter = adapter_of(P, t, rank);
+    const int n0 = blockIdx.y * columns, n1 = min(n0 + columns, P.N);
+    if (P.accumulate && j0 >= rank) return;
+    const int row0 = t.row0 + w * 32, left = t.rows - row0;
+    const int64_t first = t.first + row0;
+    float* c = P.c + first * P.ldc;
+    auto row_of = [&](int e) { return (e >> 2) * 8 + fh * 4 + (e & 3); };
+    auto put = [&](int e, int col, const f4& v) __attribute__((always_inline)) {
+        float* to = c + row_of(e) * P.ldc + col;
+        if (row_of(e) >= left) return;
+        if constexpr (CV) {
+            if (col < P.N) dev::st_stream((f4*)to, v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (col + j < P.N) to[j] = v[j];
         }
+    };
+    if (adapter < 0) {  // only without accumulate; B may not be there at all
+        for (int n = n0; n < n1; n += 128)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) put(e, n + fr * 4, f4{0.f, 0.f, 0.f, 0.f});
+        return;
+    }
+    const TW* b = (const TW*)P.b + (int64_t)adapter * P.N * P.rank;
+    auto swizzle = [](int row) { return (row / TURN) & (PIECES - 1); };
+    auto copy = [&](int n, char* to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < STAGE / (kLoraThreads * 16); ++i) {
+            const int chunk = (i * kLoraWaves + w) * 64, at = chunk + lane, row = at / PIECES, c = (at % PIECES) ^ swizzle(row);
+            const int col = min(n + (row & 31) * 4 + (row >> 5), P.N - 1), k = j0 + c * PER;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(b + (int64_t)col * P.rank + (k < P.rank ? k : 0)),
+                                             (__attribute__((address_space(3))) void*)(to + chunk * 16), 16, 0, 0);
+        }
+    };
+    copy(n0, stage0);
+    bf16x8 hp[KS][3];
+    const float* h = P.h + (first + min(fr, max(left, 1) - 1)) * P.hrank;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        const int at = j0 + ks * 16 + fh * 8;
+        Eight<float> v;
+        v.a = v.b = f4{0.f, 0.f, 0.f, 0.f};
+        if (at < rank && left > 0)
+            for (int s = 0; s < P.splits; ++s) {
+                const f4* q = (const f4*)(h + (int64_t)s * P.M * P.hrank + at);
+                v.a += q[0];
+                v.b += q[1];
+            }
+        v.parts(hp[ks]);
+    }
+    auto step = [&](int n, const char* from, char* to) __attribute__((always_inline)) {
+        // this stage has landed and nobody reads the other one any more
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (n + 128 < n1) copy(n + 128, to);
+        if (left <= 0) return;
+        const int col = n + fr * 4;
+        f4 y[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const int r = (e >> 2) * 8 + fh * 4 + (e & 3);
-            if (in && r < left) c[r * P.ldc + col] = acc[e] + y[e];
+            y[e] = f4{0.f, 0.f, 0.f, 0.f};
+            if (!P.accumulate || row_of(e) >= left) continue;
+            const float* at = c + row_of(e) * P.ldc + col;
+            if constexpr (CV) {
+                if (col < P.N) y[e] = dev::ld_stream((const f4*)at);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (col + j < P.N) y[e][j] = at[j];
+            }
         }
+        f32x16 acc[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const int row = j * 32 + fr;
+                Eight<TW> v;
+                if constexpr (sizeof(TW) == 2) {
+                    v.a = *(const u32x4*)(from + row * ROW + (((ks * 2 + fh) ^ swizzle(row)) << 4));
+                } else {
+                    v.a = *(const f4*)(from + row * ROW + (((ks * 4 + fh * 2) ^ swizzle(row)) << 4));
+                    v.b = *(const f4*)(from + row * ROW + (((ks * 4 + fh * 2 + 1) ^ swizzle(row)) << 4));
+                }
+                if (j0 + ks * 16 + 16 > rank) v.cut(rank - (j0 + ks * 16 + fh * 8));  // what lies behind the ranks that count may be anything
+                bf16x8 bp[Eight<TW>::kParts];
+                v.parts(bp);
+                acc[j] = multiply<3, Eight<TW>::kParts>(hp[ks], bp, acc[j]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) put(e, col, y[e] + f4{acc[0][e], acc[1][e], acc[2][e], acc[3][e]});
+    };
+    for (int n = n0; n < n1; n += 256) {
+        step(n, stage0, stage1);
+        if (n + 128 < n1) step(n + 128, stage1, stage0);
     }
 }
 
@@ -302,9 +441,9 @@ void launch_lora(Lora P, int64_t M, bool vec) {
     const int rt = P.rank <= 32 ? 1 : P.rank <= 64 ? 2 : 4, rf = few || rt > 2 || !vec ? 1 : 2;
     const int64_t down = M / (32 * rf) + std::min<int64_t>(P.count, M);
     if (P.rank > 0) {
-        // parts of K until the chip has two workgroups a CU, while each wave keeps two blocks
+        // parts of K until the chip has four workgroups a CU, while each wave keeps two blocks
         const int64_t most = std::max<int64_t>(1, P.K / (64 * kLoraWaves));
-        P.splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, 2 * cus / std::max<int64_t>(1, M / (32 * rf) + 1), 8}));
+        P.splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, 4 * cus / std::max<int64_t>(1, M / (32 * rf) + 1), 8}));
     }
     P.hrank = (P.rank + 31) / 32 * 32;
     P.h = (float*)scratch(std::max<size_t>((size_t)P.splits * M * P.hrank * 4, 4));
@@ -324,13 +463,23 @@ void launch_lora(Lora P, int64_t M, bool vec) {
     // columns a wave: enough waves to fill the chip, at most 512
     const int64_t waves = std::max<int64_t>(1, M / 32 + (few ? P.count : 0));
     int64_t columns = 512;
-    while (columns > 32 && waves * ((P.N + columns - 1) / columns) < 16 * (int64_t)cus) columns /= 2;
-    const bool bvec = P.rank % 8 == 0 && aligned16(P.b);
+    while (columns > 128 && waves * ((P.N + columns - 1) / columns) < 16 * (int64_t)cus) columns /= 2;
+    const bool bvec = P.rank % 8 == 0 && aligned16(P.b), cvec = P.N % 4 == 0 && P.ldc % 4 == 0 && aligned16(P.c);
     for (int j0 = 0; j0 == 0 || j0 < P.rank; j0 += 128) {
         const int ks = std::min(P.rank - j0, 128);
         const dim3 grid((unsigned)tiles, (unsigned)((P.N + columns * (few ? kLoraWaves : 1) - 1) / (columns * (few ? kLoraWaves : 1))));
         auto go = [&](auto k, auto f, auto v) {
-            k_lora_up<TW, decltype(k)::value, decltype(f)::value, decltype(v)::value><<<grid, kLoraThreads, 0, stream()>>>(P, j0, (int)columns);
+            constexpr int KS = decltype(k)::value;
+            constexpr bool F = decltype(f)::value, V = decltype(v)::value;
+            // pieces of 16 bytes, whole ones a row
+            if constexpr (!F)
+                if (P.rank % (16 / sizeof(TW)) == 0 && aligned16(P.b)) {
+                    if (cvec) k_lora_up_shared<TW, KS, true><<<grid, kLoraThreads, 0, stream()>>>(P, j0, (int)columns);
+                    else k_lora_up_shared<TW, KS, false><<<grid, kLoraThreads, 0, stream()>>>(P, j0, (int)columns);
+                    return;
+                }
+            if (cvec) k_lora_up<TW, KS, F, V, true><<<grid, kLoraThreads, 0, stream()>>>(P, j0, (int)columns);
+            else k_lora_up<TW, KS, F, V, false><<<grid, kLoraThreads, 0, stream()>>>(P, j0, (int)columns);
         };
         auto with = [&](auto f, auto v) {
             if (ks <= 16) go(integral_constant<int, 1>(), f, v);
@@ -339,7 +488,7 @@ void launch_lora(Lora P, int64_t M, bool vec) {
             else go(integral_constant<int, 8>(), f, v);
         };
         if (few) bvec ? with(T_(), T_()) : with(T_(), F_());
-        else bvec ? with(F_(), T_()) : with(F_(), F_());
+        else with(F_(), F_());
         P.accumulate = 1;
     }
 }
