@@ -950,40 +950,42 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_packed_few(Packed P, in
     }
 }
 
-// out from the parts: a workgroup of eight 32-lane groups per (query row, head), each taking
-// every eighth part. `unit`: log2(e) where the references are not in log2 units.
-__global__ __launch_bounds__(256) void k_attn_packed_join(Packed P, int out16, Parts S, float unit) {
-    __shared__ float so[8][128];
-    __shared__ float sm[8], sl[8];
+// out from the parts: a workgroup of sixteen 32-lane groups per (query row, head), each taking
+// every sixteenth part, once the parts' weights are known. `unit`: log2(e) where the references
+// are not in log2 units.
+constexpr int kMaxParts = 256, kJoin = 16;
+__global__ __launch_bounds__(32 * kJoin) void k_attn_packed_join(Packed P, int out16, Parts S, float unit) {
+    __shared__ float so[kJoin][128], weight[kMaxParts], tops[kJoin / 2], sums[kJoin / 2];
     const int t = blockIdx.x, h = blockIdx.y, c = (threadIdx.x & 31) * 4, g = threadIdx.x >> 5;
     if (dev::span_of_row(P.spans, P.seqs, t, P.Tq) < 0) return;
     const int64_t row = (int64_t)t * P.heads + h, cell = row * S.n;
-    float top = -INFINITY, l = 0.f;
+    const int i = threadIdx.x;
+    const f2 ml = i < S.n ? S.ml[cell + i] : f2{-INFINITY, 0.f};
+    const float mine = dev::wave_max(ml.x);
+    if ((i & 63) == 0) tops[i >> 6] = mine;
+    __syncthreads();
+    float top = tops[0];
+#pragma unroll
+    for (int k = 1; k < kJoin / 2; ++k) top = fmaxf(top, tops[k]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    const float x = __builtin_amdgcn_exp2f((ml.x - ref) * unit);
+    if (i < kMaxParts) weight[i] = x;
+    const float part = dev::wave_sum(i < S.n ? x * ml.y : 0.f);
+    if ((i & 63) == 0) sums[i >> 6] = part;
+    __syncthreads();
     f4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int s = g; s < S.n; s += 8) {
-        const f2 ml = S.ml[cell + s];
-        const float mnew = fmaxf(top, ml.x), ref = mnew == -INFINITY ? 0.f : mnew;
-        const float keep = __builtin_amdgcn_exp2f((top - ref) * unit), add = __builtin_amdgcn_exp2f((ml.x - ref) * unit);
-        l = l * keep + ml.y * add;
-        if (c < P.d) v = v * keep + *(const f4*)(S.o + (cell + s) * S.stride + c) * add;
-        top = mnew;
+    if (c < P.d) {
+#pragma unroll 4
+        for (int s = g; s < S.n; s += kJoin) v += weight[s] * *(const f4*)(S.o + (cell + s) * S.stride + c);
     }
     *(f4*)&so[g][c] = v;
-    if (c == 0) sm[g] = top, sl[g] = l;
     __syncthreads();
     if (g || c >= P.d) return;
-    top = sm[0];
+    float l = 0.f;
 #pragma unroll
-    for (int i = 1; i < 8; ++i) top = fmaxf(top, sm[i]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    v = f4{0.f, 0.f, 0.f, 0.f};
-    l = 0.f;
+    for (int k = 0; k < kJoin / 2; ++k) l += sums[k];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float x = __builtin_amdgcn_exp2f((sm[i] - ref) * unit);
-        l = fmaf(x, sl[i], l);
-        v += x * *(const f4*)&so[i][c];
-    }
+    for (int k = 1; k < kJoin; ++k) v += *(const f4*)&so[k][c];
     v *= l == 0.f ? 0.f : 1.0f / l;
     const int64_t at = row * P.d + c;
 #pragma unroll
@@ -1013,7 +1015,7 @@ Parts make_parts(const Packed& P, int64_t n, size_t behind, char*& front) {
 
 void join_parts(const Packed& P, bool out16, const Parts& S, bool log2_units) {
     if (S.n > 1)
-        k_attn_packed_join<<<dim3((unsigned)P.Tq, (unsigned)P.heads), 256, 0, stream()>>>(P, out16, S, log2_units ? 1.0f : kLog2e);
+        k_attn_packed_join<<<dim3((unsigned)P.Tq, (unsigned)P.heads), 32 * kJoin, 0, stream()>>>(P, out16, S, log2_units ? 1.0f : kLog2e);
 }
 
 template <int DP>
@@ -1022,7 +1024,7 @@ void run_few(const Packed& P, bool out16, int64_t items, int rows) {
     // Parts of the keys until there are eight workgroups a CU, each wave with two chunks of an average sequence.
     const int64_t wgs = items * P.kv_heads, keys = P.Tk / std::max(1, P.seqs);
     char* none;
-    const Parts S = make_parts(P, std::max<int64_t>(1, std::min<int64_t>({8 * num_cus() / wgs, keys / (kFewWaves * 64), 256})), 0, none);
+    const Parts S = make_parts(P, std::max<int64_t>(1, std::min<int64_t>({8 * num_cus() / wgs, keys / (kFewWaves * 64), (int64_t)kMaxParts})), 0, none);
     auto go = [&](auto r, auto ex) {
         k_attn_packed_few<DP, decltype(r)::value, decltype(ex)::value>
             <<<dim3((unsigned)wgs, (unsigned)S.n), 64 * kFewWaves, 0, stream()>>>(P, out16, S);
@@ -1049,7 +1051,7 @@ bool run_tiles(const Packed& P, bool out16, int64_t rows, int64_t live) {
     if (wgs * 64 * kWaves<DP> > kMaxGridItems) return false;
     const size_t cells = (size_t)ntiles * P.kv_heads, tb = cells * 4 * kKT * DP * 2;
     char* front;
-    const Parts S = make_parts(P, std::max<int64_t>(1, std::min<int64_t>(num_cus() * (8 / kWaves<DP>) / wgs, keys / (8 * kKT))),
+    const Parts S = make_parts(P, std::max<int64_t>(1, std::min<int64_t>({num_cus() * (8 / kWaves<DP>) / wgs, keys / (8 * kKT), (int64_t)kMaxParts})),
                                tb + cells * (sizeof(int4) + 2 * kKT * sizeof(int)), front);
     if (!front) return false;
     const Tiles X{(u16*)front, (int4*)(front + tb), (int*)(front + tb + cells * sizeof(int4)), (int)ntiles};

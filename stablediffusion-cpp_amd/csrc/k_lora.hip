@@ -218,6 +218,36 @@ __global__ __launch_bounds__(kLoraThreads) void k_lora_down(Lora P) {
     }
 }
 
+// A row's share of H (eight ranks of each step of 16 from j0 on), its parts of K summed, as MFMA operands.
+template <int KS>
+__device__ __forceinline__ void parts_of_h(const Lora& P, int64_t row, int j0, int rank, int fh, bf16x8 (&hp)[KS][3]) {
+    constexpr int AHEAD = KS >= 8 ? 1 : KS >= 4 ? 2 : 4;  // parts asked for at once
+    const float* h = P.h + row * P.hrank + j0 + fh * 8;
+    const int64_t next = (int64_t)P.M * P.hrank;
+    Eight<float> v[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) v[ks].a = v[ks].b = f4{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < P.splits; s += AHEAD) {
+        f4 x[AHEAD][KS][2];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                x[u][ks][0] = x[u][ks][1] = f4{0.f, 0.f, 0.f, 0.f};
+                if (s + u < P.splits && j0 + ks * 16 + fh * 8 < rank) {
+                    const f4* q = (const f4*)(h + (s + u) * next + ks * 16);
+                    x[u][ks][0] = q[0], x[u][ks][1] = q[1];
+                }
+            }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) v[ks].a += x[u][ks][0], v[ks].b += x[u][ks][1];
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) v[ks].parts(hp[ks]);
+}
+
 // ---------------------------------------------------------------------------
 // C[t, :] (+)= H[t] B_a^T over the ranks j0 .. j0 + 16 KS. A wave keeps the parts of 32 rows
 // of H in registers and goes through `columns` columns, 128 at a time: four products, the
@@ -258,20 +288,7 @@ __global__ __launch_bounds__(kLoraThreads, KS <= 4 ? 2 : 1) void k_lora_up(Lora 
         return;
     }
     bf16x8 hp[KS][3];
-    const float* h = P.h + (first + min(fr, left - 1)) * P.hrank;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-        const int at = j0 + ks * 16 + fh * 8;
-        Eight<float> v;
-        v.a = v.b = f4{0.f, 0.f, 0.f, 0.f};
-        if (at < rank)
-            for (int s = 0; s < P.splits; ++s) {
-                const f4* q = (const f4*)(h + (int64_t)s * P.M * P.hrank + at);
-                v.a += q[0];
-                v.b += q[1];
-            }
-        v.parts(hp[ks]);
-    }
+    parts_of_h<KS>(P, first + min(fr, left - 1), j0, rank, fh, hp);
     const TW* b = (const TW*)P.b + (int64_t)adapter * P.N * P.rank;
     for (; n < n1; n += 128) {
         const int col = n + fr * 4;
@@ -320,7 +337,7 @@ __global__ __launch_bounds__(kLoraThreads, KS <= 4 ? 2 : 1) void k_lora_up(Lora 
 // at [12528,64] x [10240,64]^T. The copies to LDS are of whole rows, 16 bytes a lane, two
 // stages; LDS row j*32 + i holds column 4 i + j, its 16-byte piece c at c ^ swizzle(row), so
 // that 16 neighbouring rows are read from 16 different pieces of a 256-byte window.
-template <class TW, int KS, bool CV>
+template <class TW, int KS, bool ACC, bool CV>
 __global__ __launch_bounds__(kLoraThreads, KS <= 4 ? 2 : 1) void k_lora_up_shared(Lora P, int j0, int columns) {
     constexpr int PER = 16 / sizeof(TW), PIECES = KS * 16 / PER, ROW = PIECES * 16, STAGE = 128 * ROW;  // pieces a row, bytes
     constexpr int TURN = PIECES >= 16 ? 1 : 16 / PIECES;  // rows in 256 bytes
@@ -331,7 +348,7 @@ __global__ __launch_bounds__(kLoraThreads, KS <= 4 ? 2 : 1) void k_lora_up_share
     int rank;
     const int adapter = adapter_of(P, t, rank);
     const int n0 = blockIdx.y * columns, n1 = min(n0 + columns, P.N);
-    if (P.accumulate && j0 >= rank) return;
+    if (ACC && j0 >= rank) return;
     const int row0 = t.row0 + w * 32, left = t.rows - row0;
     const int64_t first = t.first + row0;
     float* c = P.c + first * P.ldc;
@@ -366,31 +383,24 @@ __global__ __launch_bounds__(kLoraThreads, KS <= 4 ? 2 : 1) void k_lora_up_share
     };
     copy(n0, stage0);
     bf16x8 hp[KS][3];
-    const float* h = P.h + (first + min(fr, max(left, 1) - 1)) * P.hrank;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-        const int at = j0 + ks * 16 + fh * 8;
-        Eight<float> v;
-        v.a = v.b = f4{0.f, 0.f, 0.f, 0.f};
-        if (at < rank && left > 0)
-            for (int s = 0; s < P.splits; ++s) {
-                const f4* q = (const f4*)(h + (int64_t)s * P.M * P.hrank + at);
-                v.a += q[0];
-                v.b += q[1];
-            }
-        v.parts(hp[ks]);
-    }
+    parts_of_h<KS>(P, t.first + min(row0 + fr, t.rows - 1), j0, rank, fh, hp);
+    auto landed = [] { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
+    landed();
     auto step = [&](int n, const char* from, char* to) __attribute__((always_inline)) {
-        // this stage has landed and nobody reads the other one any more
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        // This stage has landed (waited for in front of the last stores of C, which have a whole
+        // step to leave) and nobody reads the other one any more.
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (n + 128 < n1) copy(n + 128, to);
-        if (left <= 0) return;
+        if (left <= 0) {
+            landed();
+            return;
+        }
         const int col = n + fr * 4;
         f4 y[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             y[e] = f4{0.f, 0.f, 0.f, 0.f};
-            if (!P.accumulate || row_of(e) >= left) continue;
+            if (!ACC || row_of(e) >= left) continue;
             const float* at = c + row_of(e) * P.ldc + col;
             if constexpr (CV) {
                 if (col < P.N) y[e] = dev::ld_stream((const f4*)at);
@@ -421,6 +431,7 @@ __global__ __launch_bounds__(kLoraThreads, KS <= 4 ? 2 : 1) void k_lora_up_share
                 acc[j] = multiply<3, Eight<TW>::kParts>(hp[ks], bp, acc[j]);
             }
         }
+        landed();
 #pragma unroll
         for (int e = 0; e < 16; ++e) put(e, col, y[e] + f4{acc[0][e], acc[1][e], acc[2][e], acc[3][e]});
     };
@@ -441,9 +452,10 @@ void launch_lora(Lora P, int64_t M, bool vec) {
     const int rt = P.rank <= 32 ? 1 : P.rank <= 64 ? 2 : 4, rf = few || rt > 2 || !vec ? 1 : 2;
     const int64_t down = M / (32 * rf) + std::min<int64_t>(P.count, M);
     if (P.rank > 0) {
-        // parts of K until the chip has four workgroups a CU, while each wave keeps two blocks
+        // Parts of K until the chip has four workgroups a CU, while each wave keeps two blocks, and at
+        // most four, which up has to sum: [2480,2560] -> 4096 takes 42 us with two, 38 with four, 44 with eight.
         const int64_t most = std::max<int64_t>(1, P.K / (64 * kLoraWaves));
-        P.splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, 4 * cus / std::max<int64_t>(1, M / (32 * rf) + 1), 8}));
+        P.splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, 4 * cus / std::max<int64_t>(1, M / (32 * rf) + 1), 4}));
     }
     P.hrank = (P.rank + 31) / 32 * 32;
     P.h = (float*)scratch(std::max<size_t>((size_t)P.splits * M * P.hrank * 4, 4));
@@ -460,10 +472,12 @@ void launch_lora(Lora P, int64_t M, bool vec) {
         else vec ? go(Four(), One(), T_()) : go(Four(), One(), F_());
     }
     const int64_t tiles = M / (few ? 32 : 128) + std::min<int64_t>(P.count, M);
-    // columns a wave: enough waves to fill the chip, at most 512
-    const int64_t waves = std::max<int64_t>(1, M / 32 + (few ? P.count : 0));
-    int64_t columns = 512;
-    while (columns > 128 && waves * ((P.N + columns - 1) / columns) < 16 * (int64_t)cus) columns /= 2;
+    // Columns of a workgroup's wave: as many as leave four workgroups a CU (with few rows, soon
+    // done, six), since each begins with H and its parts. Measured, us, for two / four a CU:
+    // [8192,640] -> 5120 rank 12 87 / 79, [12528,3840] -> 10240 rank 64 168 / 167.
+    int64_t columns = 4096;
+    while (columns > 128 && tiles * ((P.N + columns * (few ? kLoraWaves : 1) - 1) / (columns * (few ? kLoraWaves : 1))) < (few ? 6 : 4) * (int64_t)cus)
+        columns /= 2;
     const bool bvec = P.rank % 8 == 0 && aligned16(P.b), cvec = P.N % 4 == 0 && P.ldc % 4 == 0 && aligned16(P.c);
     for (int j0 = 0; j0 == 0 || j0 < P.rank; j0 += 128) {
         const int ks = std::min(P.rank - j0, 128);
@@ -474,8 +488,9 @@ void launch_lora(Lora P, int64_t M, bool vec) {
             // pieces of 16 bytes, whole ones a row
             if constexpr (!F)
                 if (P.rank % (16 / sizeof(TW)) == 0 && aligned16(P.b)) {
-                    if (cvec) k_lora_up_shared<TW, KS, true><<<grid, kLoraThreads, 0, stream()>>>(P, j0, (int)columns);
-                    else k_lora_up_shared<TW, KS, false><<<grid, kLoraThreads, 0, stream()>>>(P, j0, (int)columns);
+                    auto shared = P.accumulate ? (cvec ? k_lora_up_shared<TW, KS, true, true> : k_lora_up_shared<TW, KS, true, false>)
+                                               : (cvec ? k_lora_up_shared<TW, KS, false, true> : k_lora_up_shared<TW, KS, false, false>);
+                    shared<<<grid, kLoraThreads, 0, stream()>>>(P, j0, (int)columns);
                     return;
                 }
             if (cvec) k_lora_up<TW, KS, F, V, true><<<grid, kLoraThreads, 0, stream()>>>(P, j0, (int)columns);
