@@ -442,32 +442,61 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
                                                      0);
         }
     };
-    if (n0 < nt) copy(tile_of(n0), 0, kbuf0);
+    if (n0 < nt) {
+        copy(tile_of(n0), 0, kbuf0);
+        copy(tile_of(n0), 1, vbuf0);
+    }
     if (EXTRA && table)  // [group, 2 radius + 1]
         for (int i = threadIdx.x; i < table; i += kThreads) biases[i] = P.bias[(int64_t)kh * table + i];
 
-    // Q: the B operand of S^T, row qi of head h, dims ds*16 + fh*8 .. +7
-    const float* qp = P.q + (T.first + qi) * inner + (int64_t)h * d;
+    // Q: the B operand of S^T, row qi of head h, dims ds*16 + fh*8 .. +7. Read by its rows a
+    // fragment costs an access a lane (9200 cycles for the 256 rows of a workgroup at d = 128);
+    // whole rows come in 64 dims at a time and are dealt out through a share of the LDS that no
+    // tile is in yet, the 16-byte piece c of row i at c ^ (i & 15).
+    const float* qp = P.q + (int64_t)(T.first + qi) * inner + (int64_t)h * d;
+    float qx[DS][8];
+    if constexpr (VEC) {
+        char* mine = (char*)(w < WAVES / 2 ? kbuf1 : vbuf1) + (w % (WAVES / 2)) * (32 * 256);
+        static_assert(WAVES / 2 * 32 * 256 <= 4 * PART, "Q's rows in LDS");
+#pragma unroll
+        for (int half = 0; half < DP / 64; ++half) {
+            f4 x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {  // four rows a load
+                const int row = i * 4 + (lane >> 4), rr = min(T.row0 + w * 32 + row, rows - 1), qr = rr / group;
+                const float* from = P.q + (int64_t)(T.first + qr) * inner + (int64_t)(kh * group + rr - qr * group) * d;
+                x[i] = *(const f4*)(from + min(half * 64 + (lane & 15) * 4, d - 4));
+            }
+            __builtin_amdgcn_wave_barrier();  // a wave's LDS accesses keep their order
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int row = i * 4 + (lane >> 4);
+                *(f4*)(mine + row * 256 + (((lane & 15) ^ (row & 15)) << 4)) = x[i];
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int ds = half * 4 + k;
+                const f4 u = *(const f4*)(mine + fr * 256 + (((k * 4 + fh * 2) ^ (fr & 15)) << 4)),
+                         v = *(const f4*)(mine + fr * 256 + (((k * 4 + fh * 2 + 1) ^ (fr & 15)) << 4));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) qx[ds][e] = ds * 16 + fh * 8 < d ? (e < 4 ? u[e & 3] : v[e & 3]) : 0.f;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) qx[ds][e] = ds * 16 + fh * 8 + e < d ? qp[ds * 16 + fh * 8 + e] : 0.f;
+    }
     h8 qh[DS], ql[DS];
     int eq;
     {
-        float x[DS][8];
         int top = 0;
 #pragma unroll
-        for (int ds = 0; ds < DS; ++ds) {
-            const int c0 = ds * 16 + fh * 8;
-            if constexpr (VEC) {
-                const float* a = qp + min(c0, d - 8);
-                const f4 u = *(const f4*)a, v = *(const f4*)(a + 4);
+        for (int ds = 0; ds < DS; ++ds)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[ds][e] = c0 < d ? (e < 4 ? u[e & 3] : v[e & 3]) : 0.f;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[ds][e] = c0 + e < d ? qp[c0 + e] : 0.f;
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) top = max(top, abs_bits(x[ds][e]));
-        }
+            for (int e = 0; e < 8; ++e) top = max(top, abs_bits(qx[ds][e]));
         top = max(top, __shfl_xor(top, 32, 64));
         eq = block_exp(top);
         const float sc = copysignf(pow2(-eq), P.scale);  // a negative scale turns q's sign
@@ -476,7 +505,7 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
                 h2 hi, lo;
-                split_pair(x[ds][e] * sc, x[ds][e + 1] * sc, hi, lo);
+                split_pair(qx[ds][e] * sc, qx[ds][e + 1] * sc, hi, lo);
                 qh[ds][e] = hi[0], qh[ds][e + 1] = hi[1];
                 ql[ds][e] = lo[0], ql[ds][e + 1] = lo[1];
             }
@@ -721,7 +750,7 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
     auto meet = [&](int n, u16* kn, u16* vn) __attribute__((always_inline)) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (n + 1 < nt) copy(tile_of(n + 1), 0, kn);
-        if (n < nt) copy(tile_of(n), 1, vn);
+        if (n > n0 && n < nt) copy(tile_of(n), 1, vn);  // the first one came with its K
     };
     const bool late = w < WAVES / 2;
     int bad_first = nt, bad_last = -1;  // the tiles that hold values that are not finite
