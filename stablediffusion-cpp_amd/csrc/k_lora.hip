@@ -131,26 +131,20 @@ __device__ __forceinline__ int adapter_of(const Lora& P, const dev::SpanTile& t,
 // ---------------------------------------------------------------------------
 // H[part][t, :] = s_a X[t] A_a^T over a share of K. A workgroup takes 32 RF rows of a run
 // and 32 RT ranks (blockIdx.z the block of ranks); K goes in blocks of 32 to its four
-// waves and to blockIdx.y's workgroups in turn. A lane reads 16 neighbouring values of
+// waves and to blockIdx.y's workgroups in turn (down_sums: a wave's sums). A lane reads 16 neighbouring values of
 // a row, the first eight for one MFMA step and the others for the next: whole lines,
 // and the sum does not mind the order.
 // ---------------------------------------------------------------------------
 template <class TX, class TW, int RT, int RF, bool VEC>
-__global__ __launch_bounds__(kLoraThreads) void k_lora_down(Lora P) {
-    __shared__ float part[kLoraWaves][RF * 32][33];
+__device__ __forceinline__ void down_sums(const Lora& P, const dev::SpanTile& t, int adapter, int rank, int j0, int part, int parts,
+                                          f32x16 (&acc)[RF][RT]) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, fr = lane & 31, fh = lane >> 5;
-    dev::SpanTile t;
-    if (!dev::find_tile(P.runs, P.count, P.M, 1, RF * 32, blockIdx.x, t)) return;
-    int rank;
-    const int adapter = adapter_of(P, t, rank), j0 = blockIdx.z * RT * 32;
-    if (j0 >= rank) return;  // up reads none of them
     const TX* x[RF];
     const TW* a[RT];
 #pragma unroll
     for (int i = 0; i < RF; ++i) x[i] = (const TX*)P.x + (t.first + min(t.row0 + i * 32 + fr, t.rows - 1)) * P.ldx;
 #pragma unroll
     for (int i = 0; i < RT; ++i) a[i] = (const TW*)P.a + ((int64_t)adapter * P.rank + min(j0 + i * 32 + fr, rank - 1)) * P.K;
-    f32x16 acc[RF][RT];
 #pragma unroll
     for (int i = 0; i < RF; ++i)
 #pragma unroll
@@ -161,7 +155,7 @@ __global__ __launch_bounds__(kLoraThreads) void k_lora_down(Lora P) {
     constexpr int DEPTH = sizeof(TX) == 2 ? 2 : 1, U = 2 * DEPTH;
     Eight<TX> xn[U][RF];
     Eight<TW> an[U][RT];
-    const int step = 32 * kLoraWaves * P.splits;
+    const int step = 32 * kLoraWaves * parts;
     auto load = [&](int k0) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -172,7 +166,7 @@ __global__ __launch_bounds__(kLoraThreads) void k_lora_down(Lora P) {
             for (int i = 0; i < RT; ++i) an[u][i].template load<VEC>(a[i], k + fh * 16 + u % 2 * 8, P.K);
         }
     };
-    int k = (blockIdx.y * kLoraWaves + w) * 32;
+    int k = (part * kLoraWaves + w) * 32;
     if (k < P.K) load(k);
     for (; k < P.K; k += DEPTH * step) {
         Eight<TX> xc[U][RF];
@@ -199,6 +193,19 @@ __global__ __launch_bounds__(kLoraThreads) void k_lora_down(Lora P) {
             }
         }
     }
+}
+
+template <class TX, class TW, int RT, int RF, bool VEC>
+__global__ __launch_bounds__(kLoraThreads) void k_lora_down(Lora P) {
+    __shared__ float part[kLoraWaves][RF * 32][33];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, fr = lane & 31, fh = lane >> 5;
+    dev::SpanTile t;
+    if (!dev::find_tile(P.runs, P.count, P.M, 1, RF * 32, blockIdx.x, t)) return;
+    int rank;
+    const int adapter = adapter_of(P, t, rank), j0 = blockIdx.z * RT * 32;
+    if (j0 >= rank) return;  // up reads none of them
+    f32x16 acc[RF][RT];
+    down_sums<TX, TW, RT, RF, VEC>(P, t, adapter, rank, j0, blockIdx.y, P.splits, acc);
     const float f = P.scale ? P.scale[adapter] : 1.0f;
     float* h = P.h + ((int64_t)blockIdx.y * P.M + t.first + t.row0) * P.hrank;
     const int left = t.rows - t.row0;
@@ -256,19 +263,10 @@ __device__ __forceinline__ void parts_of_h(const Lora& P, int64_t row, int j0, i
 // workgroup have neighbouring rows and the same columns (their B comes from the L1), or,
 // with FEW, the same rows and neighbouring columns.
 // ---------------------------------------------------------------------------
-template <class TW, int KS, bool FEW, bool VEC, bool CV>
-__global__ __launch_bounds__(kLoraThreads, KS <= 4 ? 2 : 1) void k_lora_up(Lora P, int j0, int columns) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, fr = lane & 31, fh = lane >> 5;
-    dev::SpanTile t;
-    if (!dev::find_tile(P.runs, P.count, P.M, 1, FEW ? 32 : 32 * kLoraWaves, blockIdx.x, t)) return;
-    int rank;
-    const int adapter = adapter_of(P, t, rank);
-    const int row0 = t.row0 + (FEW ? 0 : w * 32), left = t.rows - row0;
-    int n = (FEW ? blockIdx.y * kLoraWaves + w : blockIdx.y) * columns;
-    const int n1 = min(n + columns, P.N);
-    if (left <= 0 || n >= n1 || (P.accumulate && j0 >= rank)) return;
-    const int64_t first = t.first + row0;
-    float* c = P.c + first * P.ldc;
+// The columns n .. n1 of a wave's rows, `left` of them, from c on; hp null without an adapter: zeros.
+template <class TW, int KS, bool VEC, bool CV>
+__device__ __forceinline__ void up_columns(const Lora& P, int adapter, int rank, int j0, const bf16x8 (*hp)[3], int n, int n1, float* c, int left) {
+    const int lane = threadIdx.x & 63, fr = lane & 31, fh = lane >> 5;
     auto row_of = [&](int e) { return (e >> 2) * 8 + fh * 4 + (e & 3); };
     auto put = [&](int e, int col, const f4& v) __attribute__((always_inline)) {
         float* to = c + row_of(e) * P.ldc + col;
@@ -281,14 +279,12 @@ __global__ __launch_bounds__(kLoraThreads, KS <= 4 ? 2 : 1) void k_lora_up(Lora 
                 if (col + j < P.N) to[j] = v[j];
         }
     };
-    if (adapter < 0) {  // only without accumulate; B may not be there at all
+    if (!hp) {
         for (; n < n1; n += 128)
 #pragma unroll
             for (int e = 0; e < 16; ++e) put(e, n + fr * 4, f4{0.f, 0.f, 0.f, 0.f});
         return;
     }
-    bf16x8 hp[KS][3];
-    parts_of_h<KS>(P, first + min(fr, left - 1), j0, rank, fh, hp);
     const TW* b = (const TW*)P.b + (int64_t)adapter * P.N * P.rank;
     for (; n < n1; n += 128) {
         const int col = n + fr * 4;
@@ -329,6 +325,73 @@ __global__ __launch_bounds__(kLoraThreads, KS <= 4 ? 2 : 1) void k_lora_up(Lora 
 #pragma unroll
         for (int e = 0; e < 16; ++e) put(e, col, y[e] + f4{acc[0][e], acc[1][e], acc[2][e], acc[3][e]});
     }
+}
+
+template <class TW, int KS, bool FEW, bool VEC, bool CV>
+__global__ __launch_bounds__(kLoraThreads, KS <= 4 ? 2 : 1) void k_lora_up(Lora P, int j0, int columns) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, fr = lane & 31, fh = lane >> 5;
+    dev::SpanTile t;
+    if (!dev::find_tile(P.runs, P.count, P.M, 1, FEW ? 32 : 32 * kLoraWaves, blockIdx.x, t)) return;
+    int rank;
+    const int adapter = adapter_of(P, t, rank);
+    const int row0 = t.row0 + (FEW ? 0 : w * 32), left = t.rows - row0;
+    const int n = (FEW ? blockIdx.y * kLoraWaves + w : blockIdx.y) * columns, n1 = min(n + columns, P.N);
+    if (left <= 0 || n >= n1 || (P.accumulate && j0 >= rank)) return;
+    const int64_t first = t.first + row0;
+    float* c = P.c + first * P.ldc;
+    if (adapter < 0) {  // only without accumulate; B may not be there at all
+        up_columns<TW, KS, VEC, CV>(P, adapter, rank, j0, nullptr, n, n1, c, left);
+        return;
+    }
+    bf16x8 hp[KS][3];
+    parts_of_h<KS>(P, first + min(fr, left - 1), j0, rank, fh, hp);
+    up_columns<TW, KS, VEC, CV>(P, adapter, rank, j0, hp, n, n1, c, left);
+}
+
+// Both in one launch, for few rows a run and a short K: every workgroup of a run forms H for
+// itself, in LDS. A is then read once for each of them (from the L2), which costs less than
+// the second launch's beginning as long as K is short (the rule stands at the launch).
+template <class TX, class TW, int KS, bool XVEC, bool VEC, bool CV>
+__global__ __launch_bounds__(kLoraThreads, 2) void k_lora_small(Lora P, int columns) {
+    constexpr int RT = (KS + 1) / 2;
+    __shared__ float part[kLoraWaves][32][33];
+    __shared__ __attribute__((aligned(16))) float h[32][RT * 32 + 4];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, fr = lane & 31, fh = lane >> 5;
+    dev::SpanTile t;
+    if (!dev::find_tile(P.runs, P.count, P.M, 1, 32, blockIdx.x, t)) return;
+    int rank;
+    const int adapter = adapter_of(P, t, rank), left = t.rows - t.row0;
+    const int n = (blockIdx.y * kLoraWaves + w) * columns, n1 = min(n + columns, P.N);
+    if (P.accumulate && !rank) return;
+    float* c = P.c + (int64_t)(t.first + t.row0) * P.ldc;
+    if (adapter < 0) {
+        up_columns<TW, KS, VEC, CV>(P, adapter, rank, 0, nullptr, n, n1, c, left);
+        return;
+    }
+    f32x16 acc[1][RT];
+    down_sums<TX, TW, RT, 1, XVEC>(P, t, adapter, rank, 0, 0, 1, acc);
+    const float f = P.scale ? P.scale[adapter] : 1.0f;
+#pragma unroll
+    for (int j = 0; j < RT; ++j) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) part[w][(e >> 2) * 8 + fh * 4 + (e & 3)][fr] = acc[0][j][e];
+        __syncthreads();
+        for (int i = threadIdx.x; i < 1024; i += kLoraThreads) {
+            const int row = i >> 5, col = i & 31;
+            const float v = (part[0][row][col] + part[1][row][col]) + (part[2][row][col] + part[3][row][col]);
+            h[row][j * 32 + col] = j * 32 + col < rank ? v * f : 0.f;
+        }
+        __syncthreads();
+    }
+    bf16x8 hp[KS][3];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        Eight<float> v;
+        v.a = *(const f4*)&h[fr][ks * 16 + fh * 8];
+        v.b = *(const f4*)&h[fr][ks * 16 + fh * 8 + 4];
+        v.parts(hp[ks]);
+    }
+    up_columns<TW, KS, VEC, CV>(P, adapter, rank, 0, hp, n, n1, c, left);
 }
 
 // The same for runs of many rows: the waves of a workgroup have neighbouring rows and share
@@ -451,6 +514,34 @@ void launch_lora(Lora P, int64_t M, bool vec) {
     const bool few = M <= 32 * (int64_t)P.count;
     const int rt = P.rank <= 32 ? 1 : P.rank <= 64 ? 2 : 4, rf = few || rt > 2 || !vec ? 1 : 2;
     const int64_t down = M / (32 * rf) + std::min<int64_t>(P.count, M);
+    const int64_t tiles = M / (few ? 32 : 128) + std::min<int64_t>(P.count, M);
+    const bool bvec = P.rank % 8 == 0 && aligned16(P.b), cvec = P.N % 4 == 0 && P.ldc % 4 == 0 && aligned16(P.c);
+    // Columns of a workgroup's wave: as many as leave four workgroups a CU (with few rows, soon
+    // done, six), since each begins with H and its parts. Measured, us, for two / four a CU:
+    // [8192,640] -> 5120 rank 12 87 / 79, [12528,3840] -> 10240 rank 64 168 / 167.
+    int64_t columns = 4096;
+    while (columns > 128 && tiles * ((P.N + columns * (few ? kLoraWaves : 1) - 1) / (columns * (few ? kLoraWaves : 1))) < (few ? 6 : 4) * (int64_t)cus)
+        columns /= 2;
+    // One launch or two, for few rows a run. Measured, us, one / two, 48 single rows to 4096 columns:
+    // K 320 rank 8 7.3 / 9.3, rank 64 13.4 / 15.8; K 640 rank 8 8.7 / 9.4, rank 64 16.0 / 16.2, rank
+    // 128 67 / 51; K 1280 rank 8 12.0 / 9.6.
+    if (few && P.rank > 0 && P.rank <= 64 && P.K <= 640) {
+        const dim3 grid((unsigned)tiles, (unsigned)((P.N + columns * kLoraWaves - 1) / (columns * kLoraWaves)));
+        auto go = [&](auto k, auto x, auto v) {
+            constexpr int KS = decltype(k)::value;
+            constexpr bool X = decltype(x)::value, V = decltype(v)::value;
+            if (cvec) k_lora_small<TX, TW, KS, X, V, true><<<grid, kLoraThreads, 0, stream()>>>(P, (int)columns);
+            else k_lora_small<TX, TW, KS, X, V, false><<<grid, kLoraThreads, 0, stream()>>>(P, (int)columns);
+        };
+        auto with = [&](auto x, auto v) {
+            if (P.rank <= 16) go(integral_constant<int, 1>(), x, v);
+            else if (P.rank <= 32) go(integral_constant<int, 2>(), x, v);
+            else go(integral_constant<int, 4>(), x, v);
+        };
+        if (vec && bvec) with(T_(), T_());
+        else with(F_(), F_());
+        return;
+    }
     if (P.rank > 0) {
         // Parts of K until the chip has four workgroups a CU, while each wave keeps two blocks, and at
         // most four, which up has to sum: [2480,2560] -> 4096 takes 42 us with two, 38 with four, 44 with eight.
@@ -471,14 +562,6 @@ void launch_lora(Lora P, int64_t M, bool vec) {
         else if (rt == 2) vec ? (rf == 2 ? go(Two(), Two(), T_()) : go(Two(), One(), T_())) : go(Two(), One(), F_());
         else vec ? go(Four(), One(), T_()) : go(Four(), One(), F_());
     }
-    const int64_t tiles = M / (few ? 32 : 128) + std::min<int64_t>(P.count, M);
-    // Columns of a workgroup's wave: as many as leave four workgroups a CU (with few rows, soon
-    // done, six), since each begins with H and its parts. Measured, us, for two / four a CU:
-    // [8192,640] -> 5120 rank 12 87 / 79, [12528,3840] -> 10240 rank 64 168 / 167.
-    int64_t columns = 4096;
-    while (columns > 128 && tiles * ((P.N + columns * (few ? kLoraWaves : 1) - 1) / (columns * (few ? kLoraWaves : 1))) < (few ? 6 : 4) * (int64_t)cus)
-        columns /= 2;
-    const bool bvec = P.rank % 8 == 0 && aligned16(P.b), cvec = P.N % 4 == 0 && P.ldc % 4 == 0 && aligned16(P.c);
     for (int j0 = 0; j0 == 0 || j0 < P.rank; j0 += 128) {
         const int ks = std::min(P.rank - j0, 128);
         const dim3 grid((unsigned)tiles, (unsigned)((P.N + columns * (few ? kLoraWaves : 1) - 1) / (columns * (few ? kLoraWaves : 1))));
@@ -516,6 +599,9 @@ void run_lora(const char* op, int64_t M, int64_t N, int64_t K, const TX* X, int6
     need(ldx >= K && ldc >= N, op, "leading dimension smaller than the row");
     need(M < kMost && N < kMost && K < kMost && adapters < kMost && count < kMost, op, "a size of 2^30 or more");
     need(rank <= 1024, op, "rank above 1024");
+    need(std::max(ldx, ldc) <= (int64_t(1) << 46) / std::max<int64_t>(M, 1) &&
+             adapters * std::max<int64_t>(rank, 1) <= (int64_t(1) << 46) / std::max<int64_t>({N, K, 1}),
+         op, "matrix too large");
     if (M == 0 || N == 0 || count == 0) return;
     ensure_init();
     check_range(segments, (size_t)count * 16, op, "segments");

@@ -98,6 +98,17 @@ def test_few_rows(be, orc, types, rows):
 
 @gpu
 @pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("N,K,rank", [(1024, 64, 24), (515, 600, 40), (640, 640, 64), (130, 33, 5), (5, 640, 65), (260, 648, 64)])
+def test_few_rows_of_a_short_k(be, orc, types, N, K, rank):
+    """Both sides of the one-launch route: ranks to 64, K to 640; runs of 0 to 70 rows among them."""
+    for rows in ([1, 0, 70, 1, 3, 1, 1, 5], [33]):
+        c = Case(orc, sum(rows), N, K, rank, 3, types, seed=250 + K)
+        for acc in (True, False):
+            c.check(be, orc, ragged(rows, 3, rank), acc, what=f"{types} {rows} {N}x{K} rank {rank} acc={acc}")
+
+
+@gpu
+@pytest.mark.parametrize("types", TYPES)
 @pytest.mark.parametrize("pad", [1, 4, 8])
 def test_strides(be, orc, types, pad):
     for rows in ([40, 90, 3], [1, 1]):
