@@ -149,9 +149,9 @@ int sdh_linear_swiglu(const float* x, const uint16_t* w1, const uint16_t* w3, fl
  * the projection accumulating). X [M, K] and C [M, N] fp32, leading dimensions in
  * elements; A [adapters, rank, K] and B [adapters, N, rank] bf16, dense; scale
  * [adapters] or NULL for ones; rank at most 1024. segments [count, 4] int32 on
- * the device, 16-byte aligned: a run's first row, its rows, its adapter, and how
- * many of the adapter's ranks count (rows of A_a and columns of B_a from there on
- * are not read as numbers). A run with no such adapter (-1) or rank 0 adds
+ * the device, 16-byte aligned, count at most 65536: a run's first row, its rows,
+ * its adapter, and how many of the adapter's ranks count (rows of A_a and columns
+ * of B_a from there on are not read as numbers). A run with no such adapter (-1) or rank 0 adds
  * nothing: its rows are left, or zero without accumulate. Runs must not share
  * rows; entries past the matrix are cut to it; rows of no run are left as they
  * were. Everything is held in fp32, X unrounded. C must not overlap an input. */
@@ -298,10 +298,10 @@ int sdh_attention_fp16(const float* q, const float* k, const float* v, void* out
 
 /* No counterpart in the reference: attention over sequences packed into one
  * tensor, every sequence's queries to its own keys. q and out [Tq, heads*d], k
- * and v [Tk, kv_heads*d], heads as sdh_attention's, out float32 or (out_bf16)
- * its bf16 bits. spans [seqs, 4] int32 on the device, 16-byte aligned: a
- * sequence's first query row, its lq query rows, its first key row, its lk key
- * rows. Rows may lie anywhere (packed, padded, keys in slots of a cache; several
+ * and v [Tk, kv_heads*d], heads as sdh_attention's, d at most 1024, out float32 or
+ * (out_bf16) its bf16 bits. spans [seqs, 4] int32 on the device, 16-byte aligned,
+ * seqs at most 65536: a sequence's first query row, its lq query rows, its first
+ * key row, its lk key rows. Rows may lie anywhere (packed, padded, keys in slots of a cache; several
  * sequences may read the same keys), but no query row may belong to two
  * sequences; entries past the tensors are cut to them. out rows of no sequence
  * are left as they were.
@@ -313,7 +313,9 @@ int sdh_attention_fp16(const float* q, const float* k, const float* v, void* out
  * (-inf hides a key). A query that sees no key gives zeros. Keys that a query
  * does not see do not change its result, whatever their values are.
  *   out must not overlap an input. The arrays are read when the work runs, so a
- * captured graph takes the spans that they hold at each replay. */
+ * captured graph takes the spans that they hold at each replay. Where no scratch
+ * can be had (a full arena; a capture that asks for more than any call before it)
+ * a slower kernel gives the same result. */
 int sdh_attention_packed(const float* q, const float* k, const float* v, void* out, int out_bf16, int64_t Tq,
                          int64_t Tk, int heads, int kv_heads, int64_t d, const int32_t* spans, int64_t seqs,
                          float scale, int causal, int64_t window, const int32_t* prefix, float cap,

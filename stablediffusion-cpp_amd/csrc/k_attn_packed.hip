@@ -449,10 +449,9 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
     if (EXTRA && table)  // [group, 2 radius + 1]
         for (int i = threadIdx.x; i < table; i += kThreads) biases[i] = P.bias[(int64_t)kh * table + i];
 
-    // Q: the B operand of S^T, row qi of head h, dims ds*16 + fh*8 .. +7. Read by its rows a
-    // fragment costs an access a lane (9200 cycles for the 256 rows of a workgroup at d = 128);
-    // whole rows come in 64 dims at a time and are dealt out through a share of the LDS that no
-    // tile is in yet, the 16-byte piece c of row i at c ^ (i & 15).
+    // Q: the B operand of S^T, row qi of head h, dims ds*16 + fh*8 .. +7. Whole rows
+    // come in 64 dims at a time and are dealt out through a share of the LDS that no tile is in
+    // yet, the 16-byte piece c of row i at c ^ (i & 15).
     const float* qp = P.q + (int64_t)(T.first + qi) * inner + (int64_t)h * d;
     float qx[DS][8];
     if constexpr (VEC) {
@@ -585,31 +584,34 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
                     if (visible(k0 + u * 16 + fh * 8 + i)) emax = max(emax, exps[kKT + u * 16 + fh * 8 + i]);
             emax = max(emax, __shfl_xor(emax, 32, 64));
         }
+        float unit = ct;  // of x
         if constexpr (EXTRA) {
             const int mid = (h - kh * group) * (2 * P.radius + 1) + P.radius;
-            const float in = P.cap > 0.f ? ct / P.cap : ct;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] *= in;
             if (P.cap > 0.f) {
+                const float in = fminf(ct / P.cap, 3.40282347e38f);
                 float top = 0.f;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(x[i]));
+                for (int i = 0; i < 32; ++i) {
+                    x[i] *= in;
+                    top = fmaxf(top, fabsf(x[i]));
+                }
+                unit = P.cap;
                 // Scores well inside the cap, as most are, take the polynomial alone (half the
                 // instructions, no exponential).
                 const bool small = !__ballot(!(top < kTanhNear));
                 if (small) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                            x[i] = P.cap * tanh_small(x[i]);
-                            few(i);
-                        }
+                        x[i] = tanh_small(x[i]);
+                        few(i);
+                    }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                            asm volatile("" : "+v"(x[i]));  // the polynomials are not to be formed in front of the branch
-                            x[i] = P.cap * tanh_near(x[i]);
-                            few(i);
-                        }
+                        asm volatile("" : "+v"(x[i]));  // the polynomials are not to be formed in front of the branch
+                        x[i] = tanh_near(x[i]);
+                        few(i);
+                    }
                 }
             }
             if (P.bias) {
@@ -617,16 +619,17 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
                 const int at = k0 + fh * 8 - p;
                 const float* bp = P.bias + (int64_t)kh * group * (2 * P.radius + 1);
                 if (to <= -P.radius || from >= P.radius) {  // one value for all
-                    const float v = table ? biases[mid + (from >= P.radius ? P.radius : -P.radius)] : bp[mid + (from >= P.radius ? P.radius : -P.radius)];
+                    const int c = mid + (from >= P.radius ? P.radius : -P.radius);
+                    const float v = table ? biases[c] : bp[c];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) x[i] += v;
+                    for (int i = 0; i < 32; ++i) x[i] = fmaf(x[i], unit, v);
                 } else if (table && from >= -P.radius && to <= P.radius) {  // none clamped
                     const float* b = biases + mid + at;
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            x[u * 8 + i] += b[u * 16 + i];
+                            x[u * 8 + i] = fmaf(x[u * 8 + i], unit, b[u * 16 + i]);
                             few(i);
                         }
                 } else {
@@ -635,10 +638,11 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             const int c = mid + min(max(at + u * 16 + i, -P.radius), P.radius);
-                            x[u * 8 + i] += table ? biases[c] : bp[c];
+                            x[u * 8 + i] = fmaf(x[u * 8 + i], unit, table ? biases[c] : bp[c]);
                             few(i);
                         }
                 }
+                unit = 1.0f;
             }
         }
         if (edge && (k0 >= pre || !pre)) {
@@ -663,7 +667,7 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
         float mt = x[0];
 #pragma unroll
         for (int i = 0; i < 32; ++i) mt = fmaxf(mt, x[i]);
-        if constexpr (!EXTRA) mt *= ct;
+        mt *= unit;
         mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
         const float mnew = mt > m + (EXTRA ? kLazy / kLog2e : kLazy) ? mt : m;
         float alpha = 1.0f;
@@ -682,9 +686,9 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
         // which would overflow.
         if (EXTRA && __ballot(!(fabsf(ref) < 1e4f))) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i] - ref, kLog2e, (float)by));
+            for (int i = 0; i < 32; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(fmaf(x[i], unit, -ref), kLog2e, (float)by));
         } else {
-            const float f = EXTRA ? kLog2e : ct, up = (float)by - (EXTRA ? ref * kLog2e : ref);
+            const float f = EXTRA ? unit * kLog2e : unit, up = (float)by - (EXTRA ? ref * kLog2e : ref);
 #pragma unroll
             for (int i = 0; i < 32; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], f, up));
         }
@@ -1114,9 +1118,11 @@ void run_attention_packed(const float* q, const float* k, const float* v, void* 
     need(Tq >= 0 && Tk >= 0 && seqs >= 0 && window >= 0 && radius >= 0, op, "negative size");
     need(heads > 0 && d > 0, op, "heads and d must be positive");
     need(heads % kv_heads == 0, op, "heads mismatch");
+    need(seqs <= dev::kMaxSpans, op, "more than 65536 sequences");
     need(d <= kMaxD, op, "head dimension above 1024");
     need(heads <= 65535, op, "too many heads for one launch");
-    need(Tq < kMost && Tk < kMost && seqs < kMost && radius < kMost, op, "a size of 2^30 or more");
+    need(Tq < kMost && Tk < kMost && radius < kMost, op, "a size of 2^30 or more");
+    need(!bias || (int64_t)heads * (2 * radius + 1) < 2 * kMost, op, "a bias of 2^31 values or more");
     need(std::isfinite(scale) && std::isfinite(cap) && cap >= 0.f, op, "scale and cap must be finite, cap not negative");
     if (Tq == 0 || seqs == 0) return;
     ensure_init();

@@ -599,6 +599,7 @@ void run_lora(const char* op, int64_t M, int64_t N, int64_t K, const TX* X, int6
     need(ldx >= K && ldc >= N, op, "leading dimension smaller than the row");
     need(M < kMost && N < kMost && K < kMost && adapters < kMost && count < kMost, op, "a size of 2^30 or more");
     need(rank <= 1024, op, "rank above 1024");
+    need(count <= dev::kMaxSpans, op, "more than 65536 segments");
     need(std::max(ldx, ldc) <= (int64_t(1) << 46) / std::max<int64_t>(M, 1) &&
              adapters * std::max<int64_t>(rank, 1) <= (int64_t(1) << 46) / std::max<int64_t>({N, K, 1}),
          op, "matrix too large");

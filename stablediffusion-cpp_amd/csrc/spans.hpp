@@ -8,6 +8,9 @@
 namespace sdh {
 namespace dev {
 
+// Every workgroup walks the list, 64 entries at a time, which is why it has a limit.
+constexpr int64_t kMaxSpans = 65536;
+
 // [first, first + rows) cut to [0, total).
 __device__ __forceinline__ void cut_span(int& first, int& rows, int total) {
     first = min(max(first, 0), total);
@@ -50,7 +53,9 @@ struct SpanTile {
     int row0;         // the tile's first row within it, in rows times `mult`
 };
 // Entries have ceil(rows * mult / tile_rows) tiles each, numbered through; false past
-// the last one. Every lane of a wave gets the answer. rows * mult < 2^30 for all.
+// the last one. Every lane of a wave gets the answer. rows * mult < 2^30 for all; no entry has more
+// tiles than the grid has items, below 2^25, so that the sums, of 64 entries behind `before` <= item,
+// stay inside 31 bits.
 __device__ __forceinline__ bool find_tile(const int4* __restrict__ list, int n, int total, int mult, int tile_rows, int item,
                                           SpanTile& t) {
     const int lane = threadIdx.x & 63;

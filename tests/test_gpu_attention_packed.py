@@ -372,7 +372,8 @@ def _args(**kw):
 @pytest.mark.parametrize("kw", [{"Tq": -1}, {"Tk": -1}, {"seqs": -1}, {"window": -1}, {"radius": -1}, {"heads": 0}, {"d": 0},
                                 {"d": 1025}, {"heads": 3, "kv": 2}, {"heads": 70000, "kv": 70000}, {"Tk": 1 << 30},
                                 {"Tq": 1 << 40}, {"seqs": 1 << 30}, {"radius": 1 << 30}, {"scale": float("nan")},
-                                {"cap": -1.0}, {"cap": float("inf")}], ids=str)
+                                {"cap": -1.0}, {"cap": float("inf")}, {"seqs": 65537},
+                                {"heads": 4, "kv": 1, "bias": 4096, "radius": 1 << 28}], ids=str)
 def test_refusals_of_sizes(kw):
     """Sizes and numbers are refused before anything else is looked at, with or without a device."""
     lib = sdhip.load_library()

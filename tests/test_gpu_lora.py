@@ -283,7 +283,8 @@ def _args(**kw):
 @pytest.mark.parametrize("name", ["sdh_lora_nt_bf16", "sdh_lora_nt_bf16_packed", "sdh_lora_nt_f32"])
 @pytest.mark.parametrize("kw", [{"M": -1}, {"N": -1}, {"K": -1}, {"rank": -1}, {"adapters": -1}, {"n": -1}, {"ldx": 7}, {"ldc": 7},
                                 {"rank": 1025}, {"M": 1 << 30}, {"N": 1 << 30, "ldc": 1 << 30}, {"n": 1 << 31},
-                                {"adapters": 1 << 30}, {"K": 1 << 30, "ldx": 1 << 30}], ids=str)
+                                {"adapters": 1 << 30}, {"K": 1 << 30, "ldx": 1 << 30}, {"n": 65537}, {"ldx": 1 << 45},
+                                {"ldc": 1 << 45}, {"adapters": 1 << 29, "N": 1 << 29, "ldc": 1 << 29}], ids=str)
 def test_refusals_of_sizes(name, kw):
     lib = sdhip.load_library()
     assert getattr(lib, name)(*_args(**kw)) == sdhip.SDH_ERR_INVALID
