@@ -60,6 +60,27 @@ inline void gemm_nt_bf16(int64_t M, int64_t N, int64_t K, const float* A, int64_
     detail::check(sdh_gemm_nt_bf16(M, N, K, A, lda, B, ldb, C, ldc, bias, accumulate ? 1 : 0), "hip::gemm_nt_bf16");
 }
 
+// Additive: each run of rows' low-rank adapter beside a projection of X, segments [count, 4] on the device; X fp32
+// or (packed) bf16 bits, the adapters bf16 or (f32) fp32
+inline void lora_nt_bf16(int64_t M, int64_t N, int64_t K, const float* X, int64_t ldx, const uint16_t* A,
+                         const uint16_t* B, int64_t rank, int64_t adapters, const float* scale, const int32_t* segments,
+                         int64_t count, float* C, int64_t ldc, bool accumulate) {
+    detail::check(sdh_lora_nt_bf16(M, N, K, X, ldx, A, B, rank, adapters, scale, segments, count, C, ldc, accumulate ? 1 : 0),
+                  "hip::lora_nt_bf16");
+}
+inline void lora_nt_bf16_packed(int64_t M, int64_t N, int64_t K, const uint16_t* X, int64_t ldx, const uint16_t* A,
+                                const uint16_t* B, int64_t rank, int64_t adapters, const float* scale,
+                                const int32_t* segments, int64_t count, float* C, int64_t ldc, bool accumulate) {
+    detail::check(sdh_lora_nt_bf16_packed(M, N, K, X, ldx, A, B, rank, adapters, scale, segments, count, C, ldc, accumulate ? 1 : 0),
+                  "hip::lora_nt_bf16_packed");
+}
+inline void lora_nt_f32(int64_t M, int64_t N, int64_t K, const float* X, int64_t ldx, const float* A, const float* B,
+                        int64_t rank, int64_t adapters, const float* scale, const int32_t* segments, int64_t count,
+                        float* C, int64_t ldc, bool accumulate) {
+    detail::check(sdh_lora_nt_f32(M, N, K, X, ldx, A, B, rank, adapters, scale, segments, count, C, ldc, accumulate ? 1 : 0),
+                  "hip::lora_nt_f32");
+}
+
 // backend_cuda.h:48-52
 inline void group_norm(const float* x, float* y, int64_t N, int64_t C, int64_t HW, int groups, const float* gamma,
                        const float* beta, float eps) {
@@ -103,6 +124,15 @@ inline void attention_fp16(const float* q, const float* k, const float* v, void*
                            int64_t Sq, int64_t Skv, int heads, int kv_heads, int64_t d, bool causal) {
     detail::check(sdh_attention_fp16(q, k, v, out, out_bf16 ? 1 : 0, N, Sq, Skv, heads, kv_heads, d, causal ? 1 : 0),
                   "hip::attention_fp16");
+}
+// Additive: attention over sequences packed into one tensor, spans [seqs, 4] on the device; out fp32 or bf16 bits
+inline void attention_packed(const float* q, const float* k, const float* v, void* out, bool out_bf16, int64_t Tq,
+                             int64_t Tk, int heads, int kv_heads, int64_t d, const int32_t* spans, int64_t seqs,
+                             float scale, bool causal, int64_t window = 0, const int32_t* prefix = nullptr,
+                             float cap = 0.0f, const float* bias = nullptr, int64_t radius = 0) {
+    detail::check(sdh_attention_packed(q, k, v, out, out_bf16 ? 1 : 0, Tq, Tk, heads, kv_heads, d, spans, seqs, scale,
+                                       causal ? 1 : 0, window, prefix, cap, bias, radius),
+                  "hip::attention_packed");
 }
 // fused: qknorm_rope of q and k, then attention; q updated in place, k and v read only
 inline void qknorm_rope_attention(float* q, const float* k, const float* v, void* out, bool out_bf16, int64_t N,
