@@ -50,14 +50,13 @@ __device__ __forceinline__ Seen seen_from(const Packed& P, int p, int lk, int pr
     return Seen{pre, lo, max(hi, lo)};
 }
 
-// tanh to about 3e-7 of itself. Near zero 1 - e would cancel: a polynomial (its next
-// term is below 2e-8 of the sum at kTanhNear).
-constexpr float kTanhNear = 0.35f;
-__device__ __forceinline__ float tanh_small(float x) {
+// tanh to about 3e-7 of itself. Near zero 1 - e would cancel: x + x^3 p(x^2), p the polynomial
+// of degree two whose largest error on [0, kTanhNear^2] is least (4e-8 of tanh x, found by weighted
+// least squares; the Taylor series needs two terms more). `last`: a loop may hold it in a register.
+constexpr float kTanhNear = 0.35f, kTanhLast = -0.0491593033f;
+__device__ __forceinline__ float tanh_small(float x, float last = kTanhLast) {
     const float x2 = x * x;
-    const float p = fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, -1382.0f / 155925.0f, 62.0f / 2835.0f), -17.0f / 315.0f), 2.0f / 15.0f),
-                         -1.0f / 3.0f);
-    return fmaf(x * x2, p, x);
+    return fmaf(x * x2, fmaf(x2, fmaf(x2, last, 0.133000106f), -0.333326697f), x);
 }
 __device__ __forceinline__ float tanh_near(float x) {
     const float a = fabsf(x);
@@ -186,6 +185,10 @@ constexpr int kKT = 64, kSplitWaves = 4;
 // The reference m of the weights is raised when a tile's largest score passes it by more
 // than this (in units of log2): weights stay below 2^(14 + kLazy), inside fp16.
 constexpr float kLazy = 1.5f;
+// The bias of a head in LDS goes on at both ends with its end values, as far as a wave's 32 rows and a
+// tile's 64 keys reach past the radius unless all of them are beyond it: no index is held to the radius
+// (ten instructions a score; the rows and tiles at the band's edges took half the softmax' time).
+constexpr int kBiasPad = 96;
 constexpr int kUnsetE = -1000;  // no values seen yet
 constexpr int kSpread = 8;
 constexpr int kFarE = -40;      // weights' exponents relative to E are not taken below this (2^-40 of the largest sum)
@@ -250,6 +253,7 @@ template <int DP, bool VEC>
 __global__ __launch_bounds__(64 * kSplitWaves) void k_attn_packed_split(Packed P, Tiles X) {
     constexpr int PART = kKT * DP, KCH = DP / 8, KROWS = 64 / KCH, KU = 16 / KROWS;  // 16-byte chunks of a K row, rows of a wave's load, loads
     constexpr int VU = DP / 64;                                                     // columns of v a lane has
+    __shared__ __attribute__((aligned(16))) u16 vt[2 * PART];
     __shared__ int tops[2][kSplitWaves], flags[kSplitWaves];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tile = blockIdx.x, kh = blockIdx.y, j0 = tile * kKT + w * 16, d = P.d;
@@ -378,9 +382,15 @@ __global__ __launch_bounds__(64 * kSplitWaves) void k_attn_packed_split(Packed P
                 lo[i] = c[0], lo[i + 1] = c[1];
             }
             const int row = lane * VU + u, to = row * kKT + (((w * 2 + b) ^ swz_v(row)) << 3);
-            *(h8*)(vd + to) = hi;
-            *(h8*)(vd + PART + to) = lo;
+            *(h8*)(vt + to) = hi;
+            *(h8*)(vt + PART + to) = lo;
         }
+    __syncthreads();  // whole lines of V^T, of which a wave has a quarter
+#pragma unroll
+    for (int i = 0; i < 2 * PART / (8 * 64 * kSplitWaves); ++i) {
+        const int to = (i * 64 * kSplitWaves + threadIdx.x) * 8;
+        *(h8*)(vd + to) = *(const h8*)(vt + to);
+    }
 }
 
 // Eight waves a workgroup, one workgroup a CU; for DP = 64, whose tiles are half the size and
@@ -409,6 +419,10 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
     dev::SpanTile T;
     if (!dev::find_tile(P.spans, P.seqs, P.Tq, group, kTileRows, lb - kh * items, T)) return;
     dev::cut_span(T.z, T.w, P.Tk);
+    // A sequence's last rows, which see most keys, come first: the short ones fill the end. Measured, us,
+    // first / last rows first, 32/8 heads of 128, causal: one sequence of 2048 to 4096 231 / 198, four of
+    // 500 to 1000 125 / 118, eight of 250 to 500 77 / 79.
+    if (P.causal) T.row0 = (T.rows * group - 1) / kTileRows * kTileRows - T.row0;
     const int d = P.d, rows = T.rows * group, lk = T.w, pre = P.prefix ? min(max(P.prefix[T.index], 0), lk) : 0;
     const int64_t inner = (int64_t)P.heads * d, kv_inner = (int64_t)P.kv_heads * d;
     const int r = T.row0 + w * 32 + fr;
@@ -446,8 +460,12 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
         copy(tile_of(n0), 0, kbuf0);
         copy(tile_of(n0), 1, vbuf0);
     }
-    if (EXTRA && table)  // [group, 2 radius + 1]
-        for (int i = threadIdx.x; i < table; i += kThreads) biases[i] = P.bias[(int64_t)kh * table + i];
+    const int row_of_bias = 2 * P.radius + 1 + 2 * kBiasPad;
+    if (EXTRA && table)  // [group, row_of_bias]
+        for (int i = threadIdx.x; i < table; i += kThreads) {
+            const int hh = i / row_of_bias, c = min(max(i - hh * row_of_bias - kBiasPad, 0), 2 * P.radius);
+            biases[i] = P.bias[(int64_t)(kh * group + hh) * (2 * P.radius + 1) + c];
+        }
 
     // Q: the B operand of S^T, row qi of head h, dims ds*16 + fh*8 .. +7. Whole rows
     // come in 64 dims at a time and are dealt out through a share of the LDS that no tile is in
@@ -512,7 +530,7 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
     const float scale = EXTRA ? fabsf(P.scale) : fabsf(P.scale) * kLog2e;
 
     f32x16 o[DT];     // O^T
-    float x[32];      // S^T of the newest tile: x[i] of the lane is the tile's key (i/8)*16 + fh*8 + i%8
+    f32x16 s[2];      // S^T of the newest tile: s[i / 16][i % 16] of the lane is the tile's key (i/8)*16 + fh*8 + i%8
     h8 ph[4], pl[4];  // its weights
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -522,7 +540,6 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
     int E = kUnsetE;
 
     auto scores = [&](const u16* kbuf) __attribute__((always_inline)) {
-        f32x16 s[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -552,8 +569,6 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
             for (int j = 0; j < 2; ++j) s[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[b][j][1], qh[ds], s[j], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int i = 0; i < 32; ++i) x[i] = s[i >> 4][i & 15];
     };
     auto visible = [&](int j) { return ((unsigned)j < (unsigned)pre) | ((unsigned)(j - see.lo) < (unsigned)(see.hi - see.lo)); };
     // Keeps the compiler from working on all 32 scores at once, for which there are no registers.
@@ -573,7 +588,7 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[u * 8 + i] = ldexpf(x[u * 8 + i], exps[u * 16 + fh * 8 + i]);
+                for (int i = 0; i < 8; ++i) s[u >> 1][(u & 1) * 8 + i] = ldexpf(s[u >> 1][(u & 1) * 8 + i], exps[u * 16 + fh * 8 + i]);
         }
         if (flag & kValueExps) {
             emax = kUnsetE;
@@ -586,30 +601,34 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
         }
         float unit = ct;  // of x
         if constexpr (EXTRA) {
-            const int mid = (h - kh * group) * (2 * P.radius + 1) + P.radius;
+            const float* near = biases + (h - kh * group) * row_of_bias + kBiasPad + P.radius;
+            const float* bp = P.bias + (int64_t)h * (2 * P.radius + 1) + P.radius;
             if (P.cap > 0.f) {
                 const float in = fminf(ct / P.cap, 3.40282347e38f);
                 float top = 0.f;
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
-                    x[i] *= in;
-                    top = fmaxf(top, fabsf(x[i]));
+                    s[i >> 4][i & 15] *= in;
+                    top = fmaxf(top, fabsf(s[i >> 4][i & 15]));
                 }
                 unit = P.cap;
                 // Scores well inside the cap, as most are, take the polynomial alone (half the
                 // instructions, no exponential).
                 const bool small = !__ballot(!(top < kTanhNear));
                 if (small) {
+                    float last = kTanhLast;
+                    asm volatile("" : "+v"(last));
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        x[i] = tanh_small(x[i]);
+                        s[i >> 4][i & 15] = tanh_small(s[i >> 4][i & 15], last);
                         few(i);
                     }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        asm volatile("" : "+v"(x[i]));  // the polynomials are not to be formed in front of the branch
-                        x[i] = tanh_near(x[i]);
+                        float y = s[i >> 4][i & 15];
+                        asm volatile("" : "+v"(y));  // the polynomials are not to be formed in front of the branch
+                        s[i >> 4][i & 15] = tanh_near(y);
                         few(i);
                     }
                 }
@@ -617,19 +636,24 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
             if (P.bias) {
                 const int from = k0 - last_p, to = k0 + kKT - 1 - first_p;  // the wave's distances
                 const int at = k0 + fh * 8 - p;
-                const float* bp = P.bias + (int64_t)kh * group * (2 * P.radius + 1);
                 if (to <= -P.radius || from >= P.radius) {  // one value for all
-                    const int c = mid + (from >= P.radius ? P.radius : -P.radius);
-                    const float v = table ? biases[c] : bp[c];
+                    const int c = from >= P.radius ? P.radius : -P.radius;
+                    float v;
+                    if (table) {
+                        v = near[c];
+                        asm volatile("" : "+v"(v));  // not one load by a chosen address: it would wait for the copies
+                    } else {
+                        v = bp[c];
+                    }
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) x[i] = fmaf(x[i], unit, v);
-                } else if (table && from >= -P.radius && to <= P.radius) {  // none clamped
-                    const float* b = biases + mid + at;
+                    for (int i = 0; i < 32; ++i) s[i >> 4][i & 15] = fmaf(s[i >> 4][i & 15], unit, v);
+                } else if (table) {  // beyond the radius by less than kBiasPad
+                    const float* b = near + at;
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            x[u * 8 + i] = fmaf(x[u * 8 + i], unit, b[u * 16 + i]);
+                            s[u >> 1][(u & 1) * 8 + i] = fmaf(s[u >> 1][(u & 1) * 8 + i], unit, b[u * 16 + i]);
                             few(i);
                         }
                 } else {
@@ -637,8 +661,7 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
                     for (int u = 0; u < 4; ++u)
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            const int c = mid + min(max(at + u * 16 + i, -P.radius), P.radius);
-                            x[u * 8 + i] = fmaf(x[u * 8 + i], unit, table ? biases[c] : bp[c]);
+                            s[u >> 1][(u & 1) * 8 + i] = fmaf(s[u >> 1][(u & 1) * 8 + i], unit, bp[min(max(at + u * 16 + i, -P.radius), P.radius)]);
                             few(i);
                         }
                 }
@@ -652,7 +675,7 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
             for (int u = 0; u < 4; ++u)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    if ((unsigned)(c + u * 16 + i) >= n) x[u * 8 + i] = -INFINITY;
+                    if ((unsigned)(c + u * 16 + i) >= n) s[u >> 1][(u & 1) * 8 + i] = -INFINITY;
                     few(i);
                 }
         } else if (edge) {
@@ -660,13 +683,13 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
             for (int u = 0; u < 4; ++u)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    if (!visible(k0 + u * 16 + fh * 8 + i)) x[u * 8 + i] = -INFINITY;
+                    if (!visible(k0 + u * 16 + fh * 8 + i)) s[u >> 1][(u & 1) * 8 + i] = -INFINITY;
                     few(i);
                 }
         }
-        float mt = x[0];
+        float mt = s[0][0];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) mt = fmaxf(mt, x[i]);
+        for (int i = 0; i < 32; ++i) mt = fmaxf(mt, s[i >> 4][i & 15]);
         mt *= unit;
         mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
         const float mnew = mt > m + (EXTRA ? kLazy / kLog2e : kLazy) ? mt : m;
@@ -686,22 +709,23 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
         // which would overflow.
         if (EXTRA && __ballot(!(fabsf(ref) < 1e4f))) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(fmaf(x[i], unit, -ref), kLog2e, (float)by));
+            for (int i = 0; i < 32; ++i) s[i >> 4][i & 15] = __builtin_amdgcn_exp2f(fmaf(fmaf(s[i >> 4][i & 15], unit, -ref), kLog2e, (float)by));
         } else {
             const float f = EXTRA ? unit * kLog2e : unit, up = (float)by - (EXTRA ? ref * kLog2e : ref);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], f, up));
+            for (int i = 0; i < 32; ++i) s[i >> 4][i & 15] = __builtin_amdgcn_exp2f(fmaf(s[i >> 4][i & 15], f, up));
         }
 #pragma unroll
-        for (int i = 0; i < 32; ++i) total += x[i];
+        for (int i = 0; i < 32; ++i) total += s[i >> 4][i & 15];
+        asm volatile("" : "+v"(total));  // not behind the branch below, for which the weights would be copied
         sum = fmaf(sum, alpha, ldexpf(total, -by));
         if (flag & kValueExps) {
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
                 for (int i = 0; i < 8; ++i)  // an unseen key's weight is zero, its exponent may be above E
-                    x[u * 8 + i] =
-                        ldexpf(x[u * 8 + i], min(max(exps[kKT + u * 16 + fh * 8 + i] - E, kFarE), 0));
+                    s[u >> 1][(u & 1) * 8 + i] =
+                        ldexpf(s[u >> 1][(u & 1) * 8 + i], min(max(exps[kKT + u * 16 + fh * 8 + i] - E, kFarE), 0));
         }
         if (__ballot(ao != 1.0f)) {
 #pragma unroll
@@ -714,7 +738,7 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
                 h2 hi, lo;
-                split_pair(x[u * 8 + i], x[u * 8 + i + 1], hi, lo);
+                split_pair(s[u >> 1][(u & 1) * 8 + i], s[u >> 1][(u & 1) * 8 + i + 1], hi, lo);
                 ph[u][i] = hi[0], ph[u][i + 1] = hi[1];
                 pl[u][i] = lo[0], pl[u][i + 1] = lo[1];
             }
@@ -1094,7 +1118,7 @@ bool run_tiles(const Packed& P, bool out16, int64_t rows, int64_t live) {
     if (kvec) k_attn_packed_split<DP, true><<<sg, 64 * kSplitWaves, 0, stream()>>>(P, X);
     else k_attn_packed_split<DP, false><<<sg, 64 * kSplitWaves, 0, stream()>>>(P, X);
     // What the tiles leave of a CU's LDS takes the bias of a group's heads, if it fits.
-    const int64_t values = P.bias ? (int64_t)(P.heads / P.kv_heads) * (2 * P.radius + 1) : 0;
+    const int64_t values = P.bias ? (int64_t)(P.heads / P.kv_heads) * (2 * P.radius + 1 + 2 * kBiasPad) : 0;
     const int table = values * 4 <= 14 * 1024 * (kWaves<DP> / 4) ? (int)values : 0;
     const bool extra = P.cap > 0.f || P.bias;
     using T_ = std::true_type;
