@@ -362,6 +362,36 @@ def test_equal_to_attention(be, orc):
         assert np.all(np.abs(c.run(be, causal=causal) - out.download()) <= 2 * tol)
 
 
+@gpu
+@pytest.mark.parametrize("radius", [0, 1, 33, 95, 200, 3000])
+@pytest.mark.parametrize("heads,kv,d", [(4, 4, 64), (6, 2, 64), (3, 1, 128)])
+def test_bias_radii(be, orc, radius, heads, kv, d):
+    """Tiles inside the radius, across it and behind it; 3000 is more than the LDS takes."""
+    c = Case(orc, [130, 400, 7], [130, 400, 420], heads, kv, d, seed=1700 + radius)
+    bias = orc.randn((heads, 2 * radius + 1), 1701, 0.0, 2.0)
+    for causal in (False, True):
+        c.check(be, orc, what=f"radius {radius} causal {causal}", bias=bias, radius=radius, causal=causal)
+
+
+@gpu
+@pytest.mark.parametrize("cap", [1e-40, 1e-3, 1.0, 8.0, 1e4])
+@pytest.mark.parametrize("lq", [1, 150])
+def test_caps(be, orc, cap, lq):
+    c = Case(orc, [lq, lq], [150, 300], 4, 2, 64, seed=1800, qstd=3.0)
+    c.check(be, orc, what=f"cap {cap}", cap=float(np.float32(cap)))
+    c.check(be, orc, what=f"cap {cap} bias", cap=float(np.float32(cap)), bias=orc.randn((4, 41), 1801), radius=20)
+
+
+@gpu
+def test_what_the_limits_allow(be, orc):
+    """A radius beyond every distance is the whole table's; the list's limit is itself allowed."""
+    c = Case(orc, [3], [5], 2, 1, 8, seed=1900)
+    c.check(be, orc, bias=orc.randn((2, 2001), 1901), radius=1000)
+    spans = np.zeros((65536, 4), np.int32)
+    spans[-1] = c.spans[0]
+    c.check(be, orc, spans=spans)
+
+
 def _args(**kw):
     a = dict(q=4096, k=4096, v=4096, out=4096, out_bf16=0, Tq=4, Tk=4, heads=2, kv=2, d=8, spans=4096, seqs=1, scale=1.0,
              causal=0, window=0, prefix=None, cap=0.0, bias=None, radius=0)

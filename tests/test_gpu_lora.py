@@ -205,6 +205,16 @@ def test_many_runs(be, orc, types):
 
 
 @gpu
+@pytest.mark.parametrize("K", [64, 1280])
+def test_as_many_runs_as_are_allowed(be, orc, K):
+    c = Case(orc, 40, 128, K, 8, 2, seed=850)
+    runs = np.zeros((65536, 4), np.int32)
+    runs[[7, 40000, 65535]] = [(0, 20, 0, 8), (20, 15, 1, 5), (35, 5, 1, 8)]
+    c.check(be, orc, runs)
+    c.check(be, orc, runs, False)
+
+
+@gpu
 @pytest.mark.parametrize("rows", [[200, 100], [1, 1, 1]])
 def test_captured(be, orc, rows):
     """Replayed with other runs and rows, the direct call between the replays."""
