@@ -130,74 +130,163 @@ __device__ __forceinline__ int adapter_of(const Lora& P, const dev::SpanTile& t,
 
 // ---------------------------------------------------------------------------
 // H[part][t, :] = s_a X[t] A_a^T over a share of K. A workgroup takes 32 RF rows of a run
-// and 32 RT ranks (blockIdx.z the block of ranks); K goes in blocks of 32 to its four
-// waves and to blockIdx.y's workgroups in turn (down_sums: a wave's sums). A lane reads 16 neighbouring values of
-// a row, the first eight for one MFMA step and the others for the next: whole lines,
-// and the sum does not mind the order.
+// and 32 RT ranks (blockIdx.z the block of ranks); K goes in blocks of a line of X (128
+// bytes) to its four waves and to blockIdx.y's workgroups in turn (down_sums: a wave's
+// sums). A lane's operands are the first or second half of a block, eight values an MFMA
+// step, of X and of A alike: the sum does not mind the order.
 // ---------------------------------------------------------------------------
-template <class TX, class TW, int RT, int RF, bool VEC>
-__device__ __forceinline__ void down_sums(const Lora& P, const dev::SpanTile& t, int adapter, int rank, int j0, int part, int parts,
+template <class TX>
+constexpr int kDownBlock = 128 / sizeof(TX);
+
+// A wave's 32 rows of `BLOCK` values as they are loaded, neighbouring lanes along a row, and their way
+// through the wave's 4 KB of LDS into MFMA operands. Loaded as operands, 16 bytes of each of 32 rows an
+// instruction, a line came to the L1 four times, and three of those went on to the L2: 47 us, now STAGED,
+// for [12528,3840] bf16 to 64 ranks.
+template <class T, int BLOCK>
+struct Staged {
+    static constexpr int kPieces = BLOCK * (int)sizeof(T) / 16, kLoads = kPieces / 2, kEach = 16 / (int)sizeof(T);
+    static_assert(kPieces == 8 || kPieces == 4, "rows of 128 or 64 bytes");
+    const T* row[kLoads];
+    u32x4 raw[kLoads];
+
+    // `rows` rows from p on, the lane's 16-byte piece of each.
+    __device__ __forceinline__ void rows_of(const T* p, int64_t ld, int rows) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) row[i] = p + min(i * (64 / kPieces) + lane / kPieces, rows - 1) * ld;
+    }
+    __device__ __forceinline__ void load(int k0, int end) {
+        const int k = k0 + (threadIdx.x & (kPieces - 1)) * kEach;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            raw[i] = *(const u32x4*)(row[i] + (k < end ? k : 0));
+            if (k >= end) raw[i] = u32x4{0u, 0u, 0u, 0u};
+        }
+    }
+    static __device__ __forceinline__ int at(int row, int piece) {
+        return row * (kPieces * 16) + ((piece ^ (kPieces == 8 ? row & 7 : (row >> 1) & 3)) << 4);
+    }
+    // The operands of the block's MFMA steps; a wave's LDS accesses keep their order.
+    __device__ __forceinline__ void deal(char* lds, Eight<T> (&out)[BLOCK / 16]) const {
+        const int lane = threadIdx.x & 63, fr = lane & 31, fh = lane >> 5;
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) *(u32x4*)(lds + at(i * (64 / kPieces) + lane / kPieces, lane & (kPieces - 1))) = raw[i];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int u = 0; u < BLOCK / 16; ++u) {
+            const int e = fh * (BLOCK / 16) + u;  // the eighth value
+            if constexpr (sizeof(T) == 2) {
+                out[u].a = *(const u32x4*)(lds + at(fr, e));
+            } else {
+                out[u].a = *(const f4*)(lds + at(fr, 2 * e));
+                out[u].b = *(const f4*)(lds + at(fr, 2 * e + 1));
+            }
+        }
+    }
+};
+
+// How X and A come: value by value (odd addresses or lengths), as operands, or STAGED. Few rows, whose
+// lines the L1 holds, come as operands, which saves the way through LDS: 48 single rows of 2560 bf16 10.6
+// us, staged 11.5; [12528,3840] bf16 to 64 ranks and 10240 columns 166 us, staged 147.
+enum { kValues, kOperands, kStaged };
+
+// `lds`: the wave's own 4 KB, 16-byte aligned.
+template <class TX, class TW, int RT, int RF, int MODE>
+__device__ __forceinline__ void down_sums(const Lora& P, const dev::SpanTile& t, int adapter, int rank, int j0, int part, int parts, char* lds,
                                           f32x16 (&acc)[RF][RT]) {
+    constexpr int BLOCK = kDownBlock<TX>, U = BLOCK / 16;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, fr = lane & 31, fh = lane >> 5;
-    const TX* x[RF];
-    const TW* a[RT];
-#pragma unroll
-    for (int i = 0; i < RF; ++i) x[i] = (const TX*)P.x + (t.first + min(t.row0 + i * 32 + fr, t.rows - 1)) * P.ldx;
-#pragma unroll
-    for (int i = 0; i < RT; ++i) a[i] = (const TW*)P.a + ((int64_t)adapter * P.rank + min(j0 + i * 32 + fr, rank - 1)) * P.K;
+    const TX* x0 = (const TX*)P.x + (t.first + t.row0) * P.ldx;
+    const TW* a0 = (const TW*)P.a + ((int64_t)adapter * P.rank + j0) * P.K;
 #pragma unroll
     for (int i = 0; i < RF; ++i)
 #pragma unroll
         for (int j = 0; j < RT; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    // bf16 rows are half the bytes a block: two blocks on their way
-    constexpr int DEPTH = sizeof(TX) == 2 ? 2 : 1, U = 2 * DEPTH;
-    Eight<TX> xn[U][RF];
-    Eight<TW> an[U][RT];
-    const int step = 32 * kLoraWaves * parts;
-    auto load = [&](int k0) __attribute__((always_inline)) {
+    const int step = BLOCK * kLoraWaves * parts;
+    int k = (part * kLoraWaves + w) * BLOCK;
+    auto add = [&](const Eight<TX> (&x)[RF][U], const Eight<TW> (&a)[U], int j) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int k = k0 + u / 2 * step;
+            bf16x8 ap[Eight<TW>::kParts];
+            a[u].parts(ap);
 #pragma unroll
-            for (int i = 0; i < RF; ++i) xn[u][i].template load<VEC>(x[i], k + fh * 16 + u % 2 * 8, P.K);
-#pragma unroll
-            for (int i = 0; i < RT; ++i) an[u][i].template load<VEC>(a[i], k + fh * 16 + u % 2 * 8, P.K);
+            for (int i = 0; i < RF; ++i) {
+                bf16x8 xp[Eight<TX>::kParts];
+                x[i][u].parts(xp);
+                acc[i][j] = multiply<Eight<TX>::kParts, Eight<TW>::kParts>(xp, ap, acc[i][j]);
+            }
         }
     };
-    int k = (part * kLoraWaves + w) * 32;
-    if (k < P.K) load(k);
-    for (; k < P.K; k += DEPTH * step) {
-        Eight<TX> xc[U][RF];
-        Eight<TW> ac[U][RT];
+    if constexpr (MODE == kStaged) {
+        Staged<TX, BLOCK> x[RF];
+        Staged<TW, BLOCK> a[RT];
+        // rows behind the run's, and ranks behind the adapter's, are its last one again
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+        for (int i = 0; i < RF; ++i) x[i].rows_of(x0 + min(i * 32, t.rows - 1 - t.row0) * P.ldx, P.ldx, max(t.rows - t.row0 - i * 32, 1));
 #pragma unroll
-            for (int i = 0; i < RF; ++i) xc[u][i] = xn[u][i];
+        for (int j = 0; j < RT; ++j) a[j].rows_of(a0 + (int64_t)min(j * 32, rank - 1 - j0) * P.K, P.K, max(rank - j0 - j * 32, 1));
+        auto load = [&](int k0) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < RT; ++i) ac[u][i] = an[u][i];
+            for (int i = 0; i < RF; ++i) x[i].load(k0, P.K);
+#pragma unroll
+            for (int j = 0; j < RT; ++j) a[j].load(k0, P.K);
+        };
+        if (k < P.K) load(k);
+        for (; k < P.K; k += step) {
+            Eight<TX> xf[RF][U];
+            Eight<TW> af[RT][U];
+#pragma unroll
+            for (int i = 0; i < RF; ++i) x[i].deal(lds, xf[i]);
+#pragma unroll
+            for (int j = 0; j < RT; ++j) a[j].deal(lds, af[j]);
+            if (k + step < P.K) load(k + step);
+#pragma unroll
+            for (int j = 0; j < RT; ++j) add(xf, af[j], j);
         }
-        if (k + DEPTH * step < P.K) load(k + DEPTH * step);
+    } else {
+        constexpr bool VEC = MODE == kOperands;
+        const TX* x[RF];
+        const TW* a[RT];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            bf16x8 xp[RF][Eight<TX>::kParts];
+        for (int i = 0; i < RF; ++i) x[i] = x0 + min(i * 32 + fr, t.rows - 1 - t.row0) * P.ldx;
 #pragma unroll
-            for (int i = 0; i < RF; ++i) xc[u][i].parts(xp[i]);
+        for (int j = 0; j < RT; ++j) a[j] = a0 + (int64_t)min(j * 32 + fr, rank - 1 - j0) * P.K;
+        Eight<TX> xn[RF][U];
+        Eight<TW> an[RT][U];
+        auto load = [&](int k0) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < RT; ++j) {
-                bf16x8 ap[Eight<TW>::kParts];
-                ac[u][j].parts(ap);
+            for (int u = 0; u < U; ++u) {
+                const int at = k0 + fh * (BLOCK / 2) + u * 8;
 #pragma unroll
-                for (int i = 0; i < RF; ++i) acc[i][j] = multiply<Eight<TX>::kParts, Eight<TW>::kParts>(xp[i], ap, acc[i][j]);
+                for (int i = 0; i < RF; ++i) xn[i][u].template load<VEC>(x[i], at, P.K);
+#pragma unroll
+                for (int j = 0; j < RT; ++j) an[j][u].template load<VEC>(a[j], at, P.K);
             }
+        };
+        if (k < P.K) load(k);
+        for (; k < P.K; k += step) {
+            Eight<TX> xc[RF][U];
+            Eight<TW> ac[RT][U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+#pragma unroll
+                for (int i = 0; i < RF; ++i) xc[i][u] = xn[i][u];
+#pragma unroll
+                for (int j = 0; j < RT; ++j) ac[j][u] = an[j][u];
+            }
+            if (k + step < P.K) load(k + step);
+#pragma unroll
+            for (int j = 0; j < RT; ++j) add(xc, ac[j], j);
         }
     }
 }
 
-template <class TX, class TW, int RT, int RF, bool VEC>
+template <class TX, class TW, int RT, int RF, int MODE>
 __global__ __launch_bounds__(kLoraThreads) void k_lora_down(Lora P) {
-    __shared__ float part[kLoraWaves][RF * 32][33];
+    __shared__ __attribute__((aligned(16))) float part[kLoraWaves][RF * 32][33];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, fr = lane & 31, fh = lane >> 5;
     dev::SpanTile t;
     if (!dev::find_tile(P.runs, P.count, P.M, 1, RF * 32, blockIdx.x, t)) return;
@@ -205,7 +294,7 @@ __global__ __launch_bounds__(kLoraThreads) void k_lora_down(Lora P) {
     const int adapter = adapter_of(P, t, rank), j0 = blockIdx.z * RT * 32;
     if (j0 >= rank) return;  // up reads none of them
     f32x16 acc[RF][RT];
-    down_sums<TX, TW, RT, RF, VEC>(P, t, adapter, rank, j0, blockIdx.y, P.splits, acc);
+    down_sums<TX, TW, RT, RF, MODE>(P, t, adapter, rank, j0, blockIdx.y, P.splits, (char*)part[w], acc);
     const float f = P.scale ? P.scale[adapter] : 1.0f;
     float* h = P.h + ((int64_t)blockIdx.y * P.M + t.first + t.row0) * P.hrank;
     const int left = t.rows - t.row0;
@@ -354,7 +443,7 @@ __global__ __launch_bounds__(kLoraThreads, KS <= 4 ? 2 : 1) void k_lora_up(Lora 
 template <class TX, class TW, int KS, bool XVEC, bool VEC, bool CV>
 __global__ __launch_bounds__(kLoraThreads, 2) void k_lora_small(Lora P, int columns) {
     constexpr int RT = (KS + 1) / 2;
-    __shared__ float part[kLoraWaves][32][33];
+    __shared__ __attribute__((aligned(16))) float part[kLoraWaves][32][33];
     __shared__ __attribute__((aligned(16))) float h[32][RT * 32 + 4];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, fr = lane & 31, fh = lane >> 5;
     dev::SpanTile t;
@@ -369,7 +458,7 @@ __global__ __launch_bounds__(kLoraThreads, 2) void k_lora_small(Lora P, int colu
         return;
     }
     f32x16 acc[1][RT];
-    down_sums<TX, TW, RT, 1, XVEC>(P, t, adapter, rank, 0, 0, 1, acc);
+    down_sums<TX, TW, RT, 1, XVEC ? kOperands : kValues>(P, t, adapter, rank, 0, 0, 1, (char*)part[w], acc);
     const float f = P.scale ? P.scale[adapter] : 1.0f;
 #pragma unroll
     for (int j = 0; j < RT; ++j) {
@@ -558,9 +647,18 @@ void launch_lora(Lora P, int64_t M, bool vec) {
         using One = integral_constant<int, 1>;
         using Two = integral_constant<int, 2>;
         using Four = integral_constant<int, 4>;
-        if (rt == 1) vec ? (rf == 2 ? go(One(), Two(), T_()) : go(One(), One(), T_())) : go(One(), One(), F_());
-        else if (rt == 2) vec ? (rf == 2 ? go(Two(), Two(), T_()) : go(Two(), One(), T_())) : go(Two(), One(), F_());
-        else vec ? go(Four(), One(), T_()) : go(Four(), One(), F_());
+        using Values = integral_constant<int, kValues>;
+        using Operands = integral_constant<int, kOperands>;
+        using Staged = integral_constant<int, kStaged>;
+        auto with = [&](auto r) {  // four tiles of ranks go with one of rows
+            if (!vec) go(r, One(), Values());
+            else if (few) go(r, One(), Operands());
+            else if constexpr (decltype(r)::value > 2) go(r, One(), Staged());
+            else go(r, Two(), Staged());
+        };
+        if (rt == 1) with(One());
+        else if (rt == 2) with(Two());
+        else with(Four());
     }
     for (int j0 = 0; j0 == 0 || j0 < P.rank; j0 += 128) {
         const int ks = std::min(P.rank - j0, 128);
