@@ -4,14 +4,18 @@
 // backend_cuda.h:38-43, gemm_nt_bf16 / gemm_nt_f32).
 //
 // Two launches: down, H = s_a X A_a^T into scratch, and up, C (+)= H B_a^T, both on
-// v_mfma_f32_32x32x16_bf16. fp32 accuracy: a float is the exact sum of three bf16
-// values (24 bits in steps of 8, cut towards zero, so nothing overflows and the range is
-// fp32's), a bf16 value its own; the products of the parts are exact in the fp32
-// accumulators. X keeps its 24 bits, unlike the A of gemm_nt_bf16. With fp32 weights the
-// product of the two smallest parts (below 2^-28) is left out.
+// v_mfma_f32_32x32x16_bf16; one for few rows and a short K (k_lora_small). fp32 accuracy:
+// a float is the exact sum of three bf16 values (24 bits in steps of 8, cut towards zero,
+// so nothing overflows and the range is fp32's), a bf16 value its own; the products of the
+// parts are exact in the fp32 accumulators. X keeps its 24 bits, unlike the A of
+// gemm_nt_bf16. With fp32 weights the product of the two smallest parts (below 2^-28) is
+// left out.
 //
-// Both are bound by memory: X is read once (a workgroup has all ranks of its
-// rows), C read and written once, while A and B come from the L2s.
+// Bound by memory for many rows: X is read once (a workgroup has all ranks of its rows), C
+// read and written once, while A, B and H come from the L2s. [12528,3840] bf16 to 10240
+// columns, rank 64: 137 us, 4.5 TB/s (down 29, up 104; a kernel that only writes C takes
+// 77); [8192,640] to 5120, fp32, rank 12: 78 us, 4.0 TB/s; 48 single rows of 2560 to 4096
+// columns, rank 16: 10.4 us, the two launches' own length.
 #include <algorithm>
 #include <string>
 #include <type_traits>
@@ -140,8 +144,8 @@ constexpr int kDownBlock = 128 / sizeof(TX);
 
 // A wave's 32 rows of `BLOCK` values as they are loaded, neighbouring lanes along a row, and their way
 // through the wave's 4 KB of LDS into MFMA operands. Loaded as operands, 16 bytes of each of 32 rows an
-// instruction, a line came to the L1 four times, and three of those went on to the L2: 47 us, now STAGED,
-// for [12528,3840] bf16 to 64 ranks.
+// instruction, a line came to the L1 four times, and three of those went on to the L2: 47 us, STAGED 34, for
+// [12528,3840] bf16 to 64 ranks.
 template <class T, int BLOCK>
 struct Staged {
     static constexpr int kPieces = BLOCK * (int)sizeof(T) / 16, kLoads = kPieces / 2, kEach = 16 / (int)sizeof(T);
@@ -483,7 +487,7 @@ __global__ __launch_bounds__(kLoraThreads, 2) void k_lora_small(Lora P, int colu
     up_columns<TW, KS, VEC, CV>(P, adapter, rank, 0, hp, n, n1, c, left);
 }
 
-// The same for runs of many rows: the waves of a workgroup have neighbouring rows and share
+// Up for runs of many rows: the waves of a workgroup have neighbouring rows and share
 // each 128 columns of B through LDS. Read from memory by its rows, a fragment (32 rows of B,
 // 16 bytes each a lane) costs the L1 an access a lane: 60 million of them took 112 of 185 us
 // at [12528,64] x [10240,64]^T. The copies to LDS are of whole rows, 16 bytes a lane, two
@@ -632,10 +636,12 @@ void launch_lora(Lora P, int64_t M, bool vec) {
         return;
     }
     if (P.rank > 0) {
-        // Parts of K until the chip has four workgroups a CU, while each wave keeps two blocks, and at
-        // most four, which up has to sum: [2480,2560] -> 4096 takes 42 us with two, 38 with four, 44 with eight.
+        // Parts of K until the chip has two workgroups a CU, as many as fit, while each wave keeps two
+        // blocks, and at most four, which up has to sum: [2480,2560] -> 4096 takes 42 us with two, 38 with
+        // four, 44 with eight; [12528,3840] bf16 -> 10240 rank 64 137 us with two (this rule), 145 with four,
+        // 150 with one.
         const int64_t most = std::max<int64_t>(1, P.K / (64 * kLoraWaves));
-        P.splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, 4 * cus / std::max<int64_t>(1, M / (32 * rf) + 1), 4}));
+        P.splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, 2 * cus / std::max<int64_t>(1, M / (32 * rf) + 1), 4}));
     }
     P.hrank = (P.rank + 31) / 32 * 32;
     P.h = (float*)scratch(std::max<size_t>((size_t)P.splits * M * P.hrank * 4, 4));
