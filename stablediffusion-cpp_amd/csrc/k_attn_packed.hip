@@ -67,7 +67,8 @@ __device__ __forceinline__ float tanh_near(float x) {
 
 // ---------------------------------------------------------------------------
 // Any head dimension: fp32 products, one wave per (query, head). Lanes take 64 keys at a
-// time for the scores, then 64 columns at a time for the weighted sum.
+// time for the scores, then 64 columns at a time for the weighted sum. Takes heads of more
+// than 128 dims, and calls whose tiles find no scratch.
 // ---------------------------------------------------------------------------
 constexpr int kRowWaves = 4, kMaxD = 1024;
 
@@ -169,6 +170,11 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_attn_packed_rows(Packed P) {
 // the wave in both, its statistics are its own. K's rows are ordered so that the eight
 // scores of a lane's half of a 16-key step are eight neighbouring keys: its weights
 // are the second product's operand as they lie, V^T in the keys' own order.
+//
+// Long sequences are bound by the three products: two images of 4200 rows, 30 heads of 128,
+// 1.42 ms, 377 TFLOP/s of 4 d a visible pair, as k_attention.hip's kernel on that shape; the split 0.1
+// ms of it. Short ones by their workgroups' starts (the list, q): 24 prompts of up to 203
+// rows, 32/8 heads of 128, 61 us, 16 of them their bytes at the rate of a copy.
 // ---------------------------------------------------------------------------
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -858,6 +864,9 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
 // DP / 4 lanes have a key, four of its values each (whole rows of 64 or 128 values a load,
 // 2 or 4 keys), a wave kLoads loads of keys and as many of values at once. Every group of
 // lanes keeps a softmax of its own keys; they are put together at the end.
+//
+// Bound by the cache's bytes: 32 tokens of 40 to 4096 keys, 32/8 heads of 128, 102 us with the
+// join, 5.4 TB/s. Four loads instead of eight, two or eight waves instead of four: all slower.
 // ---------------------------------------------------------------------------
 constexpr int kLoads = 8, kFewWaves = 4;
 
@@ -1168,9 +1177,11 @@ void run_attention_packed(const float* q, const float* k, const float* v, void* 
     Packed P{q,    k,   v,   out, (const int4*)spans, prefix, bias, (int)Tq, (int)Tk, (int)seqs, heads, kv_heads, (int)d, causal ? 1 : 0,
              window < kMost ? (int)window : 0,  // a wider one hides nothing
              bias ? (int)radius : 0, scale, cap};
-    // A sequence's rows at one key/value head are few: see k_attn_packed_few.
+    // An average sequence's rows at one key/value head: up to sixteen go to k_attn_packed_few. Measured, us, there /
+    // in tiles, 32/8 heads of 128: 32 sequences of up to 4096 keys, 8 rows 158 / 406, 16 rows 261 / 420, 40 rows 568 /
+    // 434; four sequences, 16 rows 64 / 79, 40 rows 112 / 80; 32 of up to 256 keys, 16 rows 32 / 37, 40 rows 66 / 38.
     const int64_t group = heads / kv_heads, live = std::min(seqs, Tq), mean = (Tq + live - 1) / live * group;
-    if (d <= 128 && d % 4 == 0 && mean <= 8 && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out)) {
+    if (d <= 128 && d % 4 == 0 && mean <= 16 && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out)) {
         const int r = mean <= 1 ? 1 : mean <= 4 ? 4 : 8;
         const int64_t n = Tq * group / r + live;
         if (Tq * group < kMost && n * kv_heads * 64 * kFewWaves <= kMaxGridItems) {

@@ -383,6 +383,16 @@ def test_caps(be, orc, cap, lq):
 
 
 @gpu
+@pytest.mark.parametrize("mask", ["causal", "everything", "prefix_window"])
+@pytest.mark.parametrize("heads,kv,d", [(8, 1, 128), (8, 2, 64), (3, 3, 40)])
+@pytest.mark.parametrize("lq", [[2, 2, 2], [4, 1, 7], [1, 16, 20]])
+def test_a_few_queries_of_long_rows(be, orc, lq, heads, kv, d, mask):
+    """Up to sixteen rows a sequence and key/value head, some sequences with more, one with more queries than keys."""
+    c = Case(orc, lq, [500, 37, 13], heads, kv, d, seed=1750)
+    c.check(be, orc, what=f"{lq} {mask}", **masks(orc, mask, 3, heads))
+
+
+@gpu
 def test_what_the_limits_allow(be, orc):
     """A radius beyond every distance is the whole table's; the list's limit is itself allowed."""
     c = Case(orc, [3], [5], 2, 1, 8, seed=1900)
