@@ -154,7 +154,8 @@ int sdh_linear_swiglu(const float* x, const uint16_t* w1, const uint16_t* w3, fl
  * of B_a from there on are not read as numbers). A run with no such adapter (-1) or rank 0 adds
  * nothing: its rows are left, or zero without accumulate. Runs must not share
  * rows; entries past the matrix are cut to it; rows of no run are left as they
- * were. Everything is held in fp32, X unrounded. C must not overlap an input. */
+ * were. Everything is held in fp32, X unrounded. C must not overlap an input.
+ * H = X A_a^T goes through scratch (not for few rows and K to 640). */
 int sdh_lora_nt_bf16(int64_t M, int64_t N, int64_t K, const float* X, int64_t ldx, const uint16_t* A,
                      const uint16_t* B, int64_t rank, int64_t adapters, const float* scale, const int32_t* segments,
                      int64_t count, float* C, int64_t ldc, int accumulate);
@@ -315,7 +316,9 @@ int sdh_attention_fp16(const float* q, const float* k, const float* v, void* out
  *   out must not overlap an input. The arrays are read when the work runs, so a
  * captured graph takes the spans that they hold at each replay. Where no scratch
  * can be had (a full arena; a capture that asks for more than any call before it)
- * a slower kernel gives the same result. */
+ * a slower kernel gives the same result. The kernel is chosen by Tq, Tk and seqs:
+ * single tokens against long caches are best not mixed with long prompts in a
+ * call. */
 int sdh_attention_packed(const float* q, const float* k, const float* v, void* out, int out_bf16, int64_t Tq,
                          int64_t Tk, int heads, int kv_heads, int64_t d, const int32_t* spans, int64_t seqs,
                          float scale, int causal, int64_t window, const int32_t* prefix, float cap,

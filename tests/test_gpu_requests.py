@@ -3,6 +3,10 @@ rows of ragged prompts through norm, shared projections, each request's adapter,
 positions and packed attention into a cache in slots, then single tokens against that
 cache; directly and from two captured graphs. Every step is held to its own definition
 in float64, from what the device had in hand before it."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -180,3 +184,61 @@ def test_tokens_from_graphs(be, orc):
     finally:
         for g in graphs:
             be.graph_destroy(g)
+
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+ROOT = os.path.dirname(HERE)
+FRESH = r"""
+import sys
+sys.path[:0] = [%r, %r]
+import numpy as np, sdhip
+from oracle import Oracle
+be, orc = sdhip.Backend(), Oracle()
+T, heads, d = 200, 4, 64
+q, k, v = (be.array(orc.randn((T, heads * d), i)) for i in range(3))
+out, spans = be.empty((T, heads * d)), np.array([(0, 150, 0, 150), (150, 50, 150, 50)], np.int32)
+dspans = be.array(spans)
+X, A, B, C = be.array(orc.randn((T, 1280), 4)), orc.randn((2, 8, 1280), 5, 0.0, 0.03), orc.randn((2, 96, 8), 6), be.array(np.zeros((T, 96), np.float32))
+dA, dB, runs = be.array(A), be.array(B), np.array([(0, 150, 0, 8), (150, 50, 1, 8)], np.int32)
+druns = be.array(runs)
+def attend():
+    be.attention_packed(q, k, v, out, T, T, heads, heads, d, dspans, 2, 0.125, causal=True)
+def adapt():
+    be.lora_nt_f32(T, 96, 1280, X, 1280, dA, dB, 8, 2, None, druns, 2, C, 96, accumulate=False)
+be.capture_begin()
+attend()
+try:
+    adapt()
+    raise SystemExit('not refused')
+except sdhip.SdhError as e:
+    assert e.status == sdhip.SDH_ERR_INVALID and 'captur' in str(e), e
+graph = be.capture_end()
+adapt()
+be.capture_begin()
+adapt()
+second = be.capture_end()
+for i in range(3):
+    x = orc.randn((T, heads * d), 10 + i)
+    q.upload(x)
+    be.call('sdh_zero', out.ptr, out.nbytes)
+    be.call('sdh_zero', C.ptr, C.nbytes)
+    be.graph_launch(graph)
+    be.graph_launch(second)
+    want, tol = orc.attention_packed(x, k.download(), v.download(), np.zeros((T, heads * d)), spans, heads, heads, 0.125, causal=True)
+    assert np.all(np.abs(out.download() - want) <= tol), i
+    want, tol = orc.lora(X.download(), A, B, None, runs, np.zeros((T, 96)), False)
+    assert np.all(np.abs(C.download() - want) <= tol), i
+    attend()
+    adapt()
+    be.synchronize()
+be.graph_destroy(graph)
+be.graph_destroy(second)
+print('fresh ok', flush=True)
+""" % (os.path.join(ROOT, "stablediffusion-cpp_amd"), os.path.join(ROOT, "oracle"))
+
+
+def test_captured_before_any_call():
+    """In a process where no call has had scratch: attention goes without, the adapters are refused until they have run."""
+    r = subprocess.run([sys.executable, "-u", "-c", FRESH], capture_output=True, text=True, timeout=100)
+    print(r.stdout, r.stderr[-3000:])
+    assert r.returncode == 0 and "fresh ok" in r.stdout
