@@ -153,11 +153,11 @@ struct Staged {
     const T* row[kLoads];
     u32x4 raw[kLoads];
 
-    // `rows` rows from p on, the lane's 16-byte piece of each.
-    __device__ __forceinline__ void rows_of(const T* p, int64_t ld, int rows) {
+    // Every `stride`-th row from `first` to `last` of p, the lane's 16-byte piece of each.
+    __device__ __forceinline__ void rows_of(const T* p, int64_t ld, int first, int stride, int last) {
         const int lane = threadIdx.x & 63;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) row[i] = p + min(i * (64 / kPieces) + lane / kPieces, rows - 1) * ld;
+        for (int i = 0; i < kLoads; ++i) row[i] = p + min(first + (i * (64 / kPieces) + lane / kPieces) * stride, last) * ld;
     }
     __device__ __forceinline__ void load(int k0, int end) {
         const int k = k0 + (threadIdx.x & (kPieces - 1)) * kEach;
@@ -170,8 +170,10 @@ struct Staged {
     static __device__ __forceinline__ int at(int row, int piece) {
         return row * (kPieces * 16) + ((piece ^ (kPieces == 8 ? row & 7 : (row >> 1) & 3)) << 4);
     }
-    // The operands of the block's MFMA steps; a wave's LDS accesses keep their order.
-    __device__ __forceinline__ void deal(char* lds, Eight<T> (&out)[BLOCK / 16]) const {
+    // The operands of the block's MFMA steps, a lane's half of the block (HALVES) or of each step; a wave's LDS
+    // accesses keep their order.
+    template <bool HALVES>
+    __device__ __forceinline__ void deal(char* lds, Eight<T>* out) const {
         const int lane = threadIdx.x & 63, fr = lane & 31, fh = lane >> 5;
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -179,7 +181,7 @@ struct Staged {
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int u = 0; u < BLOCK / 16; ++u) {
-            const int e = fh * (BLOCK / 16) + u;  // the eighth value
+            const int e = HALVES ? fh * (BLOCK / 16) + u : u * 2 + fh;
             if constexpr (sizeof(T) == 2) {
                 out[u].a = *(const u32x4*)(lds + at(fr, e));
             } else {
@@ -229,9 +231,9 @@ __device__ __forceinline__ void down_sums(const Lora& P, const dev::SpanTile& t,
         Staged<TW, BLOCK> a[RT];
         // rows behind the run's, and ranks behind the adapter's, are its last one again
 #pragma unroll
-        for (int i = 0; i < RF; ++i) x[i].rows_of(x0 + min(i * 32, t.rows - 1 - t.row0) * P.ldx, P.ldx, max(t.rows - t.row0 - i * 32, 1));
+        for (int i = 0; i < RF; ++i) x[i].rows_of(x0, P.ldx, i * 32, 1, t.rows - 1 - t.row0);
 #pragma unroll
-        for (int j = 0; j < RT; ++j) a[j].rows_of(a0 + (int64_t)min(j * 32, rank - 1 - j0) * P.K, P.K, max(rank - j0 - j * 32, 1));
+        for (int j = 0; j < RT; ++j) a[j].rows_of(a0, P.K, j * 32, 1, rank - 1 - j0);
         auto load = [&](int k0) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < RF; ++i) x[i].load(k0, P.K);
@@ -243,9 +245,9 @@ __device__ __forceinline__ void down_sums(const Lora& P, const dev::SpanTile& t,
             Eight<TX> xf[RF][U];
             Eight<TW> af[RT][U];
 #pragma unroll
-            for (int i = 0; i < RF; ++i) x[i].deal(lds, xf[i]);
+            for (int i = 0; i < RF; ++i) x[i].template deal<true>(lds, xf[i]);
 #pragma unroll
-            for (int j = 0; j < RT; ++j) a[j].deal(lds, af[j]);
+            for (int j = 0; j < RT; ++j) a[j].template deal<true>(lds, af[j]);
             if (k + step < P.K) load(k + step);
 #pragma unroll
             for (int j = 0; j < RT; ++j) add(xf, af[j], j);
@@ -358,7 +360,7 @@ __device__ __forceinline__ void parts_of_h(const Lora& P, int64_t row, int j0, i
 // ---------------------------------------------------------------------------
 // The columns n .. n1 of a wave's rows, `left` of them, from c on; hp null without an adapter: zeros.
 template <class TW, int KS, bool VEC, bool CV>
-__device__ __forceinline__ void up_columns(const Lora& P, int adapter, int rank, int j0, const bf16x8 (*hp)[3], int n, int n1, float* c, int left) {
+__device__ __forceinline__ void up_columns(const Lora& P, int adapter, int rank, int j0, const bf16x8 (*hp)[3], int n, int n1, float* c, int left, char* lds) {
     const int lane = threadIdx.x & 63, fr = lane & 31, fh = lane >> 5;
     auto row_of = [&](int e) { return (e >> 2) * 8 + fh * 4 + (e & 3); };
     auto put = [&](int e, int col, const f4& v) __attribute__((always_inline)) {
@@ -396,12 +398,31 @@ __device__ __forceinline__ void up_columns(const Lora& P, int adapter, int rank,
             }
         }
         f32x16 acc[4];
+        // bf16 rows of whole lines come STAGED: 48 single rows of 2560 to 4096 columns, rank 64, 19.1 -> 17.3 us. fp32 ones
+        // do not: their parts leave no registers for a second stage (rank 128 58 -> 68).
+        constexpr int BLOCK = 128 / sizeof(TW), BLOCKS = KS * 16 / BLOCK;
+        constexpr bool STAGE = VEC && sizeof(TW) == 2 && BLOCKS > 0;
+        Staged<TW, BLOCK> staged[2][STAGE ? BLOCKS : 1];
+        auto ask = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+            for (int k = 0; k < BLOCKS; ++k) {
+                staged[j & 1][k].rows_of(b, P.rank, n + j, 4, P.N - 1);
+                staged[j & 1][k].load(j0 + k * BLOCK, rank);
+            }
+        };
+        if constexpr (STAGE) ask(0);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             Eight<TW> bn[KS];
-            const TW* row = b + (int64_t)min(col + j, P.N - 1) * P.rank;
+            if constexpr (STAGE) {
+                if (j < 3) ask(j + 1);
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) bn[ks].template load<VEC>(row, j0 + ks * 16 + fh * 8, rank);
+                for (int k = 0; k < BLOCKS; ++k) staged[j & 1][k].template deal<false>(lds, bn + k * (BLOCK / 16));
+            } else {
+                const TW* row = b + (int64_t)min(col + j, P.N - 1) * P.rank;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) bn[ks].template load<VEC>(row, j0 + ks * 16 + fh * 8, rank);
+            }
             if (VEC && rank % 8) {  // what lies behind the ranks that count may be anything
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) bn[ks].cut(rank - (j0 + ks * 16 + fh * 8));
@@ -422,6 +443,7 @@ __device__ __forceinline__ void up_columns(const Lora& P, int adapter, int rank,
 
 template <class TW, int KS, bool FEW, bool VEC, bool CV>
 __global__ __launch_bounds__(kLoraThreads, KS <= 4 ? 2 : 1) void k_lora_up(Lora P, int j0, int columns) {
+    __shared__ __attribute__((aligned(16))) char lds[VEC ? kLoraWaves : 1][4096];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, fr = lane & 31, fh = lane >> 5;
     dev::SpanTile t;
     if (!dev::find_tile(P.runs, P.count, P.M, 1, FEW ? 32 : 32 * kLoraWaves, blockIdx.x, t)) return;
@@ -433,12 +455,12 @@ __global__ __launch_bounds__(kLoraThreads, KS <= 4 ? 2 : 1) void k_lora_up(Lora 
     const int64_t first = t.first + row0;
     float* c = P.c + first * P.ldc;
     if (adapter < 0) {  // only without accumulate; B may not be there at all
-        up_columns<TW, KS, VEC, CV>(P, adapter, rank, j0, nullptr, n, n1, c, left);
+        up_columns<TW, KS, VEC, CV>(P, adapter, rank, j0, nullptr, n, n1, c, left, nullptr);
         return;
     }
     bf16x8 hp[KS][3];
     parts_of_h<KS>(P, first + min(fr, left - 1), j0, rank, fh, hp);
-    up_columns<TW, KS, VEC, CV>(P, adapter, rank, j0, hp, n, n1, c, left);
+    up_columns<TW, KS, VEC, CV>(P, adapter, rank, j0, hp, n, n1, c, left, lds[VEC ? w : 0]);
 }
 
 // Both in one launch, for few rows a run and a short K: every workgroup of a run forms H for
@@ -458,7 +480,7 @@ __global__ __launch_bounds__(kLoraThreads, 2) void k_lora_small(Lora P, int colu
     if (P.accumulate && !rank) return;
     float* c = P.c + (int64_t)(t.first + t.row0) * P.ldc;
     if (adapter < 0) {
-        up_columns<TW, KS, VEC, CV>(P, adapter, rank, 0, nullptr, n, n1, c, left);
+        up_columns<TW, KS, VEC, CV>(P, adapter, rank, 0, nullptr, n, n1, c, left, nullptr);
         return;
     }
     f32x16 acc[1][RT];
@@ -484,7 +506,7 @@ __global__ __launch_bounds__(kLoraThreads, 2) void k_lora_small(Lora P, int colu
         v.b = *(const f4*)&h[fr][ks * 16 + fh * 8 + 4];
         v.parts(hp[ks]);
     }
-    up_columns<TW, KS, VEC, CV>(P, adapter, rank, 0, hp, n, n1, c, left);
+    up_columns<TW, KS, VEC, CV>(P, adapter, rank, 0, hp, n, n1, c, left, (char*)part[w]);
 }
 
 // Up for runs of many rows: the waves of a workgroup have neighbouring rows and share
@@ -615,10 +637,10 @@ void launch_lora(Lora P, int64_t M, bool vec) {
     int64_t columns = 4096;
     while (columns > 128 && tiles * ((P.N + columns * (few ? kLoraWaves : 1) - 1) / (columns * (few ? kLoraWaves : 1))) < (few ? 6 : 4) * (int64_t)cus)
         columns /= 2;
-    // One launch or two, for few rows a run. Measured, us, one / two, 48 single rows to 4096 columns:
-    // K 320 rank 8 7.3 / 9.3, rank 64 13.4 / 15.8; K 640 rank 8 8.7 / 9.4, rank 64 16.0 / 16.2, rank
-    // 128 67 / 51; K 1280 rank 8 12.0 / 9.6.
-    if (few && P.rank > 0 && P.rank <= 64 && P.K <= 640) {
+    // One launch or two, for few rows a run: by K and the bytes of a row of B. Measured, us, one / two, 48 single rows to
+    // 4096 columns: bf16 K 320 rank 8 7.4 / 9.3, rank 64 11.9 / 13.9; K 640 rank 8 8.4 / 9.3, rank 64 14.1 / 14.4; K 1280
+    // rank 8 11.7 / 9.5; fp32 rank 64 K 320 24.0 / 23.7, K 640 28.6 / 24.6.
+    if (few && P.rank > 0 && P.rank * sizeof(TW) <= 128 && P.K <= 640) {
         const dim3 grid((unsigned)tiles, (unsigned)((P.N + columns * kLoraWaves - 1) / (columns * kLoraWaves)));
         auto go = [&](auto k, auto x, auto v) {
             constexpr int KS = decltype(k)::value;
@@ -629,7 +651,7 @@ void launch_lora(Lora P, int64_t M, bool vec) {
         auto with = [&](auto x, auto v) {
             if (P.rank <= 16) go(integral_constant<int, 1>(), x, v);
             else if (P.rank <= 32) go(integral_constant<int, 2>(), x, v);
-            else go(integral_constant<int, 4>(), x, v);
+            else if constexpr (sizeof(TW) == 2) go(integral_constant<int, 4>(), x, v);
         };
         if (vec && bvec) with(T_(), T_());
         else with(F_(), F_());
@@ -666,8 +688,12 @@ void launch_lora(Lora P, int64_t M, bool vec) {
         else if (rt == 2) with(Two());
         else with(Four());
     }
-    for (int j0 = 0; j0 == 0 || j0 < P.rank; j0 += 128) {
-        const int ks = std::min(P.rank - j0, 128);
+    // Ranks of a launch: 128, for whose parts of B and H a wave of few rows has no registers. 48 single rows of 2560 to
+    // 4096 columns, rank 128, us, one launch / two of 64: bf16 35.7 / 30.0, fp32 58 / 52; eight runs of four to 1000
+    // columns 21.7 / 23.5, 40 / 45.
+    const int per = few ? 64 : 128;
+    for (int j0 = 0; j0 == 0 || j0 < P.rank; j0 += per) {
+        const int ks = std::min(P.rank - j0, per);
         const dim3 grid((unsigned)tiles, (unsigned)((P.N + columns * (few ? kLoraWaves : 1) - 1) / (columns * (few ? kLoraWaves : 1))));
         auto go = [&](auto k, auto f, auto v) {
             constexpr int KS = decltype(k)::value;
@@ -687,7 +713,7 @@ void launch_lora(Lora P, int64_t M, bool vec) {
             if (ks <= 16) go(integral_constant<int, 1>(), f, v);
             else if (ks <= 32) go(integral_constant<int, 2>(), f, v);
             else if (ks <= 64) go(integral_constant<int, 4>(), f, v);
-            else go(integral_constant<int, 8>(), f, v);
+            else if constexpr (!decltype(f)::value) go(integral_constant<int, 8>(), f, v);
         };
         if (few) bvec ? with(T_(), T_()) : with(T_(), F_());
         else with(F_(), F_());
