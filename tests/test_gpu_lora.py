@@ -109,6 +109,22 @@ def test_few_rows_of_a_short_k(be, orc, types, N, K, rank):
 
 @gpu
 @pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("rank,r", [(64, 33), (64, 57), (64, 5), (128, 70), (128, 64), (40, 37), (200, 131), (192, 129)])
+@pytest.mark.parametrize("K", [256, 1288])
+def test_ranks_that_do_not_count(be, orc, types, rank, r, K):
+    """NaN in the rows of A and columns of B behind a run's ranks, few and many rows, one launch and several."""
+    for rows in ([1, 3], [90, 170]):
+        c = Case(orc, sum(rows), 300, K, rank, 2, types, seed=270 + rank)
+        runs = np.array([(0, rows[0], 0, r), (rows[0], rows[1], 1, max(1, r - 9))], np.int32)
+        for a, n in ((0, r), (1, max(1, r - 9))):
+            c.A[a, n:] = np.nan
+            c.B[a, :, n:] = np.nan
+        for acc in (True, False):
+            c.check(be, orc, runs, acc, what=f"{types} {rows} rank {r} of {rank} acc={acc}")
+
+
+@gpu
+@pytest.mark.parametrize("types", TYPES)
 @pytest.mark.parametrize("pad", [1, 4, 8])
 def test_strides(be, orc, types, pad):
     for rows in ([40, 90, 3], [1, 1]):
