@@ -259,11 +259,15 @@ class Backend:
     def empty(self, shape) -> DArray:
         return DArray(self, shape)
 
-    def array(self, a: np.ndarray) -> DArray:
-        """float32 and int32 arrays keep their type; uint16 arrays are bf16 bit patterns."""
-        dt = np.asarray(a).dtype if np.asarray(a).dtype in (np.uint16, np.int32) else np.float32
+    def array(self, a: np.ndarray, dtype=None) -> DArray:
+        """float32 unless `dtype` says otherwise; uint16 arrays are bf16 bit patterns and stay so."""
+        dt = dtype or (np.uint16 if np.asarray(a).dtype == np.uint16 else np.float32)
         a = np.ascontiguousarray(a, dtype=dt)
         return DArray(self, a.shape, dtype=dt).upload(a)
+
+    def rows_list(self, a) -> DArray:
+        """The int32 arrays that say which rows are whose (spans, prefixes, segments)."""
+        return self.array(a, np.int32)
 
     def randn(self, shape, seed: int, mean: float = 0.0, std: float = 1.0) -> DArray:
         d = DArray(self, shape)

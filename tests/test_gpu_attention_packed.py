@@ -37,9 +37,9 @@ class Case:
         spans = self.spans if spans is None else spans
         full = np.full(self.q.shape, UNTOUCHED, np.float32)
         out = be.array((full.view(np.uint32) >> 16).astype(np.uint16) if out_bf16 else full)
-        kw = {n: be.array(a) if isinstance(a, np.ndarray) else a for n, a in kw.items()}
+        kw = {n: be.array(a, a.dtype) if isinstance(a, np.ndarray) else a for n, a in kw.items()}
         be.attention_packed(be.array(self.q), be.array(self.k if k is None else k), be.array(self.v if v is None else v),
-                            out, self.Tq, self.Tk, self.heads, self.kv, self.d, be.array(spans), len(spans), self.scale,
+                            out, self.Tq, self.Tk, self.heads, self.kv, self.d, be.rows_list(spans), len(spans), self.scale,
                             out_bf16=out_bf16, **kw)
         got = out.download()
         return bf16_value(got) if out_bf16 else got
@@ -243,7 +243,7 @@ def test_addresses(be, orc, d, lq):
     """Operands at addresses that are multiples of 4 only."""
     c = Case(orc, lq, [60, 33], 2, 2, d, seed=900)
     want, tol = orc.attention_packed(c.q, c.k, c.v, np.zeros(c.q.shape), c.spans, 2, 2, c.scale, causal=True)
-    spans = be.array(c.spans)
+    spans = be.rows_list(c.spans)
     for which in range(4):
         arrays, ptr = [], []
         for i, a in enumerate((c.q, c.k, c.v, np.zeros(c.q.shape, np.float32))):
@@ -293,7 +293,7 @@ def test_offsets_past_32_bits(be, orc, lq):
     be.upload(k.ptr + first * d * 4, c.k)
     be.upload(v.ptr + first * d * 4, c.v)
     out = be.empty(c.q.shape)
-    be.attention_packed(be.array(c.q), k, v, out, lq, Tk, heads, kv, d, be.array(np.array([[0, lq, first, L]], np.int32)), 1,
+    be.attention_packed(be.array(c.q), k, v, out, lq, Tk, heads, kv, d, be.rows_list(np.array([[0, lq, first, L]], np.int32)), 1,
                         c.scale, causal=True)
     want, tol = orc.attention_packed(c.q, c.k, c.v, np.zeros(c.q.shape), c.spans, heads, kv, c.scale, causal=True)
     assert np.all(np.abs(out.download() - want) <= tol)
@@ -304,7 +304,7 @@ def test_offsets_past_32_bits(be, orc, lq):
 def test_captured(be, orc, lq, lk):
     """A captured call replayed with other spans and values, the direct call between the replays."""
     c = Case(orc, lq, lk, 4, 2, 64, seed=1300)
-    q, k, v, out, spans = be.array(c.q), be.array(c.k), be.array(c.v), be.empty(c.q.shape), be.array(c.spans)
+    q, k, v, out, spans = be.array(c.q), be.array(c.k), be.array(c.v), be.empty(c.q.shape), be.rows_list(c.spans)
 
     def call():
         be.attention_packed(q, k, v, out, c.Tq, c.Tk, 4, 2, 64, spans, 2, c.scale, causal=True)
@@ -424,7 +424,7 @@ def test_refusals_of_sizes(kw):
 @gpu
 def test_refusals_of_pointers(be, orc):
     c = Case(orc, [4], [4], 2, 2, 8, seed=1600)
-    q, k, v, out, spans = be.array(c.q), be.array(c.k), be.array(c.v), be.empty(c.q.shape), be.array(c.spans)
+    q, k, v, out, spans = be.array(c.q), be.array(c.k), be.array(c.v), be.empty(c.q.shape), be.rows_list(c.spans)
     more = be.empty((64,))
 
     def refused(**kw):

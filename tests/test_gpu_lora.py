@@ -52,7 +52,7 @@ class Case:
         runs = np.array(runs, np.int32).reshape(-1, 4)
         X, A, B, scale = self.device(be)
         C = be.array(self.c0)
-        self.call(be, X, A, B, scale if scaled else None, be.array(runs), len(runs), C, accumulate)
+        self.call(be, X, A, B, scale if scaled else None, be.rows_list(runs), len(runs), C, accumulate)
         got = C.download()
         self.compare(orc, got, runs, accumulate, scaled, what)
         return got
@@ -148,7 +148,7 @@ def test_addresses(be, orc, types, which):
             flat = np.concatenate((np.zeros(off, np.float32), a.ravel()))
             held.append(be.array(f32_to_bf16(flat) if h else flat))
             ptr.append(held[-1].ptr + off * (2 if h else 4))
-        c.call(be, ptr[0], ptr[1], ptr[2], be.array(c.scale), be.array(runs), len(runs), ptr[3], True)
+        c.call(be, ptr[0], ptr[1], ptr[2], be.array(c.scale), be.rows_list(runs), len(runs), ptr[3], True)
         c.compare(orc, held[3].download()[1 if which == 3 else 0:].reshape(c.c0.shape), runs, what=f"{types} {which}")
 
 
@@ -190,7 +190,7 @@ def test_values_that_are_not_finite_stay_in_their_rows(be, orc, types, rows):
     c.x[rows[0], 3] = np.inf
     X, A, B, scale = c.device(be)
     C = be.array(c.c0)
-    c.call(be, X, A, B, scale, be.array(runs), 2, C, True)
+    c.call(be, X, A, B, scale, be.rows_list(runs), 2, C, True)
     got = C.download()
     for t in range(sum(rows)):
         if t in (0, rows[0]):
@@ -236,7 +236,7 @@ def test_captured(be, orc, rows):
     """Replayed with other runs and rows, the direct call between the replays."""
     c = Case(orc, sum(rows), 512, 256, 16, 3, seed=900)
     X, A, B, scale = c.device(be)
-    C, seg = be.array(c.c0), be.array(np.array(ragged(rows, 3, 16), np.int32))
+    C, seg = be.array(c.c0), be.rows_list(np.array(ragged(rows, 3, 16), np.int32))
     c.call(be, X, A, B, scale, seg, len(rows), C, True)
     be.capture_begin()
     c.call(be, X, A, B, scale, seg, len(rows), C, True)
@@ -270,7 +270,7 @@ def test_two_threads(be, orc):
         X, A, B, scale = c.device(be)
         for _ in range(10):
             C = be.array(c.c0)
-            c.call(be, X, A, B, scale, be.array(np.array(r, np.int32)), len(r), C, True)
+            c.call(be, X, A, B, scale, be.rows_list(np.array(r, np.int32)), len(r), C, True)
             if not np.array_equal(C.download(), want):
                 bad.append(c.M)
 
@@ -287,7 +287,7 @@ def test_beside_a_projection(be, orc):
     runs = np.array(ragged([100, 30], 2, 16), np.int32)
     W = f32_to_bf16(orc.randn((c.N, c.K), 1101, 0.0, 1 / np.sqrt(c.K)))
     X, A, B, scale = c.device(be)
-    dW, seg = be.array(W), be.array(runs)
+    dW, seg = be.array(W), be.rows_list(runs)
     before, after = be.empty((c.M, c.N)), be.empty((c.M, c.N))
     be.gemm_nt_bf16_packed(c.M, c.N, c.K, X, c.K, dW, c.K, after, c.N)
     c.call(be, X, A, B, scale, seg, 2, after, True)
@@ -321,7 +321,7 @@ def test_refusals_of_sizes(name, kw):
 def test_refusals_of_pointers(be, orc):
     c = Case(orc, 6, 16, 8, 4, 2, seed=1200)
     X, A, B, scale = c.device(be)
-    C, seg = be.array(c.c0), be.array(np.array([(0, 6, 0, 4)], np.int32))
+    C, seg = be.array(c.c0), be.rows_list(np.array([(0, 6, 0, 4)], np.int32))
 
     def refused(**kw):
         a = dict(M=6, N=16, K=8, X=X, ldx=8, A=A, B=B, rank=4, adapters=2, scale=scale, segments=seg, count=1, C=C, ldc=16)

@@ -48,8 +48,8 @@ class Layer:
                     "h16": be.array(np.zeros((rows, self.dim), np.uint16)), "q": be.empty((rows, hd)),
                     "k": be.empty((rows, kd)), "v": be.empty((rows, kd)), "a16": be.array(np.zeros((rows, hd), np.uint16)),
                     "cos": be.empty((rows, self.d)), "sin": be.empty((rows, self.d)),
-                    "spans": be.array(np.zeros((requests, 4), np.int32)),
-                    "runs": be.array(np.zeros((requests, 4), np.int32))}
+                    "spans": be.rows_list(np.zeros((requests, 4), np.int32)),
+                    "runs": be.rows_list(np.zeros((requests, 4), np.int32))}
 
     def set(self, x, lens, past):
         """The step's rows, lens[i] of request i behind past[i] keys."""
@@ -197,10 +197,10 @@ be, orc = sdhip.Backend(), Oracle()
 T, heads, d = 200, 4, 64
 q, k, v = (be.array(orc.randn((T, heads * d), i)) for i in range(3))
 out, spans = be.empty((T, heads * d)), np.array([(0, 150, 0, 150), (150, 50, 150, 50)], np.int32)
-dspans = be.array(spans)
+dspans = be.rows_list(spans)
 X, A, B, C = be.array(orc.randn((T, 1280), 4)), orc.randn((2, 8, 1280), 5, 0.0, 0.03), orc.randn((2, 96, 8), 6), be.array(np.zeros((T, 96), np.float32))
 dA, dB, runs = be.array(A), be.array(B), np.array([(0, 150, 0, 8), (150, 50, 1, 8)], np.int32)
-druns = be.array(runs)
+druns = be.rows_list(runs)
 def attend():
     be.attention_packed(q, k, v, out, T, T, heads, heads, d, dspans, 2, 0.125, causal=True)
 def adapt():
