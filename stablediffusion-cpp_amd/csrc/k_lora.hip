@@ -13,7 +13,7 @@
 //
 // Bound by memory for many rows: X is read once (a workgroup has all ranks of its rows), C
 // read and written once, while A, B and H come from the L2s. [12528,3840] bf16 to 10240
-// columns, rank 64: 137 us, 4.5 TB/s (down 29, up 104; a kernel that only writes C takes
+// columns, rank 64: 137 us, 4.5 TB/s (down 27, up 106; a kernel that only writes C takes
 // 77); [8192,640] to 5120, fp32, rank 12: 78 us, 4.0 TB/s; 48 single rows of 2560 to 4096
 // columns, rank 16: 10.4 us, the two launches' own length.
 #include <algorithm>
@@ -144,7 +144,7 @@ constexpr int kDownBlock = 128 / sizeof(TX);
 
 // A wave's 32 rows of `BLOCK` values as they are loaded, neighbouring lanes along a row, and their way
 // through the wave's 4 KB of LDS into MFMA operands. Loaded as operands, 16 bytes of each of 32 rows an
-// instruction, a line came to the L1 four times, and three of those went on to the L2: 47 us, STAGED 34, for
+// instruction, a line came to the L1 four times, and three of those went on to the L2: 47 us, STAGED 27, for
 // [12528,3840] bf16 to 64 ranks.
 template <class T, int BLOCK>
 struct Staged {
