@@ -8,7 +8,9 @@ array which rows are whose. Two operators work on such tensors:
   lora        sdhip.Backend.lora_nt_*: C += scale_a (X A_a^T) B_a^T, each run of rows with the adapter a of its own
               request, beside a projection that all of them share.
 
-With own false, run() computes them from elementary torch operations in fp32; with own true it calls the library.
+With own false, run() computes them from elementary torch operations in fp32; with own true it calls the library,
+which works on a stream of its own: prepare() returns once the inputs are there, and a program waits for the device
+(torch.cuda.synchronize(), Backend.synchronize()) before torch reads what run() returned.
 listed() and draw() give the cases, prepare() what a program has in hand, work() what a pass has to move and compute,
 exact() the results in 64 bits.
 """
@@ -165,6 +167,7 @@ def prepare(case, seed):
         st["scale"] = torch.rand(n, generator=g, device="cuda") + 0.5
         st["segments"] = ints(seg)
         st["y"] = randn(M, N) if c["accumulate"] else torch.zeros(M, N, device="cuda")
+        torch.cuda.synchronize()  # the library works on a stream of its own
         return st
     q, k, Tq, Tk, _ = _rows(c)
     h, kv, d = c["heads"], c["kv_heads"], c["d"]
@@ -173,6 +176,7 @@ def prepare(case, seed):
     st["prefix"] = ints(_prefixes(c)) if c["prefix"] else None
     st["bias"] = randn(h, 2 * c["radius"] + 1) if c["radius"] else None
     st["out"] = torch.zeros(Tq, h * d, device="cuda", dtype=torch.bfloat16 if c["out_bf16"] else torch.float32)
+    torch.cuda.synchronize()
     return st
 
 
