@@ -400,12 +400,18 @@ class Oracle:
         """float64 definition of sdh_attention_packed. Returns the result (rows of no
         sequence as in `out`) and a bound for its fp32 evaluation, per value.
 
+        A bias of -inf hides its key, and a key whose score is -inf (an infinity in q or
+        k) has no weight: neither counts, whatever it holds. A score that is NaN or +inf
+        makes its row NaN. Infinities and NaN among the values of the keys that count
+        show in their columns, however small the weight.
+
         The bound: a score is off by at most (d + 48) 2^-24 sum|q k| scale (its d
         fp32 sums; the operands held to 2^-22, three roundings of the scaled score)
         + 8 2^-24 (cap + |x|) (tanh to 5 2^-24 of itself, the bias' sum), the exponent
         by 2^-24 |x| of that again; softmax turns a score error e into at most 2 e per
         weight, and the weighted sum adds (keys + 64) 2^-24 sum p|v| (weights and
-        values held to 2^-21)."""
+        values held to 2^-21). Values are held to 2^-30 of the largest of their key,
+        and weighted ones to 2^-27 of the largest weighted one."""
         plant = getattr(self, "_plant_py", 0)
         q, k, v = (np.asarray(a, np.float32) for a in (q, k, v))
         d = q.shape[1] // heads
@@ -434,29 +440,43 @@ class Oracle:
                     if not len(js):
                         continue
                     g = h // (heads // kv_heads)
-                    kk = k[k0 + js, g * d:g * d + d].astype(np.float64)
-                    vv = v[k0 + js, g * d:g * d + d].astype(np.float64)
+                    b = bias[h, np.clip(js - p, -radius, radius) + radius].astype(np.float64) if bias is not None else np.zeros(len(js))
+                    seen, b = js[b != -np.inf], b[b != -np.inf]
+                    kk = k[k0 + seen, g * d:g * d + d].astype(np.float64)
+                    vv = v[k0 + seen, g * d:g * d + d].astype(np.float64)
                     qq = q[row, c].astype(np.float64)
-                    x = kk @ qq * scale
-                    e = (d + 48) * u * (np.abs(kk) @ np.abs(qq)) * abs(scale)
-                    if bias is not None and plant == 23:  # planted: the bias inside the cap
-                        x = x + bias[h, np.clip(js - p, -radius, radius) + radius]
+                    with np.errstate(invalid="ignore"):
+                        x = (kk * qq).sum(1) * scale
+                        e = (d + 48) * u * (np.abs(kk) * np.abs(qq)).sum(1) * abs(scale)
+                    e = np.where(np.isfinite(x), e, 0.0)
+                    if plant == 23:  # planted: the bias inside the cap
+                        x = x + b
                     if cap:
                         x = cap * np.tanh(x / cap)
-                    if bias is not None and plant != 23:
-                        x = x + bias[h, np.clip(js - p, -radius, radius) + radius].astype(np.float64)
-                    if np.all(x == -np.inf):
+                    if plant != 23:
+                        x = x + b
+                    some = x != -np.inf
+                    x, e, vv = x[some], e[some], vv[some]
+                    if not len(x):
                         continue
-                    e = e + 9 * u * (cap + np.where(np.isfinite(x), np.abs(x), 0))
+                    if np.any(np.isnan(x)) or x.max() == np.inf:
+                        want[row, c] = np.nan
+                        continue
+                    e = e + 9 * u * (cap + np.abs(x))
                     low = np.finfo(np.float32).min  # sums with the lowest value are taken in fp32: they stay there
-                    x = np.where((x < low / 2) & (x > -np.inf), low, x)
+                    x = np.where(x < low / 2, low, x)
                     w = np.exp(x - x.max())
                     w = w / w.sum()
                     near = np.max(e[w > 1e-30])
                     if x.max() == low:
                         near = 0.0
-                    want[row, c] = w @ vv
-                    tol[row, c] = (2 * near + (len(js) + 64) * u) * (w @ np.abs(vv))
+                    finite = np.isfinite(vv)
+                    vz, rest = np.where(finite, vv, 0.0), np.where(finite, 0.0, vv)
+                    weighted = w * np.abs(vz).max(1)
+                    with np.errstate(invalid="ignore"):
+                        want[row, c] = w @ vz + rest.sum(0)
+                    tol[row, c] = ((2 * near + (len(js) + 64) * u) * (w @ np.abs(vz)) + 2.0 ** -30 * weighted.sum()
+                                   + len(js) * 2.0 ** -27 * weighted.max())
         return want, tol
 
     # -- low-rank adapters (no reference counterpart) --
