@@ -157,12 +157,15 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_attn_packed_rows(Packed P) {
 // Operands are fp16 pairs hi + lo in block floating point, products hi hi + hi lo +
 // lo hi with fp32 sums (2^-21 of each product). A block is a row of q, or a tile of k or
 // v: scaled by 2^-e to at most 2^14, a score is s 2^(e_q + e_k), and a weight is formed as
-// p 2^(14 + e_v - E), E the largest e_v that the lane's row has met, so that the sums of
-// all tiles share the scale 2^(14 - E). The pair holds 22 bits down to 2^-16 of its
-// block's largest value.
-//   A key that a row does not see must not cost it bits: a tile whose keys are more than
-// 2^kSpread apart has an exponent for each key, and a row leaves E to the keys that it
-// sees. Values that are not finite go into the tiles as zeros, since 0 * inf would reach
+// p 2^(14 + e_v - E), so that the sums of all tiles share the scale 2^(14 - E). The pair
+// holds 22 bits down to 2^-16 of its block's largest value.
+//   E goes by the weighted values: the largest log2(p) + e_v of a row's tiles, p relative to
+// the row's reference, with which E sinks as the reference rises. A value that is large but
+// has no weight, hidden or far below in score, then costs the others nothing, and the largest
+// that has weight is near 2^28 in its sum. A tile whose values are more than 2^kSpread apart, or
+// have rows of zeros among them, has an exponent for each key: p 2^e_v of the tile says nothing
+// there about any one key. (Of its keys as well, whose largest need not be one that a row sees.)
+// Values that are not finite go into the tiles as zeros, since 0 * inf would reach
 // the rows that do not see them, and are added at the end; a key that is not finite makes
 // the scores of the rows that see it NaN, and only those.
 //
@@ -195,9 +198,9 @@ constexpr float kLazy = 1.5f;
 // tile's 64 keys reach past the radius unless all of them are beyond it: no index is held to the radius
 // (ten instructions a score; the rows and tiles at the band's edges took half the softmax' time).
 constexpr int kBiasPad = 96;
-constexpr int kUnsetE = -1000;  // no values seen yet
+constexpr int kUnsetE = -2000;  // no weighted values yet, or next to nothing beside the reference
 constexpr int kSpread = 8;
-constexpr int kFarE = -40;      // weights' exponents relative to E are not taken below this (2^-40 of the largest sum)
+constexpr int kFarE = -40;      // a tile whose exponent is below E by more adds nothing: 2^-40 of the row's largest weighted value a key
 
 __device__ __forceinline__ int swz_v(int r) { return (r >> 1) & 7; }
 template <int DP>
@@ -341,7 +344,7 @@ __global__ __launch_bounds__(64 * kSplitWaves) void k_attn_packed_split(Packed P
         if (ktop[u] && abs((kmost >> 23) - (ktop[u] >> 23)) > kSpread) flag |= kKeyExps;
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-        if (vtop[i] && (vmost >> 23) - (vtop[i] >> 23) > kSpread) flag |= kValueExps;
+        if (j0 + i < P.Tk && (vmost >> 23) - (vtop[i] >> 23) > kSpread) flag |= kValueExps;
     flag = (__ballot(flag & kKeyExps) ? kKeyExps : 0) | (__ballot(flag & kValueExps) ? kValueExps : 0) | (__ballot(flag & kNotFinite) ? kNotFinite : 0);
     if (lane == 0) flags[w] = flag;
     __syncthreads();
@@ -586,8 +589,6 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
     auto softmax = [&](int k0, int tile, int tile_ek, int tile_ev, int flag) __attribute__((always_inline)) {
         const int* exps = X.exps + ((int64_t)kh * X.n + tile) * 2 * kKT;
         const bool edge = !((k0 >= 0 && k0 + kKT <= pre) || (k0 >= last_lo && k0 + kKT <= first_hi));  // of this wave
-        int emax = tile_ev;
-        if (edge && !((k0 < pre && k0 + kKT > 0) || (k0 < see.hi && k0 + kKT > see.lo))) emax = kUnsetE;
         // kept normal: -inf stays -inf, zero zero
         const float ct = fminf(fmaxf(ldexpf(scale, eq + (flag & kKeyExps ? 0 : tile_ek)), 1.17549435e-38f), 3.40282347e38f);
         if (flag & kKeyExps) {
@@ -595,15 +596,6 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
             for (int u = 0; u < 4; ++u)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) s[u >> 1][(u & 1) * 8 + i] = ldexpf(s[u >> 1][(u & 1) * 8 + i], exps[u * 16 + fh * 8 + i]);
-        }
-        if (flag & kValueExps) {
-            emax = kUnsetE;
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (visible(k0 + u * 16 + fh * 8 + i)) emax = max(emax, exps[kKT + u * 16 + fh * 8 + i]);
-            emax = max(emax, __shfl_xor(emax, 32, 64));
         }
         float unit = ct;  // of x
         if constexpr (EXTRA) {
@@ -699,39 +691,70 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
         mt *= unit;
         mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
         const float mnew = mt > m + (EXTRA ? kLazy / kLog2e : kLazy) ? mt : m;
-        float alpha = 1.0f;
-        if (mnew != m) alpha = __builtin_amdgcn_exp2f(EXTRA ? (m - mnew) * kLog2e : m - mnew);
+        float alpha = 1.0f, ao = 1.0f;  // of the sum of weights, of o
+        if (mnew != m) {
+            const float rise = EXTRA ? (mnew - m) * kLog2e : mnew - m;
+            const float whole = fminf(floorf(rise), 1024.0f);  // taken off E, the rest off o
+            ao = __builtin_amdgcn_exp2f(whole - rise);
+            alpha = ldexpf(ao, -(int)whole);
+            E = max(E - (int)whole, kUnsetE);
+        }
         m = mnew;
         const float ref = m == -INFINITY ? 0.f : m;
-        float ao = alpha;
-        if (emax > E) {
-            const int up = min(emax + 1, 126);  // a little ahead: the next tiles' are alike
-            ao = E == kUnsetE ? 0.f : ldexpf(alpha, max(E - up, -300));
-            E = up;
-        }
-        const int by = 14 + (flag & kValueExps ? 0 : max(tile_ev - E, kFarE));
-        float total = 0.f;
-        // A reference far out (biases of the type's lowest value) is taken off before the product,
-        // which would overflow.
-        if (EXTRA && __ballot(!(fabsf(ref) < 1e4f))) {
+        float most;  // log2 of the tile's largest weighted value
+        if (flag & kValueExps) {  // scores to log2 units above the reference
+            most = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) s[i >> 4][i & 15] = __builtin_amdgcn_exp2f(fmaf(fmaf(s[i >> 4][i & 15], unit, -ref), kLog2e, (float)by));
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float x = fmaf(s[u >> 1][(u & 1) * 8 + i], unit, -ref) * (EXTRA ? kLog2e : 1.0f);
+                    s[u >> 1][(u & 1) * 8 + i] = x;
+                    most = fmaxf(most, x + (float)exps[kKT + u * 16 + fh * 8 + i]);
+                    few(i);
+                }
+            most = fmaxf(most, __shfl_xor(most, 32, 64));
         } else {
-            const float f = EXTRA ? unit * kLog2e : unit, up = (float)by - (EXTRA ? ref * kLog2e : ref);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) s[i >> 4][i & 15] = __builtin_amdgcn_exp2f(fmaf(s[i >> 4][i & 15], f, up));
+            most = fminf(EXTRA ? (mt - ref) * kLog2e : mt - ref, 0.0f) + (float)tile_ev;
         }
-#pragma unroll
-        for (int i = 0; i < 32; ++i) total += s[i >> 4][i & 15];
-        asm volatile("" : "+v"(total));  // not behind the branch below, for which the weights would be copied
-        sum = fmaf(sum, alpha, ldexpf(total, -by));
+        const int need = (int)fmaxf(ceilf(most), 2.0f * kUnsetE);
+        if (need > E) {
+            ao = ldexpf(ao, max(E - need - 1, -300));
+            E = need + 1;  // a little ahead: the next tiles' are alike
+        }
+        float total = 0.f;
         if (flag & kValueExps) {
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
-                for (int i = 0; i < 8; ++i)  // an unseen key's weight is zero, its exponent may be above E
-                    s[u >> 1][(u & 1) * 8 + i] =
-                        ldexpf(s[u >> 1][(u & 1) * 8 + i], min(max(exps[kKT + u * 16 + fh * 8 + i] - E, kFarE), 0));
+                for (int i = 0; i < 8; ++i) {
+                    const float x = s[u >> 1][(u & 1) * 8 + i];
+                    total += __builtin_amdgcn_exp2f(x);
+                    s[u >> 1][(u & 1) * 8 + i] = __builtin_amdgcn_exp2f(x + (float)(14 + exps[kKT + u * 16 + fh * 8 + i] - E));
+                    few(i);
+                }
+            sum = fmaf(sum, alpha, total);
+        } else {
+            const int above = tile_ev - E, by = 14 + max(above, kFarE);
+            // A reference far out (biases of the type's lowest value) is taken off before the product,
+            // which would overflow.
+            if (EXTRA && __ballot(!(fabsf(ref) < 1e4f))) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) s[i >> 4][i & 15] = __builtin_amdgcn_exp2f(fmaf(fmaf(s[i >> 4][i & 15], unit, -ref), kLog2e, (float)by));
+            } else {
+                const float f = EXTRA ? unit * kLog2e : unit, up = (float)by - (EXTRA ? ref * kLog2e : ref);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) s[i >> 4][i & 15] = __builtin_amdgcn_exp2f(fmaf(s[i >> 4][i & 15], f, up));
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) total += s[i >> 4][i & 15];
+            asm volatile("" : "+v"(total));  // not behind the branch below, for which the weights would be copied
+            sum = fmaf(sum, alpha, ldexpf(total, -by));
+            if (__ballot(above < kFarE)) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (above < kFarE) s[i >> 4][i & 15] = 0.f;
+            }
         }
         if (__ballot(ao != 1.0f)) {
 #pragma unroll

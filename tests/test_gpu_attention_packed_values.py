@@ -1,0 +1,89 @@
+"""GPU tests of attention over packed sequences at unlike, infinite and undefined values
+against its float64 definition (Oracle.attention_packed): keys that are hidden or have no
+weight whatever they hold, channels and values of very unlike size, infinities that are
+seen, results near fp32's least, and keys cut into several parts."""
+import numpy as np
+import pytest
+
+from test_gpu_attention_packed import MASKS, UNTOUCHED, Case, masks
+
+gpu = pytest.mark.gpu
+
+# Forty rows go in tiles (up to 128 dims), one and three in the few rows' kernel, 160 dims and more by rows.
+SHAPES = [([40], 64), ([40], 128), ([1], 64), ([3], 128), ([1], 40), ([40], 96), ([2], 160)]
+
+
+def held(c, be, orc, what="", out_bf16=False, **kw):
+    """The library's result within the definition's bound; NaN and infinities where the definition has them."""
+    got = c.run(be, out_bf16=out_bf16, **kw)
+    want, tol = orc.attention_packed(c.q, c.k, c.v, np.full(c.q.shape, UNTOUCHED), c.spans, c.heads, c.kv, c.scale, **kw)
+    if out_bf16:
+        with np.errstate(invalid="ignore"):
+            tol = tol + 2.0 ** -8 * (np.abs(want) + tol) * (tol > 0)
+    fin = np.isfinite(want)
+    assert np.array_equal(np.isnan(got), np.isnan(want)), f"{what}: NaN at {np.argwhere(np.isnan(got) != np.isnan(want))[0]}"
+    inf = np.isinf(want)
+    assert np.array_equal(got[inf], want[inf]), f"{what}: infinities"
+    over = np.abs(got[fin].astype(np.float64) - want[fin]) - tol[fin]
+    assert np.max(over, initial=0) <= 0, (f"{what}: {np.max(over):.3e} beyond the bound at {np.argwhere(fin)[np.argmax(over)]}, "
+                                          f"bound {tol[fin][np.argmax(over)]:.3e}")
+    return got
+
+
+# ------------------------------------------------- values of keys without weight
+@gpu
+@pytest.mark.parametrize("big", [1e6, 1e10, 1e20, 1e30])
+@pytest.mark.parametrize("lq,d", SHAPES)
+def test_large_values_that_a_bias_hides(be, orc, lq, d, big):
+    """The last 40 of 150 keys' rows do not see the first 50 keys, some of whose values are large."""
+    c = Case(orc, lq, [150], 4, 2, d, seed=2000)
+    c.v[[3, 20, 33, 44]] *= np.float32(big)
+    bias = orc.randn((4, 301), 2001)
+    bias[:, :91] = -np.inf
+    held(c, be, orc, f"{big}", bias=bias, radius=150)
+    held(c, be, orc, f"{big} causal", bias=bias, radius=150, causal=True)
+    c.k[[3, 20, 33, 44]] *= np.float32(big)
+    held(c, be, orc, f"{big} with their keys", bias=bias, radius=150)
+
+
+@gpu
+@pytest.mark.parametrize("depth", [20.0, 30.0, 60.0])
+@pytest.mark.parametrize("big", [1e6, 1e10, 1e30])
+@pytest.mark.parametrize("lq,d", SHAPES)
+def test_large_values_of_little_weight(be, orc, lq, d, big, depth):
+    """A key whose score lies 20 to 60 below the others', with a large value, alone in its tile or among others."""
+    for place in ([20], [100], [20, 21, 100]):
+        c = Case(orc, lq, [150], 2, 1, d, seed=2100)
+        c.q[:, ::d] = 8.0
+        c.k[place, 0] = -depth / (8.0 * c.scale)
+        c.v[place] *= np.float32(big)
+        held(c, be, orc, f"{place}")
+        held(c, be, orc, f"{place} cap", cap=100.0)
+        held(c, be, orc, f"{place} bias", bias=orc.randn((2, 61), 2101), radius=30)
+
+
+@gpu
+@pytest.mark.parametrize("lq,d", SHAPES)
+def test_the_heaviest_key_has_no_value(be, orc, lq, d):
+    """What is left of the others is theirs to the same number of bits."""
+    for depth in (5.0, 20.0, 50.0):
+        for value in (0.0, 1e-30):
+            c = Case(orc, lq, [150], 2, 1, d, seed=2200)
+            c.q[:, ::d] = 8.0
+            c.k[70, 0] = depth / (8.0 * c.scale)
+            c.v[70] *= np.float32(value)
+            held(c, be, orc, f"{depth} {value}")
+
+
+@gpu
+@pytest.mark.parametrize("lq,d", SHAPES)
+def test_values_that_grow_as_scores_fall(be, orc, lq, d):
+    """All keys give alike shares: values from 1 to 2^90 against scores that fall as fast, in either order of keys."""
+    for step in (1, -1):
+        c = Case(orc, lq, [150], 2, 1, d, seed=2300)
+        n = np.arange(150)[::step] * (60.0 / 150)
+        c.q[:, ::d] = 8.0
+        c.k[:, 0] = -n / (8.0 * c.scale)
+        c.v *= np.exp(n).astype(np.float32)[:, None]
+        held(c, be, orc, f"{step}")
+        held(c, be, orc, f"{step} causal", causal=True)
