@@ -842,7 +842,7 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
     if (r >= rows) return;
     sum += __shfl_xor(sum, 32, 64);
     // a part of the keys: the sums as they are, on the scale of the reference
-    const float inv = sum == 0.f ? 0.f : ldexpf(S.n > 1 ? 1.0f : 1.0f / sum, E - 14);
+    const float inv = sum == 0.f ? 0.f : S.n > 1 ? 1.0f : 1.0f / sum;
     for (int n = bad_first; n <= bad_last; ++n)
         for (int j = max(tile_of(n) * kKT - T.z, 0), end = min(tile_of(n) * kKT - T.z + kKT, lk); j < end; ++j) {
             if (!visible(j)) continue;
@@ -863,7 +863,9 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
         for (int g = 0; g < 4; ++g) {
             const int c = dt * 32 + g * 8 + fh * 4;
             if (c >= d) continue;
-            const f4 v = {o[dt][g * 4] * inv, o[dt][g * 4 + 1] * inv, o[dt][g * 4 + 2] * inv, o[dt][g * 4 + 3] * inv};
+            f4 v;  // two steps: 2^(E - 14) / sum may be subnormal where the results are not
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = ldexpf(o[dt][g * 4 + e] * inv, E - 14);
             if (S.n > 1) {
                 *(f4*)(S.o + cell * S.stride + c) = v;
             } else if constexpr (VEC) {

@@ -87,3 +87,14 @@ def test_values_that_grow_as_scores_fall(be, orc, lq, d):
         c.v *= np.exp(n).astype(np.float32)[:, None]
         held(c, be, orc, f"{step}")
         held(c, be, orc, f"{step} causal", causal=True)
+
+
+@gpu
+@pytest.mark.parametrize("power", [-60, -100, -110, -116, 60, 100])
+@pytest.mark.parametrize("lq,d", SHAPES)
+def test_powers_of_two(be, orc, lq, d, power):
+    """Values near fp32's least and largest."""
+    c = Case(orc, lq, [150], 2, 1, d, seed=2400)
+    c.v = (c.v * np.float64(2.0 ** power)).astype(np.float32)
+    held(c, be, orc, f"2^{power}")
+    held(c, be, orc, f"2^{power} causal", causal=True)
