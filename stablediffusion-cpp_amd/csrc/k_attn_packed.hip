@@ -166,8 +166,9 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_attn_packed_rows(Packed P) {
 // have rows of zeros among them, has an exponent for each key: p 2^e_v of the tile says nothing
 // there about any one key. (Of its keys as well, whose largest need not be one that a row sees.)
 // Values that are not finite go into the tiles as zeros, since 0 * inf would reach
-// the rows that do not see them, and are added at the end; a key that is not finite makes
-// the scores of the rows that see it NaN, and only those.
+// the rows that do not see them, and are added at the end. An infinity in q or k would be
+// inf - inf in a pair: a wave one of whose rows sees such a key, or has such a query, takes the
+// tile's scores in fp32 (fp32_scores).
 //
 // S^T = K Q^T and O^T = V^T P^T by v_mfma_f32_32x32x16_f16: lane l holds row l % 32 of
 // the wave in both, its statistics are its own. K's rows are ordered so that the eight
@@ -198,9 +199,12 @@ constexpr float kLazy = 1.5f;
 // tile's 64 keys reach past the radius unless all of them are beyond it: no index is held to the radius
 // (ten instructions a score; the rows and tiles at the band's edges took half the softmax' time).
 constexpr int kBiasPad = 96;
+constexpr int kBadKey = 1000;   // the exponent of a key that is not finite
 constexpr int kUnsetE = -2000;  // no weighted values yet, or next to nothing beside the reference
 constexpr int kSpread = 8;
-constexpr int kFarE = -40;      // a tile whose exponent is below E by more adds nothing: 2^-40 of the row's largest weighted value a key
+// A tile's weights are scaled by no less than this, which keeps their sum in range. At that scale they are below 2^(14 + kLazy - 42),
+// less than half of fp16's least: the pairs are zero, as they are to be, since the tile's values are below 2^-42 of the largest.
+constexpr int kFarE = -42;
 
 __device__ __forceinline__ int swz_v(int r) { return (r >> 1) & 7; }
 template <int DP>
@@ -341,7 +345,7 @@ __global__ __launch_bounds__(64 * kSplitWaves) void k_attn_packed_split(Packed P
     vmost = max(max(tops[1][0], tops[1][1]), max(tops[1][2], tops[1][3]));
 #pragma unroll
     for (int u = 0; u < KU; ++u)
-        if (ktop[u] && abs((kmost >> 23) - (ktop[u] >> 23)) > kSpread) flag |= kKeyExps;
+        if (ktop[u] >= kInfBits || (ktop[u] && abs((kmost >> 23) - (ktop[u] >> 23)) > kSpread)) flag |= kKeyExps;
 #pragma unroll
     for (int i = 0; i < 16; ++i)
         if (j0 + i < P.Tk && (vmost >> 23) - (vtop[i] >> 23) > kSpread) flag |= kValueExps;
@@ -357,7 +361,7 @@ __global__ __launch_bounds__(64 * kSplitWaves) void k_attn_packed_split(Packed P
 #pragma unroll
     for (int u = 0; u < KU; ++u) {
         const int key = w * 16 + u * KROWS + krow, e = flag & kKeyExps ? block_exp(ktop[u]) : ek;
-        if ((flag & kKeyExps) && kch == 0) exps[key] = e;
+        if ((flag & kKeyExps) && kch == 0) exps[key] = ktop[u] >= kInfBits ? kBadKey : e;
         const float sc = pow2(-e);
         h8 hi, lo;
 #pragma unroll
@@ -416,6 +420,7 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
     // Rows of K, hi and lo, of two tiles, and of V^T. Objects of their own, so that the compiler
     // knows which copy a read has to wait for.
     __shared__ __attribute__((aligned(1024))) u16 kbuf0[2 * PART], kbuf1[2 * PART], vbuf0[2 * PART], vbuf1[2 * PART];
+    __shared__ int odd_waves[WAVES];
     extern __shared__ float biases[];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int fr = lane & 31, fh = lane >> 5;
@@ -433,7 +438,7 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
     // 500 to 1000 125 / 118, eight of 250 to 500 77 / 79.
     if (P.causal) T.row0 = (T.rows * group - 1) / kTileRows * kTileRows - T.row0;
     const int d = P.d, rows = T.rows * group, lk = T.w, pre = P.prefix ? min(max(P.prefix[T.index], 0), lk) : 0;
-    const int64_t inner = (int64_t)P.heads * d, kv_inner = (int64_t)P.kv_heads * d;
+    const int64_t inner = (int64_t)P.heads * d;
     const int r = T.row0 + w * 32 + fr;
     const int rc = min(r, rows - 1), qi = rc / group, h = kh * group + (rc - qi * group);
     const int shift = lk - T.rows;
@@ -517,6 +522,7 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
     }
     h8 qh[DS], ql[DS];
     int eq;
+    bool bad_q;
     {
         int top = 0;
 #pragma unroll
@@ -525,6 +531,7 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
             for (int e = 0; e < 8; ++e) top = max(top, abs_bits(qx[ds][e]));
         top = max(top, __shfl_xor(top, 32, 64));
         eq = block_exp(top);
+        bad_q = top >= kInfBits;
         const float sc = copysignf(pow2(-eq), P.scale);  // a negative scale turns q's sign
 #pragma unroll
         for (int ds = 0; ds < DS; ++ds)
@@ -584,25 +591,78 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
     auto few = [](int i) __attribute__((always_inline)) {
         if (i % 8 == 7) __builtin_amdgcn_sched_barrier(0);
     };
+    // P for code that hardly ever runs, read from the kernel's arguments there: kept in registers it would push others out.
+    auto args = []() __attribute__((always_inline)) {
+        auto R = (const __attribute__((address_space(4))) Packed*)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(R));
+        return R;
+    };
+    auto hidden = [&](auto R, int j) {  // by a bias of -inf
+        return EXTRA && R->bias && R->bias[(int64_t)h * (2 * R->radius + 1) + R->radius + min(max(j - p, -R->radius), R->radius)] == -INFINITY;
+    };
+    // s = scale q.k of a tile, whatever q and k hold, -inf where a bias hides the key. Eight keys at a time, in
+    // little code: it stands twice in a loop that is to stay in the instruction cache.
+    auto fp32_scores = [&](int k0) __attribute__((always_inline)) {
+        const auto R = args();
+        const int d = R->d;
+        const int64_t kv_inner = (int64_t)R->kv_heads * d;
+        const float *qr = R->q + ((int64_t)(T.first + qi) * R->heads + h) * d, *kr = R->k + T.z * kv_inner + (int64_t)kh * d;
+#pragma unroll 1
+        for (int u = 0; u < 4; ++u) {
+            const int j = k0 + u * 16 + fh * 8;
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = 0.f;
+#pragma unroll 1
+            for (int c = 0; c < d; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = fmaf(qr[c], kr[min(max(j + i, 0), lk - 1) * kv_inner + c], x[i]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = hidden(R, j + i) ? -INFINITY : x[i] * R->scale;
+#pragma unroll
+                for (int to = 0; to < 4; ++to)
+                    if (u == to) s[to >> 1][(to & 1) * 8 + i] = x[i];
+            }
+        }
+    };
     // s -> weights in place, the statistics and the scale of o brought up to date. k0: the
-    // sequence's key at the tile's first row (below zero in front of the sequence).
-    auto softmax = [&](int k0, int tile, int tile_ek, int tile_ev, int flag) __attribute__((always_inline)) {
+    // sequence's key at the tile's first row (below zero in front of the sequence). `odd`: what the
+    // first loop leaves to the second.
+    auto softmax = [&](auto odd, int k0, int tile, int tile_ek, int tile_ev, int flag) __attribute__((always_inline)) {
+        constexpr bool ODD = decltype(odd)::value;
         const int* exps = X.exps + ((int64_t)kh * X.n + tile) * 2 * kKT;
         const bool edge = !((k0 >= 0 && k0 + kKT <= pre) || (k0 >= last_lo && k0 + kKT <= first_hi));  // of this wave
-        // kept normal: -inf stays -inf, zero zero
-        const float ct = fminf(fmaxf(ldexpf(scale, eq + (flag & kKeyExps ? 0 : tile_ek)), 1.17549435e-38f), 3.40282347e38f);
-        if (flag & kKeyExps) {
+        int ek = tile_ek;
+        bool bad = bad_q;
+        if (ODD && (flag & kKeyExps)) {
+            ek = -126;
+#pragma unroll 1
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int e = exps[u * 16 + fh * 8 + i];
+                    ek = max(ek, visible(k0 + u * 16 + fh * 8 + i) ? e : -126);
+                }
+            ek = max(ek, __shfl_xor(ek, 32, 64));
+            bad |= ek == kBadKey;
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) s[u >> 1][(u & 1) * 8 + i] = ldexpf(s[u >> 1][(u & 1) * 8 + i], exps[u * 16 + fh * 8 + i]);
+                for (int i = 0; i < 8; ++i)  // an unseen key's may be larger
+                    s[u >> 1][(u & 1) * 8 + i] = ldexpf(s[u >> 1][(u & 1) * 8 + i], min(exps[u * 16 + fh * 8 + i] - ek, 0));
         }
-        float unit = ct;  // of x
+        // kept normal: -inf stays -inf, zero zero
+        float unit = fminf(fmaxf(ldexpf(scale, eq + ek), 1.17549435e-38f), 3.40282347e38f);  // of s
+        if (ODD && __ballot(bad)) {
+            fp32_scores(k0);
+            unit = EXTRA ? 1.0f : kLog2e;
+        }
         if constexpr (EXTRA) {
             const float* near = biases + (h - kh * group) * row_of_bias + kBiasPad + P.radius;
             const float* bp = P.bias + (int64_t)h * (2 * P.radius + 1) + P.radius;
             if (P.cap > 0.f) {
-                const float in = fminf(ct / P.cap, 3.40282347e38f);
+                const float in = fminf(unit / P.cap, 3.40282347e38f);
                 float top = 0.f;
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
@@ -701,61 +761,48 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
         }
         m = mnew;
         const float ref = m == -INFINITY ? 0.f : m;
-        float most;  // log2 of the tile's largest weighted value
-        if (flag & kValueExps) {  // scores to log2 units above the reference
+        float f = EXTRA ? unit * kLog2e : unit, off = EXTRA ? ref * kLog2e : ref;
+        float most, total = 0.f;  // log2 of the tile's largest weighted value, the sum of its weights
+        const bool own = ODD && (flag & kValueExps);
+        if (own) {  // s to log2 units above the reference, with the key's exponent
             most = -INFINITY;
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float x = fmaf(s[u >> 1][(u & 1) * 8 + i], unit, -ref) * (EXTRA ? kLog2e : 1.0f);
-                    s[u >> 1][(u & 1) * 8 + i] = x;
-                    most = fmaxf(most, x + (float)exps[kKT + u * 16 + fh * 8 + i]);
+                    total += __builtin_amdgcn_exp2f(x);
+                    s[u >> 1][(u & 1) * 8 + i] = x + (float)(exps[kKT + u * 16 + fh * 8 + i] - tile_ev);
+                    most = fmaxf(most, s[u >> 1][(u & 1) * 8 + i]);
                     few(i);
                 }
             most = fmaxf(most, __shfl_xor(most, 32, 64));
+            f = 1.0f, off = 0.f;
         } else {
-            most = fminf(EXTRA ? (mt - ref) * kLog2e : mt - ref, 0.0f) + (float)tile_ev;
+            most = fminf(EXTRA ? (mt - ref) * kLog2e : mt - ref, 0.0f);
         }
-        const int need = (int)fmaxf(ceilf(most), 2.0f * kUnsetE);
+        const int need = (int)fmaxf(ceilf(most), 2.0f * kUnsetE) + tile_ev;
         if (need > E) {
             ao = ldexpf(ao, max(E - need - 1, -300));
             E = need + 1;  // a little ahead: the next tiles' are alike
         }
-        float total = 0.f;
-        if (flag & kValueExps) {
+        const int above = tile_ev - E, by = 14 + (own ? above : max(above, kFarE));
+        float weights = 0.f;
+        // A reference far out (biases of the type's lowest value) is taken off before the product,
+        // which would overflow.
+        if (EXTRA && !own && __ballot(!(fabsf(ref) < 1e4f))) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float x = s[u >> 1][(u & 1) * 8 + i];
-                    total += __builtin_amdgcn_exp2f(x);
-                    s[u >> 1][(u & 1) * 8 + i] = __builtin_amdgcn_exp2f(x + (float)(14 + exps[kKT + u * 16 + fh * 8 + i] - E));
-                    few(i);
-                }
-            sum = fmaf(sum, alpha, total);
+            for (int i = 0; i < 32; ++i) s[i >> 4][i & 15] = __builtin_amdgcn_exp2f(fmaf(fmaf(s[i >> 4][i & 15], unit, -ref), kLog2e, (float)by));
         } else {
-            const int above = tile_ev - E, by = 14 + max(above, kFarE);
-            // A reference far out (biases of the type's lowest value) is taken off before the product,
-            // which would overflow.
-            if (EXTRA && __ballot(!(fabsf(ref) < 1e4f))) {
+            const float up = (float)by - off;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) s[i >> 4][i & 15] = __builtin_amdgcn_exp2f(fmaf(fmaf(s[i >> 4][i & 15], unit, -ref), kLog2e, (float)by));
-            } else {
-                const float f = EXTRA ? unit * kLog2e : unit, up = (float)by - (EXTRA ? ref * kLog2e : ref);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) s[i >> 4][i & 15] = __builtin_amdgcn_exp2f(fmaf(s[i >> 4][i & 15], f, up));
-            }
-#pragma unroll
-            for (int i = 0; i < 32; ++i) total += s[i >> 4][i & 15];
-            asm volatile("" : "+v"(total));  // not behind the branch below, for which the weights would be copied
-            sum = fmaf(sum, alpha, ldexpf(total, -by));
-            if (__ballot(above < kFarE)) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (above < kFarE) s[i >> 4][i & 15] = 0.f;
-            }
+            for (int i = 0; i < 32; ++i) s[i >> 4][i & 15] = __builtin_amdgcn_exp2f(fmaf(s[i >> 4][i & 15], f, up));
         }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) weights += s[i >> 4][i & 15];
+        asm volatile("" : "+v"(weights));  // not behind the branch below, for which they would be copied
+        if (!own) total = ldexpf(weights, -by);
+        sum = fmaf(sum, alpha, total);
         if (__ballot(ao != 1.0f)) {
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
@@ -810,11 +857,16 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
         if (n > n0 && n < nt) copy(tile_of(n), 1, vn);  // the first one came with its K
     };
     const bool late = w < WAVES / 2;
+    // Tiles with exponents of their keys, and all tiles where a query is not finite, are behind everything that a row
+    // sees in this loop and wait for a second one: branches for them here made the compiler copy the scores around
+    // each (17 of 400 instructions a tile, distance 84 -> 88 us), ways around their products made it spill.
+    bool odd_rows = false, some_odd = false;
+    auto is_odd = [&](int flag) { return odd_rows || (flag & (kKeyExps | kValueExps)); };
+    auto sees = [&](int k0) { return active && ((k0 < pre && k0 + kKT > 0) || (k0 < last_hi && k0 + kKT > first_lo)); };
     int bad_first = nt, bad_last = -1;  // the tiles that hold values that are not finite
     // kc, vc: this tile's; vn: the next one's V (the next but one's K goes into kc)
     auto step = [&](int n, u16* kc, u16* vc, u16* vn) __attribute__((always_inline)) {
         const int tile = tile_of(n), k0 = tile * kKT - T.z;
-        const bool mine = active && ((k0 < pre && k0 + kKT > 0) || (k0 < last_hi && k0 + kKT > first_lo));
         // asked for here, so that the answer is there after the products
         const int4 about = info[tile];
         const int tile_ek = __builtin_amdgcn_readfirstlane(about.x), tile_ev = __builtin_amdgcn_readfirstlane(about.y),
@@ -823,20 +875,43 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
             bad_first = min(bad_first, n);
             bad_last = n;
         }
-        if (!mine) {
+        const bool odd = is_odd(flag);
+        some_odd |= odd;
+        if (!sees(k0)) {
             meet(n + 1, kc, vn);
             return;
         }
         scores(kc);
         if (!late) meet(n + 1, kc, vn);
-        softmax(k0, tile, tile_ek, tile_ev, flag);
+        softmax(std::false_type(), odd ? lk + kKT : k0, tile, tile_ek, tile_ev, flag);
         if (late) meet(n + 1, kc, vn);
         values(vc);
     };
+    if (lane == 0) odd_waves[w] = __ballot(bad_q) != 0;
     if (n0 < nt) meet(n0, kbuf1, vbuf0);
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) odd_rows |= __builtin_amdgcn_readfirstlane(odd_waves[i]) != 0;
     for (int n = n0; n < nt; n += 2) {
         step(n, kbuf0, vbuf0, vbuf1);
         if (n + 1 < nt) step(n + 1, kbuf1, vbuf1, vbuf0);
+    }
+    if (some_odd) {  // of all waves alike
+        auto together = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+        for (int n = n0; n < nt; n += 64) {
+            const int4 about = n + lane < nt ? info[tile_of(n + lane)] : make_int4(0, 0, 0, 0);
+            for (unsigned long long left = __ballot(n + lane < nt && is_odd(about.z)); left; left &= left - 1) {
+                const int i = (int)__ffsll(left) - 1, tile = tile_of(n + i), k0 = tile * kKT - T.z;
+                together();  // nobody reads the buffers any more
+                copy(tile, 0, kbuf0);
+                copy(tile, 1, vbuf0);
+                together();
+                if (!sees(k0)) continue;
+                scores(kbuf0);
+                softmax(std::true_type(), k0, tile, __builtin_amdgcn_readlane(about.x, i), __builtin_amdgcn_readlane(about.y, i),
+                        __builtin_amdgcn_readlane(about.z, i));
+                values(vbuf0);
+            }
+        }
     }
 
     if (r >= rows) return;
@@ -846,13 +921,25 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
     for (int n = bad_first; n <= bad_last; ++n)
         for (int j = max(tile_of(n) * kKT - T.z, 0), end = min(tile_of(n) * kKT - T.z + kKT, lk); j < end; ++j) {
             if (!visible(j)) continue;
-            const float* vp = P.v + (T.z + j) * kv_inner + (int64_t)kh * d;
+            const auto R = args();
+            const int d = R->d;
+            const int64_t key = ((int64_t)(T.z + j) * R->kv_heads + kh) * d;
+            const float *qr = R->q + ((int64_t)(T.first + qi) * R->heads + h) * d, *kr = R->k + key, *vr = R->v + key;
+            bool any = false;
+            for (int c = 0; c < d; ++c) any |= abs_bits(vr[c]) >= kInfBits;
+            if (!any || hidden(R, j)) continue;
+            float x = 0.f;
+            for (int c = 0; c < d; ++c) x = fmaf(qr[c], kr[c], x);
+            if (x * R->scale == -INFINITY && !(R->cap > 0.f)) continue;  // no weight
+            int c0 = fh * 4;
+            asm volatile("" : "+v"(c0));
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {  // columns past d are not stored
-                    const float x = vp[min(dt * 32 + (i >> 2) * 8 + fh * 4 + (i & 3), d - 1)];
-                    if (abs_bits(x) >= kInfBits) o[dt][i] += x;
+                    const float y = vr[min(dt * 32 + (i >> 2) * 8 + c0 + (i & 3), d - 1)];
+                    if (abs_bits(y) >= kInfBits) o[dt][i] += y;
+                    few(i);
                 }
         }
     const int64_t row = (int64_t)(T.first + qi) * P.heads + h, cell = row * S.n + blockIdx.y, at = row * d;

@@ -98,3 +98,27 @@ def test_powers_of_two(be, orc, lq, d, power):
     c.v = (c.v * np.float64(2.0 ** power)).astype(np.float32)
     held(c, be, orc, f"2^{power}")
     held(c, be, orc, f"2^{power} causal", causal=True)
+
+
+# ----------------------------------------------------------- keys that are not finite
+@gpu
+@pytest.mark.parametrize("lq,d", [s for s in SHAPES if s != ([1], 40)])
+def test_infinite_keys(be, orc, lq, d):
+    """Scores of -inf have no weight, scores of +inf and 0 * inf make their rows NaN, a cap makes both finite."""
+    for sign in (1.0, -1.0):
+        for where in (0, 1, d - 1):
+            c = Case(orc, lq, [150], 2, 2, d, seed=2600)
+            c.q[:, where::d] = np.abs(c.q[:, where::d]) + 0.25
+            c.k[40, where], c.k[100, d + where] = sign * np.inf, -np.inf
+            held(c, be, orc, f"{sign} {where}")
+            held(c, be, orc, f"{sign} {where} causal", causal=True)
+            held(c, be, orc, f"{sign} {where} cap", cap=5.0)
+            held(c, be, orc, f"{sign} {where} bias", bias=orc.randn((2, 21), 2601), radius=10)
+    c.q[0, :d] = 0.0
+    held(c, be, orc, "0 * inf")
+    c.q[0, :d] = np.nan
+    held(c, be, orc, "NaN query")
+    c.q[0, :d] = 1.0
+    c.q[0, 3] = np.inf
+    held(c, be, orc, "infinite query")
+    held(c, be, orc, "infinite query cap", cap=5.0)
