@@ -1034,6 +1034,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_packed_few(Packed P, in
         for (int u = 0; u < kLoads; ++u) kx[u] = dev::ld_stream((const f4*)(P.k + base + min(k0 + u * KEYS + sub, lk - 1) * kv_inner));
 #pragma unroll
         for (int u = 0; u < kLoads; ++u) vx[u] = dev::ld_stream((const f4*)(P.v + base + min(k0 + u * KEYS + sub, lk - 1) * kv_inner));
+        if (d < DP) {  // lanes past d: their zeros of q times an infinity would be NaN
+#pragma unroll
+            for (int u = 0; u < kLoads; ++u) kx[u] = c4 < d ? kx[u] : f4{0.f, 0.f, 0.f, 0.f};
+        }
         const bool full = k0 + CHUNK <= pre || (k0 >= lo[R - 1] && k0 + CHUNK <= hi[0]);
         auto visible = [&](int u, int r) {
             const int j = k0 + u * KEYS + sub;
