@@ -168,7 +168,10 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_attn_packed_rows(Packed P) {
 // Values that are not finite go into the tiles as zeros, since 0 * inf would reach
 // the rows that do not see them, and are added at the end. An infinity in q or k would be
 // inf - inf in a pair: a wave one of whose rows sees such a key, or has such a query, takes the
-// tile's scores in fp32 (fp32_scores).
+// tile's scores in fp32 (fp32_scores). So it does where values far below their block's largest, whose pairs are
+// off by up to 2^-25, could move a score by more than 2^-21: by 2^-25 (sum|q| + sum|k|) of the scaled values
+// in units of 2^(e_q + e_k) scale. Heads of 128 whose largest q and k meet at scores of 2^15 are far from that;
+// a channel of q or k that is 2^12 above the others is not.
 //
 // S^T = K Q^T and O^T = V^T P^T by v_mfma_f32_32x32x16_f16: lane l holds row l % 32 of
 // the wave in both, its statistics are its own. K's rows are ordered so that the eight
@@ -199,6 +202,7 @@ constexpr float kLazy = 1.5f;
 // tile's 64 keys reach past the radius unless all of them are beyond it: no index is held to the radius
 // (ten instructions a score; the rows and tiles at the band's edges took half the softmax' time).
 constexpr int kBiasPad = 96;
+constexpr float kMostLost = 16.0f;  // 2^25 times 2^-21
 constexpr int kBadKey = 1000;   // the exponent of a key that is not finite
 constexpr int kUnsetE = -2000;  // no weighted values yet, or next to nothing beside the reference
 constexpr int kSpread = 8;
@@ -257,7 +261,7 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)
 enum { kKeyExps = 1, kValueExps = 2, kNotFinite = 4 };
 struct Tiles {
     u16* data;   // [kv_heads, n, 4 * 64 DP]: K hi, K lo, V^T hi, V^T lo
-    int4* info;  // [kv_heads, n]: e_k, e_v, flags
+    int4* info;  // [kv_heads, n]: e_k, e_v, flags, the largest sum of a scaled key's magnitudes (a float)
     int* exps;   // [kv_heads, n, 2, 64]: of the keys, where the flags say so
     int n;
 };
@@ -268,6 +272,7 @@ __global__ __launch_bounds__(64 * kSplitWaves) void k_attn_packed_split(Packed P
     constexpr int VU = DP / 64;                                                     // columns of v a lane has
     __shared__ __attribute__((aligned(16))) u16 vt[2 * PART];
     __shared__ int tops[2][kSplitWaves], flags[kSplitWaves];
+    __shared__ float sums[kSplitWaves];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tile = blockIdx.x, kh = blockIdx.y, j0 = tile * kKT + w * 16, d = P.d;
     const int64_t kv_inner = (int64_t)P.kv_heads * d;
@@ -355,9 +360,9 @@ __global__ __launch_bounds__(64 * kSplitWaves) void k_attn_packed_split(Packed P
     flag = flags[0] | flags[1] | flags[2] | flags[3];
     const int ek = block_exp(kmost), ev = block_exp(vmost);
     const int64_t at = (int64_t)kh * X.n + tile;
-    if (threadIdx.x == 0) X.info[at] = make_int4(ek, ev, flag, 0);
     int* exps = X.exps + at * 2 * kKT;
     u16 *kd = X.data + at * 4 * PART, *vd = kd + 2 * PART;
+    float ksum = 0.f;
 #pragma unroll
     for (int u = 0; u < KU; ++u) {
         const int key = w * 16 + u * KROWS + krow, e = flag & kKeyExps ? block_exp(ktop[u]) : ek;
@@ -365,9 +370,16 @@ __global__ __launch_bounds__(64 * kSplitWaves) void k_attn_packed_split(Packed P
         const float sc = pow2(-e);
         h8 hi, lo;
 #pragma unroll
+        for (int i = 0; i < 8; ++i) kx[u][i] *= sc;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += fabsf(kx[u][i]);
+        sum = dev::group_sum<KCH>(sum);
+        if (ktop[u] < kInfBits) ksum = fmaxf(ksum, sum);
+#pragma unroll
         for (int i = 0; i < 8; i += 2) {
             h2 a, c;
-            split_pair(kx[u][i] * sc, kx[u][i + 1] * sc, a, c);
+            split_pair(kx[u][i], kx[u][i + 1], a, c);
             hi[i] = a[0], hi[i + 1] = a[1];
             lo[i] = c[0], lo[i + 1] = c[1];
         }
@@ -398,7 +410,10 @@ __global__ __launch_bounds__(64 * kSplitWaves) void k_attn_packed_split(Packed P
             *(h8*)(vt + to) = hi;
             *(h8*)(vt + PART + to) = lo;
         }
+    ksum = dev::wave_max(ksum);
+    if (lane == 0) sums[w] = ksum;
     __syncthreads();  // whole lines of V^T, of which a wave has a quarter
+    if (threadIdx.x == 0) X.info[at] = make_int4(ek, ev, flag, (int)__float_as_uint(fmaxf(fmaxf(sums[0], sums[1]), fmaxf(sums[2], sums[3]))));
 #pragma unroll
     for (int i = 0; i < 2 * PART / (8 * 64 * kSplitWaves); ++i) {
         const int to = (i * 64 * kSplitWaves + threadIdx.x) * 8;
@@ -420,7 +435,7 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
     // Rows of K, hi and lo, of two tiles, and of V^T. Objects of their own, so that the compiler
     // knows which copy a read has to wait for.
     __shared__ __attribute__((aligned(1024))) u16 kbuf0[2 * PART], kbuf1[2 * PART], vbuf0[2 * PART], vbuf1[2 * PART];
-    __shared__ int odd_waves[WAVES];
+    __shared__ f2 q_waves[WAVES];
     extern __shared__ float biases[];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int fr = lane & 31, fh = lane >> 5;
@@ -522,7 +537,6 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
     }
     h8 qh[DS], ql[DS];
     int eq;
-    bool bad_q;
     {
         int top = 0;
 #pragma unroll
@@ -531,17 +545,23 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
             for (int e = 0; e < 8; ++e) top = max(top, abs_bits(qx[ds][e]));
         top = max(top, __shfl_xor(top, 32, 64));
         eq = block_exp(top);
-        bad_q = top >= kInfBits;
         const float sc = copysignf(pow2(-eq), P.scale);  // a negative scale turns q's sign
+        float all = 0.f;
 #pragma unroll
         for (int ds = 0; ds < DS; ++ds)
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
                 h2 hi, lo;
-                split_pair(qx[ds][e] * sc, qx[ds][e + 1] * sc, hi, lo);
+                const float x = qx[ds][e] * sc, y = qx[ds][e + 1] * sc;
+                all += fabsf(x) + fabsf(y);
+                split_pair(x, y, hi, lo);
                 qh[ds][e] = hi[0], qh[ds][e + 1] = hi[1];
                 ql[ds][e] = lo[0], ql[ds][e + 1] = lo[1];
             }
+        // of the wave's rows: the largest block, and the largest sum of magnitudes
+        all += __shfl_xor(all, 32, 64);
+        const float block = pow2(eq), most = dev::wave_max(block), sum = dev::wave_max(all < INFINITY ? block * all : INFINITY);
+        if (lane == 0) q_waves[w] = f2{most, sum};
     }
     const float scale = EXTRA ? fabsf(P.scale) : fabsf(P.scale) * kLog2e;
 
@@ -626,15 +646,16 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
             }
         }
     };
+    f2 q_most = {0.f, 0.f};  // of the workgroup's rows, as q_waves
+    auto loses = [&](int ek, float ksum) { return !(ldexpf(scale * fmaf(q_most[0], ksum, q_most[1]), ek) <= kMostLost); };
     // s -> weights in place, the statistics and the scale of o brought up to date. k0: the
     // sequence's key at the tile's first row (below zero in front of the sequence). `odd`: what the
     // first loop leaves to the second.
-    auto softmax = [&](auto odd, int k0, int tile, int tile_ek, int tile_ev, int flag) __attribute__((always_inline)) {
+    auto softmax = [&](auto odd, int k0, int tile, int tile_ek, int tile_ev, int flag, float ksum) __attribute__((always_inline)) {
         constexpr bool ODD = decltype(odd)::value;
         const int* exps = X.exps + ((int64_t)kh * X.n + tile) * 2 * kKT;
         const bool edge = !((k0 >= 0 && k0 + kKT <= pre) || (k0 >= last_lo && k0 + kKT <= first_hi));  // of this wave
         int ek = tile_ek;
-        bool bad = bad_q;
         if (ODD && (flag & kKeyExps)) {
             ek = -126;
 #pragma unroll 1
@@ -645,7 +666,6 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
                     ek = max(ek, visible(k0 + u * 16 + fh * 8 + i) ? e : -126);
                 }
             ek = max(ek, __shfl_xor(ek, 32, 64));
-            bad |= ek == kBadKey;
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -654,7 +674,7 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
         }
         // kept normal: -inf stays -inf, zero zero
         float unit = fminf(fmaxf(ldexpf(scale, eq + ek), 1.17549435e-38f), 3.40282347e38f);  // of s
-        if (ODD && __ballot(bad)) {
+        if (ODD && __ballot(ek == kBadKey || loses(ek, ksum))) {
             fp32_scores(k0);
             unit = EXTRA ? 1.0f : kLog2e;
         }
@@ -857,11 +877,11 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
         if (n > n0 && n < nt) copy(tile_of(n), 1, vn);  // the first one came with its K
     };
     const bool late = w < WAVES / 2;
-    // Tiles with exponents of their keys, and all tiles where a query is not finite, are behind everything that a row
+    // Tiles with exponents of their keys, and those whose scores may need fp32, are behind everything that a row
     // sees in this loop and wait for a second one: branches for them here made the compiler copy the scores around
     // each (17 of 400 instructions a tile, distance 84 -> 88 us), ways around their products made it spill.
-    bool odd_rows = false, some_odd = false;
-    auto is_odd = [&](int flag) { return odd_rows || (flag & (kKeyExps | kValueExps)); };
+    bool some_odd = false;
+    auto is_odd = [&](int ek, int flag, float ksum) { return (flag & (kKeyExps | kValueExps)) || loses(ek, ksum); };
     auto sees = [&](int k0) { return active && ((k0 < pre && k0 + kKT > 0) || (k0 < last_hi && k0 + kKT > first_lo)); };
     int bad_first = nt, bad_last = -1;  // the tiles that hold values that are not finite
     // kc, vc: this tile's; vn: the next one's V (the next but one's K goes into kc)
@@ -870,12 +890,12 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
         // asked for here, so that the answer is there after the products
         const int4 about = info[tile];
         const int tile_ek = __builtin_amdgcn_readfirstlane(about.x), tile_ev = __builtin_amdgcn_readfirstlane(about.y),
-                  flag = __builtin_amdgcn_readfirstlane(about.z);
+                  flag = __builtin_amdgcn_readfirstlane(about.z), sum_bits = __builtin_amdgcn_readfirstlane(about.w);
         if (flag & kNotFinite) {
             bad_first = min(bad_first, n);
             bad_last = n;
         }
-        const bool odd = is_odd(flag);
+        const bool odd = is_odd(tile_ek, flag, __uint_as_float(sum_bits));
         some_odd |= odd;
         if (!sees(k0)) {
             meet(n + 1, kc, vn);
@@ -883,14 +903,14 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
         }
         scores(kc);
         if (!late) meet(n + 1, kc, vn);
-        softmax(std::false_type(), odd ? lk + kKT : k0, tile, tile_ek, tile_ev, flag);
+        softmax(std::false_type(), odd ? lk + kKT : k0, tile, tile_ek, tile_ev, flag, 0.f);
         if (late) meet(n + 1, kc, vn);
         values(vc);
     };
-    if (lane == 0) odd_waves[w] = __ballot(bad_q) != 0;
     if (n0 < nt) meet(n0, kbuf1, vbuf0);
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) odd_rows |= __builtin_amdgcn_readfirstlane(odd_waves[i]) != 0;
+    for (int i = 0; i < WAVES; ++i) q_most = f2{fmaxf(q_most[0], q_waves[i][0]), fmaxf(q_most[1], q_waves[i][1])};
+    q_most = f2{dev::readlane(q_most[0], 0), dev::readlane(q_most[1], 0)};
     for (int n = n0; n < nt; n += 2) {
         step(n, kbuf0, vbuf0, vbuf1);
         if (n + 1 < nt) step(n + 1, kbuf1, vbuf1, vbuf0);
@@ -899,7 +919,7 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
         auto together = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
         for (int n = n0; n < nt; n += 64) {
             const int4 about = n + lane < nt ? info[tile_of(n + lane)] : make_int4(0, 0, 0, 0);
-            for (unsigned long long left = __ballot(n + lane < nt && is_odd(about.z)); left; left &= left - 1) {
+            for (unsigned long long left = __ballot(n + lane < nt && is_odd(about.x, about.z, __uint_as_float(about.w))); left; left &= left - 1) {
                 const int i = (int)__ffsll(left) - 1, tile = tile_of(n + i), k0 = tile * kKT - T.z;
                 together();  // nobody reads the buffers any more
                 copy(tile, 0, kbuf0);
@@ -908,7 +928,7 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
                 if (!sees(k0)) continue;
                 scores(kbuf0);
                 softmax(std::true_type(), k0, tile, __builtin_amdgcn_readlane(about.x, i), __builtin_amdgcn_readlane(about.y, i),
-                        __builtin_amdgcn_readlane(about.z, i));
+                        __builtin_amdgcn_readlane(about.z, i), dev::readlane(__uint_as_float(about.w), i));
                 values(vbuf0);
             }
         }

@@ -122,3 +122,23 @@ def test_infinite_keys(be, orc, lq, d):
     c.q[0, 3] = np.inf
     held(c, be, orc, "infinite query")
     held(c, be, orc, "infinite query cap", cap=5.0)
+
+
+# ------------------------------------------------------------------ unlike channels
+@gpu
+@pytest.mark.parametrize("power", [12, 24, 40])
+@pytest.mark.parametrize("lq,d", SHAPES)
+def test_unlike_channels(be, orc, lq, d, power):
+    """A channel of the queries, or of the keys, that is far above the others and meets nothing, or next to nothing."""
+    up = np.float32(2.0 ** power)
+    for meets in (np.float32(0), 1 / up):
+        for which in ("q", "k", "both"):
+            c = Case(orc, lq, [150], 2, 1, d, seed=2800)
+            if which != "k":
+                c.q[:, 5::d] *= up
+                c.k[:, 5] *= meets
+            if which != "q":
+                c.k[:, 7] *= up
+                c.q[:, 7::d] *= meets
+            held(c, be, orc, f"{which} {meets}")
+            held(c, be, orc, f"{which} {meets} cap and bias", cap=4.0, bias=orc.randn((2, 61), 2801), radius=30, causal=True)
