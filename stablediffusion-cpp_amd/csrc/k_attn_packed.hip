@@ -65,6 +65,9 @@ __device__ __forceinline__ float tanh_near(float x) {
     return a < kTanhNear ? tanh_small(x) : far;
 }
 
+// A bias of -inf hides its key, whatever the key holds.
+__device__ __forceinline__ float biased(float x, float b) { return b == -INFINITY ? b : x + b; }
+
 // ---------------------------------------------------------------------------
 // Any head dimension: fp32 products, one wave per (query, head). Lanes take 64 keys at a
 // time for the scores, then 64 columns at a time for the weighted sum. Takes heads of more
@@ -106,7 +109,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_attn_packed_rows(Packed P) {
                 for (int c = 0; c < d; ++c) a = fmaf(sq[w][c], kp[c], a);
                 x = a * P.scale;
                 if (P.cap > 0.f) x = P.cap * tanh_near(x / P.cap);
-                if (P.bias) x += P.bias[(int64_t)h * (2 * P.radius + 1) + min(max(j - p, -P.radius), P.radius) + P.radius];
+                if (P.bias) x = biased(x, P.bias[(int64_t)h * (2 * P.radius + 1) + min(max(j - p, -P.radius), P.radius) + P.radius]);
             }
             const float mnew = fmaxf(m, dev::wave_max(x));
             const float ref = mnew == -INFINITY ? 0.f : mnew;  // nothing but -inf so far
@@ -125,6 +128,11 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_attn_packed_rows(Packed P) {
                 float a = acc[i] * alpha;
                 if (c < d)
                     for (int u = 0; u < nk; ++u) a = fmaf(sp[w][u], P.v[kv0 + (k0 + u) * kv_inner + c], a);
+                if (__ballot(!(fabsf(a) < INFINITY)) && c < d) {  // some may not count, whatever their values are: 0 * inf is not zero
+                    a = acc[i] * alpha;
+                    for (int u = 0; u < nk; ++u)
+                        if (sp[w][u] != 0.f) a = fmaf(sp[w][u], P.v[kv0 + (k0 + u) * kv_inner + c], a);
+                }
                 acc[i] = a;
             }
         }
@@ -1076,8 +1084,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_packed_few(Packed P, in
                 for (int r = 0; r < R; ++r) {
                     if (P.cap > 0.f) s[u][r] = P.cap * tanh_near(s[u][r] / P.cap);
                     if (P.bias)
-                        s[u][r] += P.bias[(int64_t)head[r] * (2 * P.radius + 1) + P.radius +
-                                          min(max(k0 + u * KEYS + sub - place[r], -P.radius), P.radius)];
+                        s[u][r] = biased(s[u][r], P.bias[(int64_t)head[r] * (2 * P.radius + 1) + P.radius +
+                                                         min(max(k0 + u * KEYS + sub - place[r], -P.radius), P.radius)]);
                 }
         }
         if (!full) {
@@ -1087,6 +1095,12 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_packed_few(Packed P, in
                 for (int r = 0; r < R; ++r)
                     if (!visible(u, r)) s[u][r] = -INFINITY;
         }
+        float odd = 0.f;  // NaN with a value that is not finite
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) odd = fmaf(vx[u][e], 0.f, odd);
+        const bool some_odd = __ballot(odd != 0.f) != 0;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             float mx = s[0][r];
@@ -1103,7 +1117,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_packed_few(Packed P, in
                 sum[r] += s[u][r];
             }
         }
-        if (full) {
+        if (!some_odd) {
 #pragma unroll
             for (int u = 0; u < kLoads; ++u)
 #pragma unroll
@@ -1113,7 +1127,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_packed_few(Packed P, in
             for (int u = 0; u < kLoads; ++u)
 #pragma unroll
                 for (int r = 0; r < R; ++r)
-                    if (visible(u, r)) o[r] += s[u][r] * vx[u];  // 0 * inf is not zero
+                    if (s[u][r] != 0.f) o[r] += s[u][r] * vx[u];  // 0 * inf is not zero
         }
     }
     const int g0 = w * KEYS + sub;

@@ -102,6 +102,23 @@ def test_powers_of_two(be, orc, lq, d, power):
 
 # ----------------------------------------------------------- keys that are not finite
 @gpu
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf, 3e38])
+@pytest.mark.parametrize("lq,d", SHAPES)
+def test_hidden_by_a_bias_whatever_they_hold(be, orc, lq, d, bad):
+    c = Case(orc, lq, [150], 4, 2, d, seed=2500)
+    bias = orc.randn((4, 301), 2501)
+    bias[:, :91] = -np.inf
+    bias[1] = -np.inf  # a head that sees nothing at all
+    c.v[[3, 20, 33, 44]] = bad
+    held(c, be, orc, f"{bad} values", bias=bias, radius=150)
+    c.k[[3, 21, 33, 45]] = bad
+    held(c, be, orc, f"{bad}", bias=bias, radius=150)
+    held(c, be, orc, f"{bad} causal cap", bias=bias, radius=150, causal=True, cap=30.0)
+    one = np.full((4, 1), -np.inf, np.float32)
+    assert np.all(held(c, be, orc, "nothing", bias=one, radius=0) == 0)
+
+
+@gpu
 @pytest.mark.parametrize("lq,d", SHAPES)
 def test_infinite_keys(be, orc, lq, d):
     """Scores of -inf have no weight, scores of +inf and 0 * inf make their rows NaN, a cap makes both finite."""
@@ -142,3 +159,30 @@ def test_unlike_channels(be, orc, lq, d, power):
                 c.q[:, 7::d] *= meets
             held(c, be, orc, f"{which} {meets}")
             held(c, be, orc, f"{which} {meets} cap and bias", cap=4.0, bias=orc.randn((2, 61), 2801), radius=30, causal=True)
+
+
+# --------------------------------------------------------------- keys cut into parts
+def parts_of_tiles(c, cus=256):
+    """How many parts the dispatch cuts the keys into: those that fill the chip, of 512 keys of an average sequence at least."""
+    group, waves = c.heads // c.kv, 8 if c.d > 64 else 4
+    live = min(len(c.spans), c.Tq)
+    assert -(-c.Tq // live) * group > 16, "the few rows' kernel"
+    wgs = (c.Tq * group // (32 * waves) + live) * c.kv
+    return min(cus * (8 // waves) // wgs, c.Tk // len(c.spans) // 512, 256)
+
+
+PART_SHAPES = [(4, 1, 128), (8, 2, 64), (2, 2, 40)]
+
+
+@gpu
+@pytest.mark.parametrize("lq", [[24, 33], [1, 1]])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, 1e30])
+def test_parts_that_a_bias_hides(be, orc, lq, bad):
+    c = Case(orc, lq, [3000, 4500], 4, 1, 128, seed=3100)
+    bias = orc.randn((4, 2 * 2500 + 1), 3101)
+    bias[:, :1200] = -np.inf  # more than 1300 in front
+    c.v[:1600] = bad
+    c.k[100:1500] = bad
+    c.v[3000:3000 + 3000] = bad
+    held(c, be, orc, f"{bad}", bias=bias, radius=2500)
+    held(c, be, orc, f"{bad} window", bias=bias, radius=2500, causal=True, window=2000)
