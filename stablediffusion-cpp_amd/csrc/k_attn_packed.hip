@@ -65,6 +65,15 @@ __device__ __forceinline__ float tanh_near(float x) {
     return a < kTanhNear ? tanh_small(x) : far;
 }
 
+__device__ __forceinline__ int abs_bits(float x) { return (int)(__float_as_uint(x) & 0x7FFFFFFFu); }
+constexpr int kInfBits = 0x7F800000;
+__device__ __forceinline__ bool finite(float x) { return abs_bits(x) < kInfBits; }
+__device__ __forceinline__ bool finite(const f4& x) { return finite(x.x) && finite(x.y) && finite(x.z) && finite(x.w); }
+// A sum of weighted values at another reference: what is not finite stays so, however far the reference has risen.
+__device__ __forceinline__ float scaled(float sum, float by) { return by == 0.f && !finite(sum) ? sum : sum * by; }
+__device__ __forceinline__ f4 scaled(const f4& sum, float by) {
+    return f4{scaled(sum.x, by), scaled(sum.y, by), scaled(sum.z, by), scaled(sum.w, by)};
+}
 // A bias of -inf hides its key, whatever the key holds.
 __device__ __forceinline__ float biased(float x, float b) { return b == -INFINITY ? b : x + b; }
 
@@ -119,6 +128,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_attn_packed_rows(Packed P) {
             sum = sum * alpha + dev::wave_sum(weight);
             __builtin_amdgcn_wave_barrier();
             sp[w][lane] = weight;
+            const unsigned long long count = __ballot(x != -INFINITY);
             __builtin_amdgcn_wave_barrier();
             const int nk = min(64, to - k0);
 #pragma unroll
@@ -128,10 +138,13 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_attn_packed_rows(Packed P) {
                 float a = acc[i] * alpha;
                 if (c < d)
                     for (int u = 0; u < nk; ++u) a = fmaf(sp[w][u], P.v[kv0 + (k0 + u) * kv_inner + c], a);
-                if (__ballot(!(fabsf(a) < INFINITY)) && c < d) {  // some may not count, whatever their values are: 0 * inf is not zero
-                    a = acc[i] * alpha;
-                    for (int u = 0; u < nk; ++u)
-                        if (sp[w][u] != 0.f) a = fmaf(sp[w][u], P.v[kv0 + (k0 + u) * kv_inner + c], a);
+                if (__ballot(!finite(a)) && c < d) {  // 0 * inf is neither zero nor inf: keys that do not count, weights that underflow
+                    a = scaled(acc[i], alpha);
+                    for (int u = 0; u < nk; ++u) {
+                        if (!(count >> u & 1)) continue;
+                        const float x = P.v[kv0 + (k0 + u) * kv_inner + c];
+                        a = finite(x) ? fmaf(sp[w][u], x, a) : a + x;
+                    }
                 }
                 acc[i] = a;
             }
@@ -258,8 +271,6 @@ __device__ __forceinline__ unsigned wave_max_halves(unsigned v) {
     const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     return larger(b[0], b[1]);
 }
-__device__ __forceinline__ int abs_bits(float x) { return (int)(__float_as_uint(x) & 0x7FFFFFFFu); }
-constexpr int kInfBits = 0x7F800000;
 // The exponent that brings a block's largest magnitude into [2^13, 2^14); zero and
 // subnormal blocks the least there is.
 __device__ __forceinline__ int block_exp(int bits) { return min(max((bits >> 23) - 140, -126), 126); }
@@ -1055,6 +1066,40 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_packed_few(Packed P, in
     const int all = npre + (hi[R - 1] > lo[0] ? max(0, (hi[R - 1] + CHUNK - 1) / CHUNK - next) : 0);
     const int n0 = (int)((int64_t)all * blockIdx.y / S.n), n1 = (int)((int64_t)all * (blockIdx.y + 1) / S.n);
     const int64_t base = T.z * kv_inner + (int64_t)kh * d + (c4 < d ? c4 : 0);
+    // The weighted values of a chunk some of which are not finite, a key at a time: 0 * inf is neither zero nor inf, where a
+    // key does not count or its weight underflows. What is not finite waits in the lane's place of so for the end.
+    bool had_odd = false;
+    const int g0 = w * KEYS + sub;
+    auto odd_values = [&](int k0) __attribute__((always_inline)) {
+        if (!had_odd) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) *(f4*)&so[g0][r][c4] = f4{0.f, 0.f, 0.f, 0.f};
+        }
+        had_odd = true;
+#pragma unroll 1
+        for (int u = 0; u < kLoads; ++u) {
+            const int j = k0 + u * KEYS + sub;
+            const int64_t at = base + min(j, lk - 1) * kv_inner;
+            f4 k = *(const f4*)(P.k + at);
+            const f4 v = *(const f4*)(P.v + at);
+            if (c4 >= d) k = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float x = lanes_sum<LANES>(fmaf(q[r].x, k.x, q[r].y * k.y) + fmaf(q[r].z, k.z, q[r].w * k.w));
+                if constexpr (EXTRA) {
+                    if (P.cap > 0.f) x = P.cap * tanh_near(x / P.cap);
+                    if (P.bias) x = biased(x, P.bias[(int64_t)head[r] * (2 * P.radius + 1) + P.radius + min(max(j - place[r], -P.radius), P.radius)]);
+                }
+                if (!((j < pre) | ((j >= lo[r]) & (j < hi[r]))) || x == -INFINITY) continue;
+                const float weight = __builtin_amdgcn_exp2f((x - m[r]) * (EXTRA ? kLog2e : 1.0f));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (finite(v[e])) o[r][e] = fmaf(weight, v[e], o[r][e]);
+                    else so[g0][r][c4 + e] += v[e];
+                }
+            }
+        }
+    };
     for (int n = n0 + w; n < n1; n += kFewWaves) {
         const int k0 = (n < npre ? n : next + n - npre) * CHUNK;
         f4 kx[kLoads], vx[kLoads];
@@ -1100,7 +1145,6 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_packed_few(Packed P, in
         for (int u = 0; u < kLoads; ++u)
 #pragma unroll
             for (int e = 0; e < 4; ++e) odd = fmaf(vx[u][e], 0.f, odd);
-        const bool some_odd = __ballot(odd != 0.f) != 0;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             float mx = s[0][r];
@@ -1117,23 +1161,18 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_packed_few(Packed P, in
                 sum[r] += s[u][r];
             }
         }
-        if (!some_odd) {
-#pragma unroll
-            for (int u = 0; u < kLoads; ++u)
-#pragma unroll
-                for (int r = 0; r < R; ++r) o[r] += s[u][r] * vx[u];
+        if (__ballot(odd != 0.f)) {
+            odd_values(k0);
         } else {
 #pragma unroll
             for (int u = 0; u < kLoads; ++u)
 #pragma unroll
-                for (int r = 0; r < R; ++r)
-                    if (s[u][r] != 0.f) o[r] += s[u][r] * vx[u];  // 0 * inf is not zero
+                for (int r = 0; r < R; ++r) o[r] += s[u][r] * vx[u];
         }
     }
-    const int g0 = w * KEYS + sub;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        *(f4*)&so[g0][r][c4] = o[r];
+        *(f4*)&so[g0][r][c4] = had_odd ? o[r] + *(const f4*)&so[g0][r][c4] : o[r];
         if (c4 == 0) sm[g0][r] = m[r], sl[g0][r] = sum[r];
     }
     __syncthreads();
@@ -1152,6 +1191,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_packed_few(Packed P, in
             v += x * *(const f4*)&so[g][r][c];
         }
         if (c >= d) continue;
+        if (!finite(v)) {  // a group's infinity times its weight of zero
+            v = f4{0.f, 0.f, 0.f, 0.f};
+            for (int g = 0; g < GROUPS; ++g)
+                v += scaled(*(const f4*)&so[g][r][c], __builtin_amdgcn_exp2f(EXTRA ? (sm[g][r] - ref) * kLog2e : sm[g][r] - ref));
+        }
         const int rr = T.row0 + r, qi = rr / group, h = kh * group + rr - qi * group;
         const int64_t row = (int64_t)(T.first + qi) * P.heads + h;
         if (S.n > 1) {
@@ -1193,6 +1237,10 @@ __global__ __launch_bounds__(32 * kJoin) void k_attn_packed_join(Packed P, int o
     if (c < P.d) {
 #pragma unroll 4
         for (int s = g; s < S.n; s += kJoin) v += weight[s] * *(const f4*)(S.o + (cell + s) * S.stride + c);
+        if (!finite(v)) {  // a part's infinity times its weight of zero
+            v = f4{0.f, 0.f, 0.f, 0.f};
+            for (int s = g; s < S.n; s += kJoin) v += scaled(*(const f4*)(S.o + (cell + s) * S.stride + c), weight[s]);
+        }
     }
     *(f4*)&so[g][c] = v;
     __syncthreads();

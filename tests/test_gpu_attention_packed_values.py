@@ -141,6 +141,34 @@ def test_infinite_keys(be, orc, lq, d):
     held(c, be, orc, "infinite query cap", cap=5.0)
 
 
+@gpu
+@pytest.mark.parametrize("lq,d", SHAPES)
+def test_infinite_keys_with_infinite_values(be, orc, lq, d):
+    """A score of -inf leaves its value out; under a cap, or with a score that is finite, it shows."""
+    c = Case(orc, lq, [150], 2, 2, d, seed=2650)
+    c.q[:, 3::d] = np.abs(c.q[:, 3::d]) + 0.25
+    c.k[40, 3], c.k[100, d + 3] = -np.inf, -np.inf
+    c.v[40] = np.inf
+    c.v[100, 1] = np.nan
+    for kw in ({}, {"causal": True}, {"cap": 5.0}, {"bias": orc.randn((2, 21), 2651), "radius": 10}):
+        held(c, be, orc, str(list(kw)), **kw)
+
+
+@gpu
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("lq,d", SHAPES)
+def test_seen_infinities_of_hardly_any_weight(be, orc, lq, d, value):
+    """A key 300 below the others, in front of them, behind them or between them."""
+    for place in (0, 75, 149):
+        c = Case(orc, lq, [150], 2, 1, d, seed=2700)
+        c.q[:, ::d] = 8.0
+        c.k[place, 0] = -300.0 / (8.0 * c.scale)
+        c.v[place, 2] = value
+        c.v[place, d - 1] = value
+        held(c, be, orc, f"{place}")
+        held(c, be, orc, f"{place} causal", causal=True)
+
+
 # ------------------------------------------------------------------ unlike channels
 @gpu
 @pytest.mark.parametrize("power", [12, 24, 40])
@@ -172,6 +200,45 @@ def parts_of_tiles(c, cus=256):
 
 
 PART_SHAPES = [(4, 1, 128), (8, 2, 64), (2, 2, 40)]
+
+
+@gpu
+@pytest.mark.parametrize("lq", [[24, 33], [1, 1]])
+@pytest.mark.parametrize("heads,kv,d", PART_SHAPES)
+def test_parts_of_unlike_values(be, orc, heads, kv, d, lq):
+    """What one part holds: large values, hidden or of little weight, infinities of hardly any, keys that are not finite."""
+    def case(seed=3000):
+        c = Case(orc, lq, [3000, 4500], heads, kv, d, seed=seed)
+        c.q[:, ::d] = 8.0
+        return c
+
+    def low(c, j, depth):
+        c.k[j, 0] = -depth / (8.0 * c.scale)
+
+    for depth, value in ((30.0, 1e10), (60.0, 1e30)):
+        c = case()
+        low(c, [700, 3000 + 2000], depth)
+        c.v[[700, 3000 + 2000]] *= np.float32(value)
+        held(c, be, orc, f"{depth} {value}")
+    c = case()
+    low(c, [700, 3000 + 2000], 300.0)
+    c.v[700, 3], c.v[3000 + 2000, 5] = np.inf, np.nan
+    held(c, be, orc, "infinity of hardly any weight")
+    c = case()
+    c.q[:, 3::d] = np.abs(c.q[:, 3::d]) + 0.25
+    c.k[700, 3], c.k[3000 + 2000, 3] = -np.inf, -np.inf
+    c.v[700] = np.inf
+    held(c, be, orc, "scores of -inf")
+    c.k[800, 3] = np.nan
+    held(c, be, orc, "a NaN key")
+    c = case()
+    c.v = (c.v * np.float64(2.0 ** -112)).astype(np.float32)
+    held(c, be, orc, "least values")
+    c = case()
+    low(c, np.arange(0, 1500), 100.0)
+    c.v[:1500] = 0
+    c.v[1500:3000] *= np.float32(2.0 ** -40)
+    held(c, be, orc, "parts of no value and no weight")
 
 
 @gpu
