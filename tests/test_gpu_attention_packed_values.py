@@ -203,6 +203,18 @@ PART_SHAPES = [(4, 1, 128), (8, 2, 64), (2, 2, 40)]
 
 
 @gpu
+@pytest.mark.parametrize("mask", list(MASKS) + ["long_prefix"])
+@pytest.mark.parametrize("heads,kv,d", PART_SHAPES)
+def test_parts(be, orc, heads, kv, d, mask):
+    """Some tens of rows against thousands of keys."""
+    c = Case(orc, [24, 33], [3000, 4500], heads, kv, d, seed=2900, gap=1)
+    assert parts_of_tiles(c) >= 4
+    kw = {"causal": True, "window": 900, "prefix": np.array([1500, 2777], np.int32)} if mask == "long_prefix" else masks(orc, mask, 2, heads)
+    for out_bf16 in (False, True):
+        held(c, be, orc, f"{mask} bf16 {out_bf16}", out_bf16, **kw)
+
+
+@gpu
 @pytest.mark.parametrize("lq", [[24, 33], [1, 1]])
 @pytest.mark.parametrize("heads,kv,d", PART_SHAPES)
 def test_parts_of_unlike_values(be, orc, heads, kv, d, lq):
