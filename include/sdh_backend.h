@@ -154,7 +154,8 @@ int sdh_linear_swiglu(const float* x, const uint16_t* w1, const uint16_t* w3, fl
  * of B_a from there on are not read as numbers). A run with no such adapter (-1) or rank 0 adds
  * nothing: its rows are left, or zero without accumulate. Runs must not share
  * rows; entries past the matrix are cut to it; rows of no run are left as they
- * were. Everything is held in fp32, X unrounded. C must not overlap an input.
+ * were. Everything is held in fp32, X unrounded; infinities in X and A give what
+ * fp32 sums give, in B they give NaN. C must not overlap an input.
  * H = X A_a^T goes through scratch (not for few rows and K to 640). */
 int sdh_lora_nt_bf16(int64_t M, int64_t N, int64_t K, const float* X, int64_t ldx, const uint16_t* A,
                      const uint16_t* B, int64_t rank, int64_t adapters, const float* scale, const int32_t* segments,

@@ -9,7 +9,8 @@
 // so nothing overflows and the range is fp32's), a bf16 value its own; the products of the
 // parts are exact in the fp32 accumulators. X keeps its 24 bits, unlike the A of
 // gemm_nt_bf16. With fp32 weights the product of the two smallest parts (below 2^-28) is
-// left out.
+// left out. An infinity has no such parts (inf - inf): sums of H that come out not finite are
+// formed again from X and A as they are, and what such rows of H add to C in fp32.
 //
 // Bound by memory for many rows: X is read once (a workgroup has all ranks of its rows), C
 // read and written once, while A, B and H come from the L2s. [12528,3840] bf16 to 10240
@@ -105,6 +106,9 @@ struct Eight<u16> {
     }
     __device__ __forceinline__ void parts(bf16x8* out) const { out[0] = __builtin_bit_cast(bf16x8, a); }
 };
+__device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
+__device__ __forceinline__ float value(float x) { return x; }
+__device__ __forceinline__ float value(u16 x) { return __uint_as_float((unsigned)x << 16); }
 template <int PA, int PB>
 __device__ __forceinline__ f32x16 multiply(const bf16x8* a, const bf16x8* b, f32x16 c) {
     // the smallest products first
@@ -290,6 +294,18 @@ __device__ __forceinline__ void down_sums(const Lora& P, const dev::SpanTile& t,
     }
 }
 
+// One of those sums, over the blocks of a part of K, in fp32.
+template <class TX, class TW>
+__device__ __forceinline__ float plain_sum(const Lora& P, const dev::SpanTile& t, int adapter, int row, int j, int part, int parts) {
+    constexpr int STEP = kDownBlock<TX> * kLoraWaves;
+    const TX* x = (const TX*)P.x + (t.first + t.row0 + row) * P.ldx;
+    const TW* a = (const TW*)P.a + ((int64_t)adapter * P.rank + j) * P.K;
+    float sum = 0.f;
+    for (int64_t k0 = part * STEP; k0 < P.K; k0 += STEP * parts)
+        for (int64_t k = k0, end = min(k0 + STEP, (int64_t)P.K); k < end && sum == sum; ++k) sum = fmaf(value(x[k]), value(a[k]), sum);
+    return sum;
+}
+
 template <class TX, class TW, int RT, int RF, int MODE>
 __global__ __launch_bounds__(kLoraThreads) void k_lora_down(Lora P) {
     __shared__ __attribute__((aligned(16))) float part[kLoraWaves][RF * 32][33];
@@ -313,16 +329,38 @@ __global__ __launch_bounds__(kLoraThreads) void k_lora_down(Lora P) {
         __syncthreads();
         for (int i = threadIdx.x; i < RF * 1024; i += kLoraThreads) {
             const int row = i >> 5, c = i & 31, at = j0 + j * 32 + c;
-            const float v = (part[0][row][c] + part[1][row][c]) + (part[2][row][c] + part[3][row][c]);
+            float v = (part[0][row][c] + part[1][row][c]) + (part[2][row][c] + part[3][row][c]);
+            if (!finite(v) && row < left && at < rank) v = plain_sum<TX, TW>(P, t, adapter, row, at, blockIdx.y, P.splits);
             if (row < left && at < P.hrank) h[(int64_t)row * P.hrank + at] = at < rank ? v * f : 0.f;
         }
         __syncthreads();
     }
 }
 
-// A row's share of H (eight ranks of each step of 16 from j0 on), its parts of K summed, as MFMA operands.
+// A row's share of H (eight ranks of each step of 16) as MFMA operands. Returns which of a wave's 32 rows have a value
+// that is not finite: zeros here, for plain_columns.
 template <int KS>
-__device__ __forceinline__ void parts_of_h(const Lora& P, int64_t row, int j0, int rank, int fh, bf16x8 (&hp)[KS][3]) {
+__device__ __forceinline__ unsigned operands_of_h(Eight<float> (&v)[KS], bf16x8 (&hp)[KS][3]) {
+    float odd = 0.f;  // NaN then
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) odd = fmaf(v[ks].a[e], 0.f, fmaf(v[ks].b[e], 0.f, odd));
+    const unsigned long long m = __ballot(odd != 0.f);
+    const unsigned rows = (unsigned)m | (unsigned)(m >> 32);
+    if (rows) {
+        const int n = rows >> (threadIdx.x & 31) & 1 ? 0 : 8;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) v[ks].cut(n);
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) v[ks].parts(hp[ks]);
+    return rows;
+}
+
+// The same from scratch, from j0 on, its parts of K summed.
+template <int KS>
+__device__ __forceinline__ unsigned parts_of_h(const Lora& P, int64_t row, int j0, int rank, int fh, bf16x8 (&hp)[KS][3]) {
     constexpr int AHEAD = KS >= 8 ? 1 : KS >= 4 ? 2 : 4;  // parts asked for at once
     const float* h = P.h + row * P.hrank + j0 + fh * 8;
     const int64_t next = (int64_t)P.M * P.hrank;
@@ -346,8 +384,37 @@ __device__ __forceinline__ void parts_of_h(const Lora& P, int64_t row, int j0, i
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) v[ks].a += x[u][ks][0], v[ks].b += x[u][ks][1];
     }
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) v[ks].parts(hp[ks]);
+    return operands_of_h<KS>(v, hp);
+}
+
+// A bit for each of the first `left` of 32 rows.
+__device__ __forceinline__ unsigned rows_of(int left) { return left >= 32 ? ~0u : (1u << max(left, 0)) - 1u; }
+
+// What the values of H at the ranks j0 .. j1 add to the columns n .. n1 of `rows` of the 32 from `first` on, in fp32, behind
+// a wave's other work on them; h: H's rows, or null for those in scratch. Each lane takes the places of C that it has itself
+// written there. A call, and P by the address of the kernel's arguments: inside the kernels it cost their loops 30 registers.
+typedef const __attribute__((address_space(4))) Lora* LoraArgs;
+__device__ __forceinline__ LoraArgs lora_args() { return (LoraArgs)__builtin_amdgcn_kernarg_segment_ptr(); }  // a kernel's first argument
+template <class TW>
+__device__ __attribute__((noinline)) void plain_columns(LoraArgs P, int adapter, int j0, int j1, unsigned rows, int64_t first, int n, int n1, const float* h,
+                                                        int ldh) {
+    const TW* b = (const TW*)P->b + (int64_t)adapter * P->N * P->rank;
+    for (; rows; rows &= rows - 1) {
+        const int row = __ffs(rows) - 1;
+        if ((row >> 2 & 1) != (int)(threadIdx.x >> 5 & 1)) continue;
+        for (int n0 = n; n0 < n1; n0 += 128)
+            for (int col = n0 + (threadIdx.x & 31) * 4, end = min(col + 4, P->N); col < end; ++col) {
+                float sum = 0.f;
+                for (int r = j0; r < j1 && sum == sum; ++r) {
+                    float x = 0.f;
+                    if (h) x = h[row * ldh + r];
+                    else
+                        for (int s = 0; s < P->splits; ++s) x += P->h[((int64_t)s * P->M + first + row) * P->hrank + r];
+                    sum = fmaf(x, value(b[(int64_t)col * P->rank + r]), sum);
+                }
+                P->c[(first + row) * P->ldc + col] += sum;
+            }
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -444,7 +511,7 @@ __device__ __forceinline__ void up_columns(const Lora& P, int adapter, int rank,
 template <class TW, int KS, bool FEW, bool VEC, bool CV>
 __global__ __launch_bounds__(kLoraThreads, KS <= 4 ? 2 : 1) void k_lora_up(Lora P, int j0, int columns) {
     __shared__ __attribute__((aligned(16))) char lds[VEC ? kLoraWaves : 1][4096];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, fr = lane & 31, fh = lane >> 5;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 31, fh = lane >> 5;
     dev::SpanTile t;
     if (!dev::find_tile(P.runs, P.count, P.M, 1, FEW ? 32 : 32 * kLoraWaves, blockIdx.x, t)) return;
     int rank;
@@ -459,8 +526,9 @@ __global__ __launch_bounds__(kLoraThreads, KS <= 4 ? 2 : 1) void k_lora_up(Lora 
         return;
     }
     bf16x8 hp[KS][3];
-    parts_of_h<KS>(P, first + min(fr, left - 1), j0, rank, fh, hp);
+    const unsigned odd = parts_of_h<KS>(P, first + min(fr, left - 1), j0, rank, fh, hp) & rows_of(left);
     up_columns<TW, KS, VEC, CV>(P, adapter, rank, j0, hp, n, n1, c, left, lds[VEC ? w : 0]);
+    if (odd) plain_columns<TW>(lora_args(), adapter, j0, min(rank, j0 + KS * 16), odd, first, n, n1, nullptr, 0);
 }
 
 // Both in one launch, for few rows a run and a short K: every workgroup of a run forms H for
@@ -471,7 +539,7 @@ __global__ __launch_bounds__(kLoraThreads, 2) void k_lora_small(Lora P, int colu
     constexpr int RT = (KS + 1) / 2;
     __shared__ __attribute__((aligned(16))) float part[kLoraWaves][32][33];
     __shared__ __attribute__((aligned(16))) float h[32][RT * 32 + 4];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, fr = lane & 31, fh = lane >> 5;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 31, fh = lane >> 5;
     dev::SpanTile t;
     if (!dev::find_tile(P.runs, P.count, P.M, 1, 32, blockIdx.x, t)) return;
     int rank;
@@ -493,20 +561,22 @@ __global__ __launch_bounds__(kLoraThreads, 2) void k_lora_small(Lora P, int colu
         __syncthreads();
         for (int i = threadIdx.x; i < 1024; i += kLoraThreads) {
             const int row = i >> 5, col = i & 31;
-            const float v = (part[0][row][col] + part[1][row][col]) + (part[2][row][col] + part[3][row][col]);
+            float v = (part[0][row][col] + part[1][row][col]) + (part[2][row][col] + part[3][row][col]);
+            if (!finite(v) && row < left && j * 32 + col < rank) v = plain_sum<TX, TW>(P, t, adapter, row, j * 32 + col, 0, 1);
             h[row][j * 32 + col] = j * 32 + col < rank ? v * f : 0.f;
         }
         __syncthreads();
     }
     bf16x8 hp[KS][3];
+    Eight<float> v[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-        Eight<float> v;
-        v.a = *(const f4*)&h[fr][ks * 16 + fh * 8];
-        v.b = *(const f4*)&h[fr][ks * 16 + fh * 8 + 4];
-        v.parts(hp[ks]);
+        v[ks].a = *(const f4*)&h[fr][ks * 16 + fh * 8];
+        v[ks].b = *(const f4*)&h[fr][ks * 16 + fh * 8 + 4];
     }
+    const unsigned odd = operands_of_h<KS>(v, hp) & rows_of(left);
     up_columns<TW, KS, VEC, CV>(P, adapter, rank, 0, hp, n, n1, c, left, (char*)part[w]);
+    if (odd) plain_columns<TW>(lora_args(), adapter, 0, rank, odd, t.first + t.row0, n, n1, &h[0][0], RT * 32 + 4);
 }
 
 // Up for runs of many rows: the waves of a workgroup have neighbouring rows and share
@@ -561,7 +631,7 @@ __global__ __launch_bounds__(kLoraThreads, KS <= 4 ? 2 : 1) void k_lora_up_share
     };
     copy(n0, stage0);
     bf16x8 hp[KS][3];
-    parts_of_h<KS>(P, t.first + min(row0 + fr, t.rows - 1), j0, rank, fh, hp);
+    const unsigned odd = parts_of_h<KS>(P, t.first + min(row0 + fr, t.rows - 1), j0, rank, fh, hp) & rows_of(left);
     auto landed = [] { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
     landed();
     auto step = [&](int n, const char* from, char* to) __attribute__((always_inline)) {
@@ -617,6 +687,7 @@ __global__ __launch_bounds__(kLoraThreads, KS <= 4 ? 2 : 1) void k_lora_up_share
         step(n, stage0, stage1);
         if (n + 128 < n1) step(n + 128, stage1, stage0);
     }
+    if (odd) plain_columns<TW>(lora_args(), adapter, j0, min(rank, j0 + KS * 16), odd, first, n0, n1, nullptr, 0);
 }
 
 template <class TX, class TW>
