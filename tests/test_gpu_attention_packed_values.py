@@ -265,3 +265,43 @@ def test_parts_that_a_bias_hides(be, orc, lq, bad):
     c.v[3000:3000 + 3000] = bad
     held(c, be, orc, f"{bad}", bias=bias, radius=2500)
     held(c, be, orc, f"{bad} window", bias=bias, radius=2500, causal=True, window=2000)
+
+
+# ------------------------------------------------- tiles that wait, among many that do not
+@gpu
+@pytest.mark.parametrize("kw", [{}, {"causal": True}, {"causal": True, "window": 300, "prefix": 70, "cap": 20.0}], ids=str)
+@pytest.mark.parametrize("heads,kv,d", [(4, 2, 128), (2, 2, 64), (2, 1, 72)])
+def test_odd_tiles_among_others(be, orc, heads, kv, d, kw):
+    """Keys and values of unlike size, rows of zeros, keys that are not finite and infinite values in some tiles of
+    sequences of several workgroups, checked at rows of each."""
+    lens = [700, 130, 1000]
+    c = Case(orc, lens, lens, heads, kv, d, seed=3200, gap=3)
+    first = c.spans[:, 2]
+    c.k[first[0] + 70] *= np.float32(2.0 ** 14)     # the second tile
+    c.v[first[0] + 200] *= np.float32(2.0 ** -20)   # the fourth
+    c.v[first[0] + 390:first[0] + 400] = 0.0        # the seventh
+    c.v[first[1]] *= np.float32(1e-6)               # a first key that gives next to nothing
+    c.q[:, 3::d] = np.abs(c.q[:, 3::d]) + 0.25
+    c.k[first[2] + 500, 3] = -np.inf
+    c.k[first[2] + 640, d * (kv - 1) + 5] = np.nan  # rows that see it are NaN, in their heads
+    c.v[first[2] + 333, 7] = np.inf
+    c.q[first[2] + 900] = 0.0                       # a zero query: 0 * inf
+    pre = kw.get("prefix")
+    kw = dict(kw, prefix=np.array([pre, 0, pre + 30], np.int32)) if pre else kw
+    got = c.run(be, **kw)
+    for s, n in enumerate(lens):
+        for i in sorted({0, 1, 31, 32, 63, 64, 127, 128, 255, 256, 333, 334, 390, 499, 500, 639, 640, 699, 900, n // 2, n - 1} & set(range(n))):
+            one = dict(kw, prefix=kw["prefix"][s:s + 1]) if pre else kw
+            row = first[s] + i
+            # the row alone, with the keys up to its own place or, not causal, all of its sequence's
+            keys = i + 1 if kw.get("causal") else n
+            if pre and keys < one["prefix"][0]:
+                continue  # it sees keys behind its place, which a row alone cannot
+            want, tol = orc.attention_packed(c.q[row:row + 1], c.k, c.v, np.zeros((1, heads * d)), [(0, 1, first[s], keys)], heads, kv,
+                                             c.scale, **one)
+            fin = np.isfinite(want[0])
+            assert np.array_equal(np.isnan(got[row]), np.isnan(want[0])), (s, i)
+            assert np.array_equal(got[row][np.isinf(want[0])], want[0][np.isinf(want[0])]), (s, i)
+            assert np.all(np.abs(got[row][fin] - want[0][fin]) <= tol[0][fin]), (s, i)
+    again = c.run(be, **kw)
+    assert np.array_equal(got.view(np.uint32), again.view(np.uint32))
