@@ -322,24 +322,31 @@ __global__ __launch_bounds__(64 * kSplitWaves) void k_attn_packed_split(Packed P
             for (int u = 0; u < VU; ++u) vx[i][u] = a[min(lane * VU + u, d - 1)];
         }
     }
-    bool read = false;
-    for (int s0 = 0; s0 < P.seqs && !read; s0 += 64) {
+    // The tile's rows that sequences read. What the others hold does not matter, and is not to cost them anything: behind the
+    // sequences in their slots a cache may have zeros, or anything.
+    unsigned long long used = 0;
+    for (int s0 = 0; s0 < P.seqs && ~used; s0 += 64) {
         int4 e = make_int4(0, 0, 0, 0);
         if (s0 + lane < P.seqs) {
             e = P.spans[s0 + lane];
             dev::cut_span(e.z, e.w, P.Tk);
         }
-        read = __ballot(e.y > 0 && e.w > 0 && e.z < tile * kKT + kKT && e.z + e.w > tile * kKT) != 0;
+        const int from = max(e.z - tile * kKT, 0), to = min(e.z + e.w - tile * kKT, kKT);
+        for (unsigned long long m = __ballot(e.y > 0 && from < to); m && ~used; m &= m - 1) {
+            const int at = (int)__ffsll(m) - 1, lo = __builtin_amdgcn_readlane(from, at), hi = __builtin_amdgcn_readlane(to, at);
+            used |= ~0ull >> (kKT - (hi - lo)) << lo;
+        }
     }
-    if (!read) return;
-    // a key's largest magnitudes, rows past the tensor and columns past d zero, and what is not finite
+    if (!used) return;
+    const unsigned mine = (unsigned)(used >> (w * 16)) & 0xFFFFu;
+    // a key's largest magnitudes, rows of no sequence and columns past d zero, and what is not finite
     int ktop[KU], vtop[16], kmost = 0, vmost = 0, flag = 0;
 #pragma unroll
     for (int u = 0; u < KU; ++u) {
         ktop[u] = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            if (j0 + u * KROWS + krow >= P.Tk || kch * 8 + e >= d) kx[u][e] = 0.f;
+            if (!(mine >> (u * KROWS + krow) & 1) || kch * 8 + e >= d) kx[u][e] = 0.f;
             ktop[u] = max(ktop[u], abs_bits(kx[u][e]));
         }
         ktop[u] = group_imax<KCH>(ktop[u]);
@@ -350,7 +357,7 @@ __global__ __launch_bounds__(64 * kSplitWaves) void k_attn_packed_split(Packed P
         vtop[i] = 0;
 #pragma unroll
         for (int u = 0; u < VU; ++u) {
-            if (j0 + i >= P.Tk || lane * VU + u >= d) vx[i][u] = 0.f;
+            if (!(mine >> i & 1) || lane * VU + u >= d) vx[i][u] = 0.f;
             if (abs_bits(vx[i][u]) >= kInfBits) vx[i][u] = 0.f, flag = kNotFinite;
             vtop[i] = max(vtop[i], abs_bits(vx[i][u]));
         }
@@ -372,7 +379,7 @@ __global__ __launch_bounds__(64 * kSplitWaves) void k_attn_packed_split(Packed P
         if (ktop[u] >= kInfBits || (ktop[u] && abs((kmost >> 23) - (ktop[u] >> 23)) > kSpread)) flag |= kKeyExps;
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-        if (j0 + i < P.Tk && (vmost >> 23) - (vtop[i] >> 23) > kSpread) flag |= kValueExps;
+        if ((mine >> i & 1) && (vmost >> 23) - (vtop[i] >> 23) > kSpread) flag |= kValueExps;
     flag = (__ballot(flag & kKeyExps) ? kKeyExps : 0) | (__ballot(flag & kValueExps) ? kValueExps : 0) | (__ballot(flag & kNotFinite) ? kNotFinite : 0);
     if (lane == 0) flags[w] = flag;
     __syncthreads();
