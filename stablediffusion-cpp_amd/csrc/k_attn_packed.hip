@@ -219,6 +219,7 @@ constexpr int kKT = 64, kSplitWaves = 4;
 // The reference m of the weights is raised when a tile's largest score passes it by more
 // than this (in units of log2): weights stay below 2^(14 + kLazy), inside fp16.
 constexpr float kLazy = 1.5f;
+constexpr float kFarRef = 1e4f;  // rounded by less than 2^-10
 // The bias of a head in LDS goes on at both ends with its end values, as far as a wave's 32 rows and a
 // tile's 64 keys reach past the radius unless all of them are beyond it: no index is held to the radius
 // (ten instructions a score; the rows and tiles at the band's edges took half the softmax' time).
@@ -834,11 +835,14 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
         }
         const int above = tile_ev - E, by = 14 + (own ? above : max(above, kFarE));
         float weights = 0.f;
-        // A reference far out (biases of the type's lowest value) is taken off before the product,
-        // which would overflow.
-        if (EXTRA && !own && __ballot(!(fabsf(ref) < 1e4f))) {
+        // A reference far out (biases of the type's lowest value, for one) is taken off before the product, which could overflow.
+        // It was rounded, as the scores here are not: their weights are held to what the others may reach.
+        if (!own && __ballot(!(fabsf(ref) < kFarRef))) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) s[i >> 4][i & 15] = __builtin_amdgcn_exp2f(fmaf(fmaf(s[i >> 4][i & 15], unit, -ref), kLog2e, (float)by));
+            for (int i = 0; i < 32; ++i) {
+                const float x = fmaf(s[i >> 4][i & 15], unit, -ref) * (EXTRA ? kLog2e : 1.0f);
+                s[i >> 4][i & 15] = __builtin_amdgcn_exp2f((x > kLazy ? kLazy : x) + (float)by);  // NaN stays
+            }
         } else {
             const float up = (float)by - off;
 #pragma unroll

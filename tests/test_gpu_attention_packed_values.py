@@ -189,6 +189,19 @@ def test_unlike_channels(be, orc, lq, d, power):
             held(c, be, orc, f"{which} {meets} cap and bias", cap=4.0, bias=orc.randn((2, 61), 2801), radius=30, causal=True)
 
 
+@gpu
+@pytest.mark.parametrize("lq,d", SHAPES)
+def test_keys_far_above_the_others(be, orc, lq, d):
+    """One in each tile, with the others' values or with few."""
+    for up in (1e4, 1e8):
+        c = Case(orc, lq, [150], 2, 1, d, seed=2850)
+        c.k[::64] *= np.float32(up)
+        held(c, be, orc, f"{up}")
+        held(c, be, orc, f"{up} causal", causal=True)
+        c.k[::64, : d // 2] *= np.float32(1 / up)
+        held(c, be, orc, f"{up} half")
+
+
 # --------------------------------------------------------------- keys cut into parts
 def parts_of_tiles(c, cus=256):
     """How many parts the dispatch cuts the keys into: those that fill the chip, of 512 keys of an average sequence at least."""
