@@ -191,8 +191,9 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_attn_packed_rows(Packed P) {
 // inf - inf in a pair: a wave one of whose rows sees such a key, or has such a query, takes the
 // tile's scores in fp32 (fp32_scores). So it does where values far below their block's largest, whose pairs are
 // off by up to 2^-25, could move a score by more than 2^-21: by 2^-25 (sum|q| + sum|k|) of the scaled values
-// in units of 2^(e_q + e_k) scale. Heads of 128 whose largest q and k meet at scores of 2^15 are far from that;
-// a channel of q or k that is 2^12 above the others is not.
+// in units of 2^(e_q + e_k) scale, or, where that says so, by how many such values there are against a largest of 2^14.
+// Heads of 128 whose largest q and k meet at scores of 2^15 are far from that; a channel of q or k that is 2^12 above
+// the others is not.
 //
 // S^T = K Q^T and O^T = V^T P^T by v_mfma_f32_32x32x16_f16: lane l holds row l % 32 of
 // the wave in both, its statistics are its own. K's rows are ordered so that the eight
@@ -225,6 +226,7 @@ constexpr float kFarRef = 1e4f;  // rounded by less than 2^-10
 // (ten instructions a score; the rows and tiles at the band's edges took half the softmax' time).
 constexpr int kBiasPad = 96;
 constexpr float kMostLost = 16.0f;  // 2^25 times 2^-21
+constexpr int kInfinite = 1 << 16;  // values that are not finite, in a count of others
 constexpr int kBadKey = 1000;   // the exponent of a key that is not finite
 constexpr int kUnsetE = -2000;  // no weighted values yet, or next to nothing beside the reference
 constexpr int kSpread = 8;
@@ -673,6 +675,24 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
             }
         }
     };
+    // How many values of a row of q, and of a key of the tile in kbuf, at most have pairs of fewer than 22 bits, down to none; a
+    // query that is not finite counts kInfinite. For tiles that may lose some by their sums of magnitudes.
+    auto few_bits = [&](const u16* kbuf) __attribute__((always_inline)) {
+        auto lost = [](unsigned hi) {  // of two values
+            const unsigned a = hi & 0x7FFFu, b = hi >> 16 & 0x7FFFu;
+            return (int)(a < 0x3000u) + (int)(b < 0x3000u) + ((a >= 0x7C00u) + (b >= 0x7C00u)) * kInfinite;
+        };
+        auto of_row = [&](int n) { return n == DP ? 0 : n - (DP - P.d); };  // rows of zeros lose nothing, nor do the columns past d
+        int nq = 0, nk = 0;
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) nq += lost(__builtin_bit_cast(unsigned, h2{qh[ds][e], qh[ds][e + 1]}));
+#pragma unroll 1
+        for (int i = 0; i < DP / 2; ++i)  // a key a lane, from a bank each
+            nk += lost(((const unsigned*)kbuf)[lane * (DP / 2) + ((i + lane) & (DP / 2 - 1))]) % kInfinite;
+        return group_imax<64>(of_row(nq + __shfl_xor(nq, 32, 64))) + group_imax<64>(of_row(nk));
+    };
     f2 q_most = {0.f, 0.f};  // of the workgroup's rows, as q_waves
     auto loses = [&](int ek, float ksum) { return !(ldexpf(scale * fmaf(q_most[0], ksum, q_most[1]), ek) <= kMostLost); };
     // s -> weights in place, the statistics and the scale of o brought up to date. k0: the
@@ -702,8 +722,11 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
         // kept normal: -inf stays -inf, zero zero
         float unit = fminf(fmaxf(ldexpf(scale, eq + ek), 1.17549435e-38f), 3.40282347e38f);  // of s
         if (ODD && __ballot(ek == kBadKey || loses(ek, ksum))) {
-            fp32_scores(k0);
-            unit = EXTRA ? 1.0f : kLog2e;
+            const int n = few_bits(kbuf0);
+            if (n >= kInfinite || __ballot(ek == kBadKey || !(unit * (float)n <= kMostLost * 0x1p-14f))) {
+                fp32_scores(k0);
+                unit = EXTRA ? 1.0f : kLog2e;
+            }
         }
         if constexpr (EXTRA) {
             const float* near = biases + (h - kh * group) * row_of_bias + kBiasPad + P.radius;
