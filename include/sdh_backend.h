@@ -312,14 +312,20 @@ int sdh_attention_fp16(const float* q, const float* k, const float* v, void* out
  * 0 or |p - j| < window). prefix [seqs] int32 on the device, or NULL for none.
  *   Scores: scale * q.k; with cap > 0 then cap * tanh(score / cap); with bias
  * [heads, 2 radius + 1] then + bias[h, clamp(j - p, -radius, radius) + radius]
- * (-inf hides a key). A query that sees no key gives zeros. Keys that a query
- * does not see do not change its result, whatever their values are.
+ * (-inf hides a key). A query that sees no key gives zeros. What a query does not
+ * see does not change its result, whatever it holds; nor does a key whose score is
+ * -inf (an infinity in q or k). A score that is NaN or +inf makes its query's
+ * results NaN; infinities and NaN among the values of the other keys show in their
+ * columns, however small the weight. Up to 128 dims values are held to 2^-30 of
+ * their key's largest and weighted ones to 2^-27 of the largest weighted one; all
+ * else is as close as fp32 sums are.
  *   out must not overlap an input. The arrays are read when the work runs, so a
  * captured graph takes the spans that they hold at each replay. Where no scratch
  * can be had (a full arena; a capture that asks for more than any call before it)
- * a slower kernel gives the same result. The kernel is chosen by Tq, Tk and seqs:
- * single tokens against long caches are best not mixed with long prompts in a
- * call. */
+ * a slower kernel gives the same result. The kernel is chosen by Tq, Tk and seqs
+ * (entries without rows count): single tokens against long caches are best not
+ * mixed with long prompts in a call. For prompts scratch is about as large as k and
+ * v with heads of the next 64 or 128 dims, whatever of them the sequences read. */
 int sdh_attention_packed(const float* q, const float* k, const float* v, void* out, int out_bf16, int64_t Tq,
                          int64_t Tk, int heads, int kv_heads, int64_t d, const int32_t* spans, int64_t seqs,
                          float scale, int causal, int64_t window, const int32_t* prefix, float cap,

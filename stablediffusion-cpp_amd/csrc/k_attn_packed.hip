@@ -184,16 +184,18 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_attn_packed_rows(Packed P) {
 // the row's reference, with which E sinks as the reference rises. A value that is large but
 // has no weight, hidden or far below in score, then costs the others nothing, and the largest
 // that has weight is near 2^28 in its sum. A tile whose values are more than 2^kSpread apart, or
-// have rows of zeros among them, has an exponent for each key: p 2^e_v of the tile says nothing
-// there about any one key. (Of its keys as well, whose largest need not be one that a row sees.)
-// Values that are not finite go into the tiles as zeros, since 0 * inf would reach
-// the rows that do not see them, and are added at the end. An infinity in q or k would be
-// inf - inf in a pair: a wave one of whose rows sees such a key, or has such a query, takes the
-// tile's scores in fp32 (fp32_scores). So it does where values far below their block's largest, whose pairs are
-// off by up to 2^-25, could move a score by more than 2^-21: by 2^-25 (sum|q| + sum|k|) of the scaled values
-// in units of 2^(e_q + e_k) scale, or, where that says so, by how many such values there are against a largest of 2^14.
-// Heads of 128 whose largest q and k meet at scores of 2^15 are far from that; a channel of q or k that is 2^12 above
-// the others is not.
+// that has rows of zeros among them, has an exponent for each key: p 2^e_v of the tile says
+// nothing there about any one key. So it has for keys that far apart, whose largest need not be
+// one that a row sees. Rows that no sequence reads are zeros that do not count.
+//   Values that are not finite go into the tiles as zeros, since 0 * inf would reach the rows
+// that do not see them, and are added at the end. An infinity in q or k would be inf - inf in a
+// pair: a wave one of whose rows sees such a key, or has such a query, takes the tile's scores
+// in fp32 (fp32_scores). So it does where values far below their block's largest, whose pairs
+// are off by up to 2^-25, could move a score by more than 2^-21: by 2^-25 (sum|q| + sum|k|) of
+// the scaled values in units of 2^(e_q + e_k) scale, and, where that says so, by how many such
+// values there are against a largest of 2^14. Heads of 128 whose largest q and k meet at scores
+// of 2^15 are far from that; a channel of q or k that is 2^12 above the others is not. Such
+// tiles, and those with exponents of their keys, go through a second loop, one at a time.
 //
 // S^T = K Q^T and O^T = V^T P^T by v_mfma_f32_32x32x16_f16: lane l holds row l % 32 of
 // the wave in both, its statistics are its own. K's rows are ordered so that the eight
@@ -201,9 +203,10 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_attn_packed_rows(Packed P) {
 // are the second product's operand as they lie, V^T in the keys' own order.
 //
 // Long sequences are bound by the three products: two images of 4200 rows, 30 heads of 128,
-// 1.42 ms, 377 TFLOP/s of 4 d a visible pair, as k_attention.hip's kernel on that shape; the split 0.1
+// 1.45 ms, 369 TFLOP/s of 4 d a visible pair, near k_attention.hip's kernel on that shape; the split 0.1
 // ms of it. Short ones by their workgroups' starts (the list, q): 24 prompts of up to 203
-// rows, 32/8 heads of 128, 61 us, 16 of them their bytes at the rate of a copy.
+// rows, 32/8 heads of 128, 63 us, 16 of them their bytes at the rate of a copy. The rules for
+// unlike and infinite values cost 1 % of the former and 2 to 3 % of the latter.
 // ---------------------------------------------------------------------------
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
