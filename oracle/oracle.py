@@ -398,7 +398,7 @@ class Oracle:
     def attention_packed(self, q, k, v, out, spans, heads, kv_heads, scale, causal=False, window=0, prefix=None,
                          cap=0.0, bias=None, radius=0):
         """float64 definition of sdh_attention_packed. Returns the result (rows of no
-        sequence as in `out`) and a bound for its fp32 evaluation, per value.
+        sequence as in `out`) and a bound for its evaluation, per value.
 
         A bias of -inf hides its key, and a key whose score is -inf (an infinity in q or
         k) has no weight: neither counts, whatever it holds. A score that is NaN or +inf
