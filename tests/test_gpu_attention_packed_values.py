@@ -318,3 +318,39 @@ def test_odd_tiles_among_others(be, orc, heads, kv, d, kw):
             assert np.all(np.abs(got[row][fin] - want[0][fin]) <= tol[0][fin]), (s, i)
     again = c.run(be, **kw)
     assert np.array_equal(got.view(np.uint32), again.view(np.uint32))
+
+
+@gpu
+@pytest.mark.parametrize("lq,lk", [([30, 260], [150, 260]), ([1, 1], [500, 2000]), ([24, 33], [3000, 4500])])
+def test_captured_with_unlike_values(be, orc, lq, lk):
+    """Replayed with values that send other tiles to the second loop, the direct call between the replays."""
+    c = Case(orc, lq, lk, 4, 1, 128, seed=3300)
+    q, k, v, out, spans = be.array(c.q), be.array(c.k), be.array(c.v), be.empty(c.q.shape), be.rows_list(c.spans)
+
+    def call():
+        be.attention_packed(q, k, v, out, c.Tq, c.Tk, 4, 1, 128, spans, 2, c.scale, causal=True)
+
+    call()
+    be.capture_begin()
+    call()
+    g = be.capture_end()
+    try:
+        for rep in range(4):
+            hk, hv = c.k.copy(), c.v.copy()
+            hv[rep * 30 + 5] *= np.float32(1e-5)
+            hk[rep * 20 + 3] *= np.float32(1e5)
+            if rep % 2:
+                hv[7, 3], hk[lk[0] + 100, 2] = np.inf, np.nan
+            k.upload(hk)
+            v.upload(hv)
+            be.call("sdh_zero", out.ptr, out.nbytes)
+            be.graph_launch(g)
+            got = out.download()
+            want, tol = orc.attention_packed(c.q, hk, hv, np.zeros(c.q.shape), c.spans, 4, 1, c.scale, causal=True)
+            fin = np.isfinite(want)
+            assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got[np.isinf(want)], want[np.isinf(want)]), rep
+            assert np.all(np.abs(got[fin] - want[fin]) <= tol[fin]), rep
+            call()
+            assert np.array_equal(out.download().view(np.uint32), got.view(np.uint32)), rep
+    finally:
+        be.graph_destroy(g)

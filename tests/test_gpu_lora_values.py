@@ -123,3 +123,36 @@ def test_offsets_past_32_bits(be, orc, types, M, N, K, rank):
     want, tol = orc.lora(c.x, c.A[1:], c.B[1:], None, [(0, M, 0, rank)], c.c0, True)
     assert np.all(np.abs(C.download() - want) <= tol)
     [f.free() for f in far]
+
+
+@gpu
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("rows,K", [([200, 100], 256), ([1, 1, 1], 256), ([1, 1, 1], 1280)])
+def test_captured_with_infinities(be, orc, types, rows, K):
+    """Replayed with an infinity in another row each time, the direct call between the replays."""
+    c = Case(orc, sum(rows), 300, K, 16, 3, types, seed=1600)
+    runs = np.array(ragged(rows, 3, 16), np.int32)
+    X, A, B, scale = c.device(be)
+    C, seg = be.array(c.c0), be.rows_list(runs)
+    c.call(be, X, A, B, scale, seg, len(rows), C, True)
+    be.capture_begin()
+    c.call(be, X, A, B, scale, seg, len(rows), C, True)
+    g = be.capture_end()
+    clean = c.x.copy()
+    try:
+        for rep in range(4):
+            c.x = clean.copy()
+            c.x[rep * 7 % len(c.x), 5] = np.inf if rep else 1.0
+            X.upload(f32_to_bf16(c.x) if types.startswith("bf16") else c.x)
+            C.upload(c.c0)
+            be.graph_launch(g)
+            got = C.download()
+            with np.errstate(invalid="ignore"):
+                want, tol = orc.lora(c.x, c.A, c.B, c.scale, runs, c.c0, True)
+            fin = np.isfinite(want)
+            assert np.array_equal(np.isfinite(got), fin) and np.all(np.abs(got[fin] - want[fin]) <= tol[fin]), rep
+            C.upload(c.c0)
+            c.call(be, X, A, B, scale, seg, len(rows), C, True)
+            assert np.array_equal(C.download().view(np.uint32), got.view(np.uint32)), rep
+    finally:
+        be.graph_destroy(g)
