@@ -653,7 +653,7 @@ __global__ __launch_bounds__(64 * kWaves<DP>, 2 / (kWaves<DP> / 4)) void k_attn_
         return EXTRA && R->bias && R->bias[(int64_t)h * (2 * R->radius + 1) + R->radius + min(max(j - p, -R->radius), R->radius)] == -INFINITY;
     };
     // s = scale q.k of a tile, whatever q and k hold, -inf where a bias hides the key. Eight keys at a time, in
-    // little code: it stands twice in a loop that is to stay in the instruction cache.
+    // little code and few registers.
     auto fp32_scores = [&](int k0) __attribute__((always_inline)) {
         const auto R = args();
         const int d = R->d;
